@@ -69,6 +69,12 @@ SIGNATURES = {
     "exl_silu_mul": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "exl_update_cache": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
     "exl_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "exl_paged_slots": (c_int, [c_void_p] * 6 + [c_int] * 8 + [c_void_p] * 5),
+    "exl_paged_append": (c_int, [c_void_p, c_void_p, C.c_long, C.c_long, c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 5 + [c_void_p] * 3 +
+                         [c_int, c_void_p]),
+    "exl_paged_attention_workspace": (c_size_t, [c_int] * 8),
+    "exl_paged_attention": (c_int, [c_void_p, C.c_long] + [c_void_p] * 3 + [c_int] * 3 + [c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 6 +
+                            [c_float, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "exl_q4_attn": (c_int, [c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                             c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
                             c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,

@@ -26,6 +26,10 @@ from ._lib import check
 none_tensor = torch.empty((1, 1), device="meta")
 
 
+# the 8-bit types a paged cache's pages can have -> include/exl_amd.h: EXL_PAGE_FP8, EXL_PAGE_INT8
+PAGE_CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
+
+
 def _is_none(t):
     return t is none_tensor or t is None or t.device.type == "meta"      # (identity first: the reference passes THE sentinel, 14 times per layer)
 
@@ -440,6 +444,122 @@ class _ExllamaExt:
                                           _ptr(mask), bsz, q_len, num_heads, kvh, hd, max_seq, int(past_len),
                                           _ptr(past_len_dev), _stream(q)), "attention")
 
+    # -- the paged 8-bit cache (include/exl_amd.h: exl_paged_slots, exl_paged_append, exl_paged_attention): no counterpart in exllama_ext
+    def paged_slots(self, past_lens, new_lens, held, block_table, ring, counters, block_size, rows, max_new=None, max_len=None, row_stride=0):
+        n = past_lens.numel()
+        for t, name, numel in ((past_lens, "past_lens", n), (new_lens, "new_lens", n), (held, "held", n), (counters, "counters", 4),
+                               (ring, "ring", None), (block_table, "block_table", None)):
+            _req_dtype(t, torch.int32, name)
+            _req_cuda(t, name)
+            _req(t.device == past_lens.device, f"{name} must be on the device of past_lens")
+            _req(numel is None or t.numel() == numel, f"{name} has the wrong size")
+        _req(block_table.dim() == 2 and block_table.size(0) == n, "block_table must be [rows of the batch, blocks]")
+        _req(rows >= 0, "rows must not be negative")
+        width = block_table.size(1)
+        buf = torch.empty(n + 1 + 2 * rows + 8 * n, dtype=torch.int32, device=past_lens.device)
+        starts, slots, positions = buf[:n + 1], buf[n + 1:n + 1 + rows], buf[n + 1 + rows:n + 1 + 2 * rows]
+        base = buf.data_ptr()
+        with _Guard(past_lens.device):
+            check(self._lib.exl_paged_slots(past_lens.data_ptr(), new_lens.data_ptr(), held.data_ptr(), block_table.data_ptr(), ring.data_ptr(),
+                                            counters.data_ptr(), n, width, int(block_size), ring.numel(),
+                                            width * int(block_size) if max_len is None else int(max_len), rows if max_new is None else int(max_new),
+                                            rows, int(row_stride), base, base + 4 * (n + 1), base + 4 * (n + 1 + rows),
+                                            base + 4 * (n + 1 + 2 * rows), _stream(past_lens)), "paged_slots")
+        return starts, slots, positions
+
+    @staticmethod
+    def _pages(key_pages, value_pages, key_scales, value_scales, head_dim):
+        """Checks the pool of pages; returns (code, blocks, kv_heads, block_size)."""
+        code = PAGE_CODES.get(key_pages.dtype)
+        _req(code is not None, "key_pages is incorrect datatype, must be torch.float8_e4m3fn or torch.int8")
+        _req_dtype(value_pages, key_pages.dtype, "value_pages")
+        _req(key_pages.dim() == 4 and value_pages.dim() == 4, "key_pages must be [blocks, kv_heads, block, hd16], value_pages [blocks, kv_heads, hd16, block]")
+        blocks, kvh, block, hd16 = key_pages.shape
+        _req(tuple(value_pages.shape) == (blocks, kvh, hd16, block), "value_pages must be [blocks, kv_heads, hd16, block] for key_pages [blocks, kv_heads, block, hd16]")
+        _req(hd16 == (head_dim + 15) // 16 * 16, f"pages hold {hd16} columns, head_dim {head_dim} needs {(head_dim + 15) // 16 * 16}")
+        for t, n in ((key_scales, "key_scales"), (value_scales, "value_scales")):
+            _req_dtype(t, torch.float32, n)
+            _req(tuple(t.shape) == (blocks, kvh), f"{n} must be [blocks, kv_heads]")
+        for t, n in ((key_pages, "key_pages"), (value_pages, "value_pages"), (key_scales, "key_scales"), (value_scales, "value_scales")):
+            _req_cuda(t, n)
+            _req(t.device == key_pages.device, f"{n} must be on the device of key_pages")
+        return code, blocks, kvh, block
+
+    @staticmethod
+    def _rows16(t, name, device):
+        """fp16 rows: the columns of a row next to each other, the rows any multiple of four elements apart.  Returns the row stride."""
+        _req_dtype(t, torch.float16, name)
+        _req(t.is_cuda, f"{name} must be on a HIP device (exllama_amd has no CPU path), got {t.device}")
+        _req(t.device == device, f"{name} must be on the device of the pages")
+        _req(t.dim() == 2 and t.stride(1) == 1, f"{name} must be [rows, width] with the columns of a row next to each other")
+        return t.stride(0) if t.size(0) > 1 else max(t.size(1), 4)
+
+    @staticmethod
+    def _angles(sin, cos, head_dim, device):
+        """Checks the rotation's tables (both or neither); returns (sin pointer, cos pointer, rows)."""
+        if _is_none(sin) and _is_none(cos):
+            return None, None, 0
+        _req(not _is_none(sin) and not _is_none(cos), "a rotation needs both sin and cos")
+        for t, n in ((sin, "sin"), (cos, "cos")):
+            _req_dtype(t, torch.float16, n)
+            _req_cuda(t, n)
+            _req(t.device == device, f"{n} must be on the device of the pages")
+            _req(t.size(-1) == head_dim, f"{n} table does not match head_dim")
+        _req(sin.numel() == cos.numel() and sin.numel() > 0, "sin and cos have incompatible shapes")
+        return sin.data_ptr(), cos.data_ptr(), sin.numel() // head_dim
+
+    def paged_append(self, key_states, value_states, slots, key_pages, value_pages, key_scales, value_scales, positions=None, sin=None, cos=None):
+        _req(key_pages.dim() == 4 and key_states.dim() == 2 and key_states.size(1) % max(key_pages.size(1), 1) == 0,
+             "key_states must be [rows, kv_heads * head_dim], key_pages [blocks, kv_heads, block, hd16]")
+        head_dim = key_states.size(1) // key_pages.size(1)
+        code, blocks, kvh, block = self._pages(key_pages, value_pages, key_scales, value_scales, head_dim)
+        dev = key_pages.device
+        ks, vs = self._rows16(key_states, "key_states", dev), self._rows16(value_states, "value_states", dev)
+        _req(key_states.shape == value_states.shape, "key_states and value_states have incompatible shapes")
+        sp, cp, ar = self._angles(sin, cos, head_dim, dev)
+        _req(sp is None or not _is_none(positions), "a rotation needs positions")
+        for t, n in ((slots, "slots"), (positions, "positions")):
+            if not _is_none(t):
+                _req_dtype(t, torch.int32, n)
+                _req_cuda(t, n)
+                _req(t.device == dev and t.numel() == key_states.size(0), f"{n} must hold one int for each row of key_states, on the device of the pages")
+        _req(not _is_none(slots), "slots is missing")
+        with _Guard(dev):
+            check(self._lib.exl_paged_append(key_states.data_ptr(), value_states.data_ptr(), ks, vs, slots.data_ptr(), key_states.size(0),
+                                             key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), code,
+                                             blocks, kvh, block, head_dim, _ptr(positions), sp, cp, ar, _stream(key_pages)), "paged_append")
+
+    def paged_attention(self, q, starts, past_lens, new_lens, block_table, key_pages, value_pages, key_scales, value_scales, num_heads, max_new=None,
+                        sin=None, cos=None, scale=0.0, out=None):
+        _req(num_heads > 0 and q.dim() == 2 and q.size(1) % num_heads == 0, "q must be [rows, num_heads * head_dim]")
+        head_dim = q.size(1) // num_heads
+        code, blocks, kvh, block = self._pages(key_pages, value_pages, key_scales, value_scales, head_dim)
+        dev = key_pages.device
+        qs = self._rows16(q, "q", dev)
+        n = past_lens.numel()
+        for t, name in ((starts, "starts"), (past_lens, "past_lens"), (new_lens, "new_lens"), (block_table, "block_table")):
+            _req_dtype(t, torch.int32, name)
+            _req_cuda(t, name)
+            _req(t.device == dev, f"{name} must be on the device of the pages")
+        _req(starts.numel() >= n and new_lens.numel() == n, "starts, past_lens and new_lens have incompatible shapes")
+        _req(block_table.dim() == 2 and block_table.size(0) == n, "block_table must be [rows of the batch, blocks]")
+        sp, cp, ar = self._angles(sin, cos, head_dim, dev)
+        if out is None:
+            out = torch.zeros(q.shape, dtype=torch.float16, device=dev)
+        _req_dtype(out, torch.float16, "out")
+        _req_cuda(out, "out")
+        _req(out.shape == q.shape and out.device == dev, "q and out have incompatible shapes")
+        max_new = q.size(0) if max_new is None else int(max_new)
+        need = self._lib.exl_paged_attention_workspace(n, q.size(0), max_new, int(num_heads), kvh, head_dim, block_table.size(1), block)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None      # of the call's own stream: the allocator keeps it until the work has run
+        with _Guard(dev):
+            check(self._lib.exl_paged_attention(q.data_ptr(), qs, starts.data_ptr(), past_lens.data_ptr(), new_lens.data_ptr(), n, q.size(0),
+                                                max_new, block_table.data_ptr(), block_table.size(1), key_pages.data_ptr(),
+                                                value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), code, blocks, block,
+                                                int(num_heads), kvh, head_dim, float(scale), sp, cp, ar, out.data_ptr(), _ptr(ws), need,
+                                                _stream(key_pages)), "paged_attention")
+        return out
+
     # -- exllama_ext.cpp:424-528
     def q4_attn(self, x, rms_norm_weight, epsilon, query_states, key_states, value_states, q_proj, k_proj, v_proj,
                 sin, cos, q_len, past_len, num_heads, num_kv_heads, head_dim, key_cache, value_cache, max_seq_len,
@@ -560,6 +680,9 @@ rms_norm = exllama_ext.rms_norm
 rope_ = exllama_ext.rope_
 rep_penalty = exllama_ext.rep_penalty
 apply_rep_penalty = exllama_ext.apply_rep_penalty
+paged_slots = exllama_ext.paged_slots
+paged_append = exllama_ext.paged_append
+paged_attention = exllama_ext.paged_attention
 
 
 # ---- Python wrappers (reference: cuda_ext.py:87-166) -------------------------------------------------------
@@ -622,3 +745,31 @@ def ext_rep_penalty_mask_cpu(vocab_size, sequence, penalty_max, sustain, decay):
 
 def ext_apply_rep_penalty_mask_cpu(sequence, penalty_max, sustain, decay, logits):
     apply_rep_penalty(sequence, penalty_max, sustain, decay, logits)
+
+
+# ---- the paged 8-bit cache: no counterpart in the reference, whose cache is fp16 with one length for all rows -----------------------------
+
+def ext_paged_slots(past_lens, new_lens, held, block_table, ring, counters, block_size, rows, max_new=None, max_len=None, row_stride=0):
+    """Block tables and slot maps from request lengths; returns (starts [n + 1], slots [rows], positions [rows]), int32.
+
+    Row b holds past_lens[b] tokens and brings new_lens[b] (at most max_new; < 0: it has ended and gives its blocks back).  Its tokens take the
+    token rows from starts[b] on (one row of the batch behind the other; row_stride > 0: starts[b] = b * row_stride), and block_table
+    [n, width], held [n], ring [blocks], counters [4] (head of the ring, free blocks, missing blocks, 0) are updated in place so that the
+    row owns the blocks of past + new tokens (at most max_len).  slots: block * block_size + offset, -1 without a token or a block.
+    The same call again changes nothing more; past_lens stays as it is.  All lengths are read on the device."""
+    return paged_slots(past_lens, new_lens, held, block_table, ring, counters, block_size, rows, max_new, max_len, row_stride)
+
+
+def ext_paged_append(key_states, value_states, slots, key_pages, value_pages, key_scales, value_scales, positions=None, sin=None, cos=None):
+    """New keys and values [rows, kv_heads * head_dim] (fp16) into the 8-bit pages at `slots`, in place; with sin / cos the keys are rotated
+    at `positions` first.  One rounding for each code; one power-of-two scale for each (page, head)."""
+    paged_append(key_states, value_states, slots, key_pages, value_pages, key_scales, value_scales, positions, sin, cos)
+
+
+def ext_paged_attention(q, starts, past_lens, new_lens, block_table, key_pages, value_pages, key_scales, value_scales, num_heads, max_new=None,
+                        sin=None, cos=None, scale=0.0, out=None):
+    """Causal attention of q [rows, num_heads * head_dim] over the pages; returns out.  Row b's queries are q[starts[b]:starts[b] +
+    new_lens[b]] (at most max_new) and see its past_lens[b] earlier keys and the new ones up to their own; with sin / cos they are
+    rotated first.  Rows of an `out` that was given and belong to no row of the batch stay as they are."""
+    return paged_attention(q, starts, past_lens, new_lens, block_table, key_pages, value_pages, key_scales, value_scales, num_heads, max_new, sin, cos,
+                           scale, out)

@@ -203,6 +203,47 @@ int exl_attention(const void* q, const void* key_cache, const void* value_cache,
                   int bsz, int q_len, int num_heads, int num_kv_heads, int head_dim, int max_seq_len,
                   int past_len, const int32_t* past_len_dev, void* stream);
 
+/* ---- paged 8-bit key / value cache (no counterpart in the reference, whose cache is fp16 with one length for all rows) ------------- */
+/* Pages of block_size (16, 32, 64, 128) tokens in a pool of num_blocks: key_pages [blocks, kv_heads, block, hd16], value_pages
+ * [blocks, kv_heads, hd16, block] (a value's tokens next to each other), hd16 = head_dim rounded up to 16, 16-byte aligned; one float scale
+ * for each (page, head), a power of two: x = code * scale.  code: EXL_PAGE_FP8 (e4m3, scales 2^-15 .. 2^7) or EXL_PAGE_INT8 (-127 .. 127,
+ * scales 2^-24 .. 2^9); values beyond 57344 / 65024 saturate.  head_dim: a multiple of 4, at most 256.  Row b's token at position
+ * p lies in page block_table[b][p / block_size].  Lengths and tables are read on the DEVICE: every call can be captured and replayed
+ * while they change; nothing synchronises or allocates, and no result depends on the order of workgroups. */
+#define EXL_PAGE_FP8  0
+#define EXL_PAGE_INT8 1
+/* Block tables and slot maps from request lengths.  For each of n_rows rows, in order: its new tokens (clamp(new_lens, 0, max_new), while
+ * token rows last) take the token rows starts[b] .. (an exclusive prefix sum; row_stride > 0: b * row_stride, at most row_stride
+ * tokens), and the row gets the blocks that past + new tokens (at most max_len, which the table must hold) need beyond the `held` first
+ * entries of its block_table row [n_rows, table_width], from the ring of free blocks: counters[0] = the ring's head, counters[1] = free
+ * blocks, ring [num_blocks].  new_lens[b] < 0: the row has ended, its blocks go to the ring's end (free from the NEXT call on), its table
+ * entries become -1, held 0.  slots [rows] = block * block_size + offset of each token row, -1 without a token or a block; positions [rows];
+ * starts [n_rows + 1].  counters[2] = blocks that were wanted and not there.  block_table, held, ring and counters are updated in place;
+ * the same call again changes nothing more.  past_lens is not touched.  scratch: 8 * n_rows ints. */
+int exl_paged_slots(const int32_t* past_lens, const int32_t* new_lens, int32_t* held, int32_t* block_table, int32_t* ring, int32_t* counters,
+                    int n_rows, int table_width, int block_size, int num_blocks, int max_len, int max_new, int rows, int row_stride,
+                    int32_t* starts, int32_t* slots, int32_t* positions, int32_t* scratch, void* stream);
+/* New keys and values, fp16 rows key_states + t * key_stride (elements) of kv_heads * head_dim, into the pages at slots[t] (-1, or outside
+ * the pool: skipped).  The tokens of one page stand next to each other in ascending order, as exl_paged_slots lays them; a page is
+ * written through one row of the batch at a time.  A run of tokens that starts a page sets the page's scale from its largest
+ * magnitude; one that continues a page keeps the earlier tokens, whose codes move to the larger of the two scales.  Each code is ONE
+ * rounding (nearest even) of x / scale; NaN stays NaN (int8: 0).  sin / cos (fp16 [angle_rows, head_dim], both or neither): keys are rotated
+ * by halves at positions[t] first (exactly; the code is one rounding of the rotated key). */
+int exl_paged_append(const void* key_states, const void* value_states, long key_stride, long value_stride, const int32_t* slots, int rows,
+                     void* key_pages, void* value_pages, float* key_scales, float* value_scales, int code, int num_blocks, int num_kv_heads,
+                     int block_size, int head_dim, const int32_t* positions, const void* sin, const void* cos, int angle_rows, void* stream);
+/* Attention over the pages: query row starts[b] + i (q + t * q_stride, heads * head_dim fp16; i < new_lens[b], at most max_new) sees the keys
+ * j <= past_lens[b] + i of row b, j < past + new and inside the table; softmax(scale * q . k), fp32 sums, one rounding to fp16.  scale <= 0:
+ * 1 / sqrt(head_dim).  sin / cos: q is rotated at its position first (fp32, rounded to fp16).  Pages outside the pool are not seen; a
+ * query that sees nothing gives zeros; rows of `out` [rows, heads * head_dim] that belong to no row of the batch are left as they were.
+ * workspace: at least exl_paged_attention_workspace(...) bytes, for this call alone until it has run. */
+size_t exl_paged_attention_workspace(int n_rows, int rows, int max_new, int num_heads, int num_kv_heads, int head_dim, int table_width, int block_size);
+int exl_paged_attention(const void* q, long q_stride, const int32_t* starts, const int32_t* past_lens, const int32_t* new_lens, int n_rows, int rows,
+                        int max_new, const int32_t* block_table, int table_width, const void* key_pages, const void* value_pages,
+                        const float* key_scales, const float* value_scales, int code, int num_blocks, int block_size, int num_heads,
+                        int num_kv_heads, int head_dim, float scale, const void* sin, const void* cos, int angle_rows, void* out, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 /* ---- fused decode ops ------------------------------------------------------------------------------- */
 /* reference: exllama_ext.cpp:424-528 q4_attn -> q4_attn.cu:74-204:
  *   rms_norm(x) -> q/k/v projections (+LoRA) -> RoPE(q), RoPE(k) -> KV scatter at past_len.
