@@ -9,6 +9,8 @@
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
@@ -271,6 +273,178 @@ FAST(attention, 6, 8, "q", "key_cache", "value_cache", "out", "past_len", "num_h
                         opt_i32_ptr(a[7], "past_len_dev"), stream_of(dev)), "attention");
 FAST_END
 
+// ---- the paged 8-bit cache (exl_paged_*; no pybind counterpart): the checks of exllama_amd/cuda_ext.py, in the same order -----------------
+
+// contiguous int32 tensor on device `dev` (< 0: any HIP device)
+int32_t* i32_on(PyObject* o, const char* name, int dev)
+{
+    const at::Tensor& t = tensor(o, name);
+    if (t.scalar_type() != at::kInt) failf(name, "is incorrect datatype, must be torch.int32");
+    if (!t.is_cuda()) failf(name, "must be on a HIP device (exllama_amd has no CPU path)");
+    if (!t.is_contiguous()) failf(name, "must be contiguous");
+    if (dev >= 0 && (int) t.get_device() != dev) failf(name, "must be on the device of the other tensors");
+    return (int32_t*) t.data_ptr();
+}
+
+long opt_long(PyObject* o, const char* name, long otherwise) { return o == Py_None ? otherwise : as_long(o, name); }
+
+int as_int(long v, const char* name)
+{
+    if (v < -0x7fffffffL || v > 0x7fffffffL) failf(name, "is out of range");
+    return (int) v;
+}
+
+struct Pages { void* kp; void* vp; float* ks; float* vs; int code, blocks, kvh, block, dev; };
+
+// a[0 .. 3] = key_pages, value_pages, key_scales, value_scales
+Pages pages(PyObject* const* a, long head_dim)
+{
+    const at::Tensor& k = tensor(a[0], "key_pages"); const at::Tensor& v = tensor(a[1], "value_pages");
+    Pages p;
+    if (k.scalar_type() == at::kFloat8_e4m3fn) p.code = EXL_PAGE_FP8;
+    else if (k.scalar_type() == at::kChar) p.code = EXL_PAGE_INT8;
+    else fail("key_pages is incorrect datatype, must be torch.float8_e4m3fn or torch.int8");
+    if (v.scalar_type() != k.scalar_type()) fail("value_pages is incorrect datatype, must be key_pages'");
+    if (k.dim() != 4 || v.dim() != 4) fail("key_pages must be [blocks, kv_heads, block, hd16], value_pages [blocks, kv_heads, hd16, block]");
+    const long nb = k.size(0), kvh = k.size(1), block = k.size(2), hd16 = k.size(3);
+    if (v.size(0) != nb || v.size(1) != kvh || v.size(2) != hd16 || v.size(3) != block)
+        fail("value_pages must be [blocks, kv_heads, hd16, block] for key_pages [blocks, kv_heads, block, hd16]");
+    if (hd16 != (head_dim + 15) / 16 * 16) fail("the pages' columns do not match head_dim rounded up to 16");
+    for (int i = 2; i < 4; ++i) {
+        const at::Tensor& s = tensor(a[i], i == 2 ? "key_scales" : "value_scales");
+        if (s.scalar_type() != at::kFloat) failf(i == 2 ? "key_scales" : "value_scales", "is incorrect datatype, must be torch.float32");
+        if (s.dim() != 2 || s.size(0) != nb || s.size(1) != kvh) failf(i == 2 ? "key_scales" : "value_scales", "scales must be [blocks, kv_heads]");
+    }
+    static const char* const names[] = {"key_pages", "value_pages", "key_scales", "value_scales"};
+    for (int i = 0; i < 4; ++i) {
+        const at::Tensor& t = THPVariable_Unpack(a[i]);
+        if (!t.is_cuda()) failf(names[i], "must be on a HIP device (exllama_amd has no CPU path)");
+        if (!t.is_contiguous()) failf(names[i], "must be contiguous");
+        if (t.get_device() != k.get_device()) failf(names[i], "must be on the device of key_pages");
+    }
+    p.kp = k.data_ptr(); p.vp = v.data_ptr();
+    p.ks = (float*) THPVariable_Unpack(a[2]).data_ptr(); p.vs = (float*) THPVariable_Unpack(a[3]).data_ptr();
+    p.blocks = as_int(nb, "blocks"); p.kvh = as_int(kvh, "kv_heads"); p.block = as_int(block, "block"); p.dev = (int) k.get_device();
+    return p;
+}
+
+// fp16 rows with their columns next to each other; returns the row stride
+long rows16(const at::Tensor& t, const char* name, int dev)
+{
+    if (t.scalar_type() != at::kHalf) failf(name, "is incorrect datatype, must be torch.float16");
+    if (!t.is_cuda()) failf(name, "must be on a HIP device (exllama_amd has no CPU path)");
+    if ((int) t.get_device() != dev) failf(name, "must be on the device of the pages");
+    if (t.dim() != 2 || t.stride(1) != 1) failf(name, "must be [rows, width] with the columns of a row next to each other");
+    return t.size(0) > 1 ? t.stride(0) : std::max<long>(t.size(1), 4);
+}
+
+struct Angles { void* sin; void* cos; int rows; };
+Angles angles(PyObject* so, PyObject* co, long head_dim, int dev)
+{
+    if (is_none(so) && is_none(co)) return {nullptr, nullptr, 0};
+    if (is_none(so) || is_none(co)) fail("a rotation needs both sin and cos");
+    int ds = 0, dc = 0;
+    Angles a = {half_ptr(so, "sin", &ds), half_ptr(co, "cos", &dc), 0};
+    const at::Tensor& s = THPVariable_Unpack(so); const at::Tensor& c = THPVariable_Unpack(co);
+    if (ds != dev || dc != dev) fail("sin and cos must be on the device of the pages");
+    if (s.dim() == 0 || c.dim() == 0 || s.size(-1) != head_dim || c.size(-1) != head_dim) fail("sin / cos table does not match head_dim");
+    if (s.numel() != c.numel() || s.numel() == 0) fail("sin and cos have incompatible shapes");
+    a.rows = as_int(s.numel() / head_dim, "sin");
+    return a;
+}
+
+at::Tensor bytes_on(int64_t n, at::ScalarType type, int dev)
+{
+    return at::empty({n}, at::TensorOptions().dtype(type).device(at::Device(at::kCUDA, (c10::DeviceIndex) dev)));
+}
+
+FAST(paged_slots, 8, 11, "past_lens", "new_lens", "held", "block_table", "ring", "counters", "block_size", "rows", "max_new", "max_len", "row_stride")
+    const at::Tensor& past = tensor(a[0], "past_lens"); const at::Tensor& table = tensor(a[3], "block_table");
+    const long n = past.numel();
+    int32_t* pp = i32_on(a[0], "past_lens", -1);
+    const int dev = (int) past.get_device();
+    int32_t* np = i32_on(a[1], "new_lens", dev);
+    int32_t* hp = i32_on(a[2], "held", dev);
+    int32_t* cp = i32_on(a[5], "counters", dev);
+    int32_t* rp = i32_on(a[4], "ring", dev);
+    int32_t* tp = i32_on(a[3], "block_table", dev);
+    if (THPVariable_Unpack(a[1]).numel() != n) fail("new_lens has the wrong size");
+    if (THPVariable_Unpack(a[2]).numel() != n) fail("held has the wrong size");
+    if (THPVariable_Unpack(a[5]).numel() != 4) fail("counters has the wrong size");
+    if (table.dim() != 2 || table.size(0) != n) fail("block_table must be [rows of the batch, blocks]");
+    const long block = as_long(a[6], "block_size"), rows = as_long(a[7], "rows"), width = table.size(1);
+    if (rows < 0) fail("rows must not be negative");
+    const long max_new = opt_long(a[8], "max_new", rows), max_len = opt_long(a[9], "max_len", width * block), stride = opt_long(a[10], "row_stride", 0);
+    DevGuard guard(dev);
+    const at::Tensor buf = bytes_on(n + 1 + 2 * rows + 8 * n, at::kInt, dev);
+    int32_t* b = (int32_t*) buf.data_ptr();
+    check(exl_paged_slots(pp, np, hp, tp, rp, cp, as_int(n, "past_lens"), as_int(width, "block_table"), as_int(block, "block_size"),
+                          as_int(THPVariable_Unpack(a[4]).numel(), "ring"), as_int(max_len, "max_len"), as_int(max_new, "max_new"), as_int(rows, "rows"),
+                          as_int(stride, "row_stride"), b, b + n + 1, b + n + 1 + rows, b + n + 1 + 2 * rows, stream_of(dev)), "paged_slots");
+    PyObject* r = PyTuple_New(3);
+    if (!r) throw Err();
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(buf.narrow(0, 0, n + 1)));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(buf.narrow(0, n + 1, rows)));
+    PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(buf.narrow(0, n + 1 + rows, rows)));
+    return r;
+FAST_END
+
+FAST(paged_append, 7, 10, "key_states", "value_states", "slots", "key_pages", "value_pages", "key_scales", "value_scales", "positions", "sin", "cos")
+    const at::Tensor& k = tensor(a[0], "key_states"); const at::Tensor& v = tensor(a[1], "value_states"); const at::Tensor& kp = tensor(a[3], "key_pages");
+    if (kp.dim() != 4 || k.dim() != 2 || kp.size(1) < 1 || k.size(1) % kp.size(1) != 0)
+        fail("key_states must be [rows, kv_heads * head_dim], key_pages [blocks, kv_heads, block, hd16]");
+    const long hd = k.size(1) / kp.size(1);
+    const Pages p = pages(a + 3, hd);
+    const long ks = rows16(k, "key_states", p.dev), vs = rows16(v, "value_states", p.dev);
+    if (k.size(0) != v.size(0) || k.size(1) != v.size(1)) fail("key_states and value_states have incompatible shapes");
+    const Angles an = angles(a[8], a[9], hd, p.dev);
+    if (an.sin && is_none(a[7])) fail("a rotation needs positions");
+    if (is_none(a[2])) fail("slots is missing");
+    int32_t* sp = i32_on(a[2], "slots", p.dev);
+    int32_t* pp = is_none(a[7]) ? nullptr : i32_on(a[7], "positions", p.dev);
+    if (THPVariable_Unpack(a[2]).numel() != k.size(0)) fail("slots must hold one int for each row of key_states, on the device of the pages");
+    if (pp && THPVariable_Unpack(a[7]).numel() != k.size(0)) fail("positions must hold one int for each row of key_states, on the device of the pages");
+    DevGuard guard(p.dev);
+    check(exl_paged_append(k.data_ptr(), v.data_ptr(), ks, vs, sp, as_int(k.size(0), "key_states"), p.kp, p.vp, p.ks, p.vs, p.code, p.blocks, p.kvh, p.block,
+                           as_int(hd, "head_dim"), pp, an.sin, an.cos, an.rows, stream_of(p.dev)), "paged_append");
+FAST_END
+
+FAST(paged_attention, 10, 15, "q", "starts", "past_lens", "new_lens", "block_table", "key_pages", "value_pages", "key_scales", "value_scales", "num_heads",
+     "max_new", "sin", "cos", "scale", "out")
+    const at::Tensor& q = tensor(a[0], "q"); const at::Tensor& table = tensor(a[4], "block_table");
+    const long heads = as_long(a[9], "num_heads");
+    if (heads < 1 || q.dim() != 2 || q.size(1) % heads != 0) fail("q must be [rows, num_heads * head_dim]");
+    const long hd = q.size(1) / heads, rows = q.size(0);
+    const Pages p = pages(a + 5, hd);
+    const long qs = rows16(q, "q", p.dev);
+    int32_t* sp = i32_on(a[1], "starts", p.dev);
+    int32_t* pp = i32_on(a[2], "past_lens", p.dev);
+    int32_t* np = i32_on(a[3], "new_lens", p.dev);
+    int32_t* tp = i32_on(a[4], "block_table", p.dev);
+    const long n = THPVariable_Unpack(a[2]).numel();
+    if (THPVariable_Unpack(a[1]).numel() < n || THPVariable_Unpack(a[3]).numel() != n) fail("starts, past_lens and new_lens have incompatible shapes");
+    if (table.dim() != 2 || table.size(0) != n) fail("block_table must be [rows of the batch, blocks]");
+    const Angles an = angles(a[11], a[12], hd, p.dev);
+    DevGuard guard(p.dev);
+    const bool given = !is_none(a[14]);
+    const at::Tensor out = given ? tensor(a[14], "out")
+                                 : at::zeros({rows, q.size(1)}, at::TensorOptions().dtype(at::kHalf).device(at::Device(at::kCUDA, (c10::DeviceIndex) p.dev)));
+    if (given) {
+        half_ptr(a[14], "out");
+        if (out.dim() != 2 || out.size(0) != rows || out.size(1) != q.size(1) || (int) out.get_device() != p.dev) fail("q and out have incompatible shapes");
+    }
+    const int max_new = as_int(opt_long(a[10], "max_new", rows), "max_new");
+    const size_t need = exl_paged_attention_workspace(as_int(n, "past_lens"), as_int(rows, "q"), max_new, as_int(heads, "num_heads"), p.kvh, as_int(hd, "head_dim"),
+                                                      as_int(table.size(1), "block_table"), p.block);
+    at::Tensor ws;                                               // of the call's own stream: the allocator keeps it until the work has run
+    if (need) ws = bytes_on((int64_t) need, at::kByte, p.dev);
+    check(exl_paged_attention(q.data_ptr(), qs, sp, pp, np, (int) n, (int) rows, max_new, tp, (int) table.size(1), p.kp, p.vp, p.ks, p.vs, p.code, p.blocks,
+                              p.block, (int) heads, p.kvh, (int) hd, (float) (a[13] == Py_None ? 0.0 : as_double(a[13], "scale")), an.sin, an.cos, an.rows,
+                              out.data_ptr(), need ? ws.data_ptr() : nullptr, need, stream_of(p.dev)), "paged_attention");
+    if (given) { Py_INCREF(a[14]); return a[14]; }
+    return THPVariable_Wrap(out);
+FAST_END
+
 #define KW (METH_FASTCALL | METH_KEYWORDS)
 #define FN(f) (PyCFunction) (void (*)(void)) f
 PyMethodDef methods[] = {
@@ -287,6 +461,15 @@ PyMethodDef methods[] = {
      "exllama_ext.cpp:567-602"},
     {"attention", FN(attention), KW,
      "attention($module, /, q, key_cache, value_cache, out, past_len, num_heads, mask=None, past_len_dev=None)\n--\n\nexl_attention"},
+    {"paged_slots", FN(paged_slots), KW,
+     "paged_slots($module, /, past_lens, new_lens, held, block_table, ring, counters, block_size, rows, max_new=None, max_len=None, row_stride=0)\n--\n\n"
+     "exl_paged_slots"},
+    {"paged_append", FN(paged_append), KW,
+     "paged_append($module, /, key_states, value_states, slots, key_pages, value_pages, key_scales, value_scales, positions=None, sin=None, "
+     "cos=None)\n--\n\nexl_paged_append"},
+    {"paged_attention", FN(paged_attention), KW,
+     "paged_attention($module, /, q, starts, past_lens, new_lens, block_table, key_pages, value_pages, key_scales, value_scales, num_heads, "
+     "max_new=None, sin=None, cos=None, scale=0.0, out=None)\n--\n\nexl_paged_attention"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef moddef = {PyModuleDef_HEAD_INIT, "_exl_fast", "compiled binding of the per-token entry points of libexl_amd.so", -1, methods};

@@ -22,86 +22,776 @@ __device__ __forceinline__ PaRow pa_row(const PagedAttn& a, int b)
     return r;
 }
 
-#define PA_TILE 256
+// ---- rows of few queries: the cache's bytes are all that counts ------------------------------------------------------------------------
+// One workgroup (4 waves) streams a piece of one row's keys and values of one kv head, in tiles of 64 keys, for all of the row's queries and
+// all query heads of that kv head (up to 16 * NT of them: GQA reads the cache once).  Both products are MFMAs on fp16 numbers converted from the
+// codes in registers; nothing goes through LDS in the loop:
+//   S^T = K Q^T   (16x16x32): A = keys.  MFMA row m of product t4 is key 16 * (m >> 2) + 4 * t4 + (m & 3) of the tile, so that a lane (query
+//                 column c = lane & 15, group g = lane >> 4) gets the 16 scores of keys 16 g .. 16 g + 15, in order, over the four products;
+//   O^T = V^T P^T : A = value columns, 16 bytes = keys 16 g .. 16 g + 15 of one column, as the page holds them; B = the lane's own 16 weights.
+// Running maximum and sum stay in the lane of the query; the four waves (64 keys each in turn) join through LDS at the end.  A piece's key range is
+// a function of the lengths alone, and the pieces of a row are joined in order: results do not depend on scheduling.
+#define PA_WAVES 4
+#define PA_KEYS 64
+#define PA_MAX_ROWS 1024                                       // rows of the batch up to which their keys are cut into pieces of equal size
 
-// One workgroup = one query row of one head: a thread per key of a tile of 256 for the scores, then a thread per column for the sum.
-template <int CODE> __global__ __launch_bounds__(PA_TILE) void paged_attn_row_kernel(PagedAttn a)
+template <int CODE> __device__ __forceinline__ f16x8 pa_numbers(uint32_t lo, uint32_t hi, float scale)     // 8 codes * scale (a power of two)
 {
-    __shared__ float qs[256], sc[PA_TILE], red[8];
-    const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-    int lo = 0, hi = a.n;
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (a.starts[mid] <= t) lo = mid; else hi = mid; }
-    const PaRow row = pa_row(a, lo);
-    const int i = t - row.start, past = row.past;
-    if (i < 0 || i >= row.fresh) return;
-    const int keys = (int) min((int64_t) past + i + 1, (int64_t) row.keys);
-    const int kvh = h / (a.heads / a.kv_heads);
-    const f16* q = a.q + (size_t) t * a.q_stride + (size_t) h * a.hd;
-    if (tid < a.hd) {
-        float x = (float) q[tid];
-        if (a.sin) {
-            const int pos = (int) min((int64_t) past + i, (int64_t) a.angle_rows - 1), half = a.hd >> 1;
-            const float s = (float) a.sin[(size_t) pos * a.hd + tid], c = (float) a.cos[(size_t) pos * a.hd + tid];
-            x = x * c + (tid < half ? -(float) q[tid + half] : (float) q[tid - half]) * s;
+    f16x8 r;
+    if (CODE == EXL_PAGE_FP8) {
+        f16x2* p = (f16x2*) &r;
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) lo, scale, false);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) lo, scale, true);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) hi, scale, false);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) hi, scale, true);
+    } else {
+        // 0x6400 | u is the fp16 number 1024 + u: the bytes with the sign bit flipped (u = code + 128), minus 1152
+        const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
+        union { uint32_t u[4]; f16x2 h[4]; f16x8 v; } x;
+        x.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+        x.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+        x.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+        x.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+        const f16 s = (f16) scale;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.h[i] = (x.h[i] - (f16) 1152.f) * s;
+        r = x.v;
+    }
+    return r;
+}
+
+// Query elements d .. d + 7 of one token and head (zeros behind head_dim), rotated at `pos` when there are tables
+__device__ __forceinline__ f16x8 pa_query(const PagedAttn& a, const f16* q, int64_t pos, int d)
+{
+    f16x8 r = {};
+    if (d >= a.hd) return r;
+    const int half = a.hd >> 1;
+    const f16* sin = nullptr; const f16* cos = nullptr;
+    if (a.sin) {
+        const size_t at = (size_t) (pos < a.angle_rows ? pos : a.angle_rows - 1) * a.hd;
+        sin = a.sin + at; cos = a.cos + at;
+    }
+    if (a.hd % 16 == 0) {
+        r = *(const f16x8_a8*) (q + d);
+        if (sin) {
+            const f16x8 o = *(const f16x8_a8*) (q + (d < half ? d + half : d - half)), s = *(const f16x8_a8*) (sin + d), c = *(const f16x8_a8*) (cos + d);
+            const float sign = d < half ? -1.f : 1.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = (f16) fmaf((float) r[i], (float) c[i], sign * (float) o[i] * (float) s[i]);
         }
-        qs[tid] = x;
+        return r;
+    }
+    for (int i = 0; i < 8; ++i) {                                // head_dim not a multiple of 16: the halves meet inside eight elements
+        const int e = d + i;
+        if (e >= a.hd) break;
+        float x = (float) q[e];
+        if (sin) x = fmaf(x, (float) cos[e], (e < half ? -(float) q[e + half] : (float) q[e - half]) * (float) sin[e]);
+        r[i] = (f16) x;
+    }
+    return r;
+}
+
+// Which rows of the batch the kernel for few queries takes, and how their keys are cut: `tiles` tiles of a row in pieces of `piece` tiles
+struct PaCut { int few, target, min_piece, split; };             // few: queries of a row (tokens * group) up to which it is taken
+
+__device__ __forceinline__ int pa_few_tiles(const PagedAttn& a, const PaCut& cut, int b, PaRow& r)
+{
+    r = pa_row(a, b);
+    const int64_t queries = (int64_t) r.fresh * (a.heads / a.kv_heads);
+    return queries > 0 && queries <= cut.few ? (r.keys + PA_KEYS - 1) / PA_KEYS : 0;
+}
+
+struct PaItem { int row, first, last, piece, pieces; };          // tiles first .. last - 1, piece number `piece` of `pieces`
+
+// Item `w` of the launch; row < 0: none.  Every thread of the workgroup calls it.
+__device__ __forceinline__ PaItem pa_find(const PagedAttn& a, const PaCut& cut, int w)
+{
+    __shared__ int64_t sums[PA_WAVES];
+    __shared__ PaItem found;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    PaRow r;
+    PaItem it = {-1, 0, 0, 0, 0};
+    if (a.n > PA_MAX_ROWS) {
+        const int tiles = pa_few_tiles(a, cut, w, r);
+        if (tiles > 0) it = {w, 0, tiles, 0, 1};
+        return it;
+    }
+    int64_t total = 0;
+    int tiles0 = 0;
+    for (int b = tid; b < a.n; b += PA_WAVES * 64) {
+        const int tiles = pa_few_tiles(a, cut, b, r);
+        if (b == tid) tiles0 = tiles;
+        total += tiles;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+    if (lane == 0) sums[wave] = total;
+    if (tid == 0) found = it;
+    __syncthreads();
+    total = sums[0] + sums[1] + sums[2] + sums[3];
+    const int64_t even = (total + cut.target - 1) / cut.target;
+    const int piece = (int) (even > cut.min_piece ? even : cut.min_piece);
+    int before = 0;
+    for (int b0 = 0; b0 < a.n; b0 += PA_WAVES * 64) {
+        const int b = b0 + tid;
+        const int tiles = b >= a.n ? 0 : b0 == 0 ? tiles0 : pa_few_tiles(a, cut, b, r);
+        const int mine = (tiles + piece - 1) / piece;
+        int inc = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) { const int o = __shfl_up(inc, off, 64); if (lane >= off) inc += o; }
+        __syncthreads();
+        if (lane == 63) sums[wave] = inc;
+        __syncthreads();
+        int base = before + inc - mine;
+        for (int u = 0; u < wave; ++u) base += (int) sums[u];
+        if (w >= base && w < base + mine) {
+            const int k = w - base;
+            // equal pieces: their number is settled, the tiles are shared out evenly
+            found = {b, (int) ((int64_t) tiles * k / mine), (int) ((int64_t) tiles * (k + 1) / mine), k, mine};
+        }
+        before += (int) (sums[0] + sums[1] + sums[2] + sums[3]);
+        if (before > w) break;
     }
     __syncthreads();
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int j0 = 0; j0 < keys; j0 += PA_TILE) {
-        const int j = j0 + tid;
-        float s = -INFINITY;
-        if (j < keys) {
-            const int id = a.table[(size_t) lo * a.width + j / a.block];
-            if (id >= 0 && id < a.blocks) {
-                const size_t base = (size_t) id * a.kv_heads + kvh;
-                const uint32_t* k = (const uint32_t*) (a.kp + (base * a.block + j % a.block) * a.hd16);
-                s = 0.f;
-                for (int d = 0; d < a.hd; d += 4) {
-                    float x[4];
-                    paged_decode4<CODE>(k[d >> 2], x);
-                    s += x[0] * qs[d] + x[1] * qs[d + 1] + x[2] * qs[d + 2] + x[3] * qs[d + 3];
-                }
-                s *= a.ks[base] * a.scale;
+    return found;
+}
+
+// Partial results of an item that is one of several pieces: [item * kv_heads + kv_head][16 * NT queries][DP + 2] floats (o, then m and l)
+__host__ __device__ constexpr size_t pa_part_floats(int dp, int nt) { return (size_t) 16 * nt * (dp + 2); }
+
+// Registers (DP = 128, NT = 1): 64 for a tile's bytes, twice (the next tile is on its way while one is worked on), 32 of O, 32 of Q: two waves per
+// SIMD.  Twice the queries take one wave per SIMD, and so do wider heads, without the second set of bytes.
+template <int CODE, int DP, int NT>
+__global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_attn_few_kernel(PagedAttn a, PaCut cut, float* __restrict__ parts,
+                                                                                            int2* __restrict__ firsts)
+{
+    constexpr int KS = DP / 64, DT = DP / 16, ROW = DP + 4;
+    constexpr bool AHEAD = DP <= 128;
+    __shared__ __attribute__((aligned(16))) float joined[PA_WAVES][16 * ROW];
+    __shared__ float stat[PA_WAVES][2][16];
+    const int kvh = blockIdx.y, w = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const PaItem it = pa_find(a, cut, w);
+    if (it.row < 0) return;
+    if (kvh == 0 && tid == 0 && it.piece == 0) firsts[it.row] = make_int2(w, it.pieces);       // for the joining kernel
+    const PaRow row = pa_row(a, it.row);
+    const int group = a.heads / a.kv_heads, queries = row.fresh * group;
+    const int lbs = 31 - __clz(a.block);
+
+    f16x8 qf[NT][KS][2];
+    int limit[NT];                                               // the last key this lane's query sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 16 + c, i = r / group;
+        const bool in = r < queries;
+        limit[nt] = in ? (int) min((int64_t) row.past + i, (int64_t) row.keys - 1) : -1;
+        const f16* q = a.q + (size_t) (row.start + (in ? i : 0)) * a.q_stride + (size_t) (kvh * group + (in ? r % group : 0)) * a.hd;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                f16x8 x = pa_query(a, q, (int64_t) row.past + i, 64 * s + 16 * g + 8 * half);
+                if (!in) x = (f16x8) {};
+                qf[nt][s][half] = x;
             }
-        }
-        float mx = s;
-        for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-        if ((tid & 63) == 0) red[tid >> 6] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
-        const float p = s == -INFINITY ? 0.f : __expf(s - ref), keep = m == -INFINITY ? 0.f : __expf(m - ref);
-        float sum = p;
-        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-        if ((tid & 63) == 0) red[4 + (tid >> 6)] = sum;
-        sc[tid] = p;
-        __syncthreads();
-        l = l * keep + red[4] + red[5] + red[6] + red[7];
-        m = mn;
-        o *= keep;
-        if (tid < a.hd) {
-            for (int u = 0; u < PA_TILE && j0 + u < keys; ++u) {
-                const float w = sc[u];
-                if (w == 0.f) continue;
-                const int id = a.table[(size_t) lo * a.width + (j0 + u) / a.block];
-                if (id < 0 || id >= a.blocks) continue;
-                const size_t base = (size_t) id * a.kv_heads + kvh;
-                const uint8_t* v = a.vp + (base * a.hd16 + tid) * a.block + (j0 + u) % a.block;
-                float x[4];
-                paged_decode4<CODE>(*v, x);
-                o += w * x[0] * a.vs[base];
-            }
-        }
-        __syncthreads();
     }
-    if (tid < a.hd) a.out[(size_t) t * a.heads * a.hd + (size_t) h * a.hd + tid] = (f16) (l > 0.f || l != l ? o / l : 0.f);
+
+    const int32_t* table = a.table + (size_t) it.row * a.width;
+    const size_t kpage = (size_t) a.block * a.hd16;              // bytes of one page of one head, keys or values
+    // byte offsets inside a key row / inside a value page; columns behind head_dim read column 0 (their queries are zeros, their results unused)
+    int kd[KS], vd[DT];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) kd[s] = 64 * s + 16 * g < a.hd16 ? 64 * s + 16 * g : 0;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) vd[t] = (16 * t + c < a.hd16 ? 16 * t + c : 0) * a.block;
+
+    struct Ids { int k, v; };
+    auto look = [&](int tile) -> Ids {                            // the pages of this lane's key rows and of its group's values
+        const int ik = (tile * PA_KEYS + 16 * (c >> 2)) >> lbs, iv = (tile * PA_KEYS + 16 * g) >> lbs;
+        Ids r = {-1, -1};
+        if (ik < a.width) r.k = table[ik];
+        if (iv < a.width) r.v = table[iv];
+        return r;
+    };
+    struct Stage { uint4 k[4][KS]; uint4 v[DT]; float ks, vs; bool there; };
+    auto fetch = [&](int tile, Ids id, Stage& st) {
+        const bool kok = id.k >= 0 && id.k < a.blocks, vok = id.v >= 0 && id.v < a.blocks;
+        const size_t kb = (size_t) (kok ? id.k : 0) * a.kv_heads + kvh, vb = (size_t) (vok ? id.v : 0) * a.kv_heads + kvh;
+        const int key = tile * PA_KEYS + 16 * (c >> 2) + (c & 3);
+        const uint8_t* kp = a.kp + kb * kpage + (size_t) (key & (a.block - 1)) * a.hd16;
+#pragma unroll
+        for (int t4 = 0; t4 < 4; ++t4)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) st.k[t4][s] = *(const uint4*) (kp + 4 * t4 * a.hd16 + kd[s]);
+        const uint8_t* vp = a.vp + vb * kpage + ((tile * PA_KEYS + 16 * g) & (a.block - 1));
+#pragma unroll
+        for (int t = 0; t < DT; ++t) st.v[t] = *(const uint4*) (vp + vd[t]);
+        st.ks = paged_pow2(paged_scale_exp<CODE>(a.ks[vb]));
+        st.vs = paged_pow2(paged_scale_exp<CODE>(a.vs[vb]));
+        st.there = vok;
+    };
+
+    f32x4 o[NT][DT];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt] = -INFINITY; l[nt] = 0.f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[nt][t] = (f32x4) {0.f, 0.f, 0.f, 0.f};
+    }
+    const float c1 = a.scale * 1.44269504f;                       // scores in powers of two
+
+    auto work = [&](int tile, Stage& st) {
+        const int key0 = tile * PA_KEYS + 16 * g;
+        const bool border = tile * PA_KEYS + PA_KEYS - 1 > row.past || __any(!st.there);
+        if (border) {                                            // weights of 0 do not hide what may stand in bytes that hold no value: NaN
+            const int n = st.there ? min(max(row.keys - key0, 0), 16) : 0;
+            uint32_t mask[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mask[i] = n >= 4 * i + 4 ? 0xffffffffu : n <= 4 * i ? 0u : (1u << (8 * (n - 4 * i))) - 1;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) { st.v[t].x &= mask[0]; st.v[t].y &= mask[1]; st.v[t].z &= mask[2]; st.v[t].w &= mask[3]; }
+        }
+        f32x4 s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int t4 = 0; t4 < 4; ++t4) s[nt][t4] = (f32x4) {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t4 = 0; t4 < 4; ++t4)
+#pragma unroll
+            for (int u = 0; u < KS; ++u) {
+                const f16x8 k0 = pa_numbers<CODE>(st.k[t4][u].x, st.k[t4][u].y, 1.f), k1 = pa_numbers<CODE>(st.k[t4][u].z, st.k[t4][u].w, 1.f);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    s[nt][t4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[nt][u][0], s[nt][t4], 0, 0, 0);
+                    s[nt][t4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf[nt][u][1], s[nt][t4], 0, 0, 0);
+                }
+            }
+        f16x8 p[NT][2];
+        const float sc = st.ks * c1;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float x[16], mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                x[i] = s[nt][i >> 2][i & 3] * sc;
+                if (border && (!st.there || key0 + i > limit[nt])) x[i] = -INFINITY;
+                mx = fmaxf(mx, x[i]);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float mn = fmaxf(m[nt], mx);
+            if (__any(mn > m[nt])) {
+                const float keep = m[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[nt] - mn);
+                l[nt] *= keep;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[nt][t][j] *= keep;
+                m[nt] = mn;
+            }
+            const float ref = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(x[i] - ref);
+                l[nt] += e;
+                p[nt][i >> 3][i & 7] = (f16) e;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            const f16x8 v0 = pa_numbers<CODE>(st.v[t].x, st.v[t].y, st.vs), v1 = pa_numbers<CODE>(st.v[t].z, st.v[t].w, st.vs);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                o[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[nt][0], o[nt][t], 0, 0, 0);
+                o[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[nt][1], o[nt][t], 0, 0, 0);
+            }
+        }
+    };
+
+    int tile = it.first + wave;
+    if (tile < it.last) {
+        Stage st;
+        fetch(tile, look(tile), st);
+        for (; tile < it.last; tile += PA_WAVES) {
+            const int next = tile + PA_WAVES;
+            if (AHEAD) {
+                Stage nx;
+                if (next < it.last) fetch(next, look(next), nx);
+                work(tile, st);
+                st = nx;
+            } else {
+                work(tile, st);
+                if (next < it.last) fetch(next, look(next), st);
+            }
+        }
+    }
+
+    // ---- the four waves' results, and out
+    float* part = parts + ((size_t) w * a.kv_heads + kvh) * pa_part_floats(DP, NT);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        float ls = l[nt];
+        ls += __shfl_xor(ls, 16, 64);
+        ls += __shfl_xor(ls, 32, 64);
+        if (nt) __syncthreads();
+        if (g == 0) { stat[wave][0][c] = m[nt]; stat[wave][1][c] = ls; }
+        __syncthreads();
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < PA_WAVES; ++u) top = fmaxf(top, stat[u][0][c]);
+        const float keep = m[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[nt] - top);
+#pragma unroll
+        for (int t = 0; t < DT; ++t) *(f32x4*) &joined[wave][c * ROW + 16 * t + 4 * g] = o[nt][t] * keep;
+        __syncthreads();
+        for (int x = tid; x < 16 * DP; x += PA_WAVES * 64) {
+            const int col = x / DP, d = x % DP, r = nt * 16 + col;
+            if (r >= queries) break;
+            const float v = joined[0][col * ROW + d] + joined[1][col * ROW + d] + joined[2][col * ROW + d] + joined[3][col * ROW + d];
+            top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < PA_WAVES; ++u) top = fmaxf(top, stat[u][0][col]);
+#pragma unroll
+            for (int u = 0; u < PA_WAVES; ++u) sum += stat[u][1][col] * (stat[u][0][col] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stat[u][0][col] - top));      // (0 * NaN: a NaN stays)
+            if (it.pieces == 1) {
+                if (d < a.hd)
+                    a.out[(size_t) (row.start + r / group) * a.heads * a.hd + (size_t) (kvh * group + r % group) * a.hd + d] = (f16) (sum == 0.f ? 0.f : v / sum);
+            } else {
+                part[(size_t) r * (DP + 2) + d] = v;
+                if (d == 0) { part[(size_t) r * (DP + 2) + DP] = top; part[(size_t) r * (DP + 2) + DP + 1] = sum; }
+            }
+        }
+    }
+}
+
+// The pieces of a row joined, in order: one workgroup per row of the batch, query and kv head.
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, PaCut cut, const float* __restrict__ parts, const int2* __restrict__ firsts, int dp, int nt)
+{
+    __shared__ float part_o[16][256 + 4];
+    __shared__ float part_l[16];
+    const int b = blockIdx.x, r = blockIdx.y, kvh = blockIdx.z, group = a.heads / a.kv_heads, tid = threadIdx.x;
+    PaRow row;
+    if (pa_few_tiles(a, cut, b, row) == 0 || r >= row.fresh * group) return;
+    const int2 first = firsts[b];                                 // (the row had a first piece: it was written)
+    if (first.y < 2) return;
+    const size_t step = a.kv_heads * pa_part_floats(dp, nt);
+    const float* p0 = parts + ((size_t) first.x * a.kv_heads + kvh) * pa_part_floats(dp, nt) + (size_t) r * (dp + 2);
+    float top = -INFINITY;
+    for (int k = tid & 63; k < first.y; k += 64) top = fmaxf(top, p0[k * step + dp]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const int lanes = dp >> 2, slices = 256 / lanes, sl = tid / lanes, d = (tid % lanes) * 4;      // dp 64, 128, 256: 16, 8, 4 slices of the pieces
+    float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll 4
+    for (int k = sl; k < first.y; k += slices) {
+        const float* p = p0 + k * step;
+        const float m = p[dp], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        sum += f * p[dp + 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += f * p[d + j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part_o[sl][d + j] = o[j];
+    if (d == 0) part_l[sl] = sum;
+    __syncthreads();
+    if (tid < a.hd) {
+        float v = 0.f, l = 0.f;
+        for (int u = 0; u < slices; ++u) { v += part_o[u][tid]; l += part_l[u]; }
+        a.out[(size_t) (row.start + r / group) * a.heads * a.hd + (size_t) (kvh * group + r % group) * a.hd + tid] = (f16) (l == 0.f ? 0.f : v / l);
+    }
+}
+
+// ---- rows of many queries: prompts and pieces of prompts --------------------------------------------------------------------------------
+// One workgroup (4 waves) takes 128 queries (token * group + head of the group, so that GQA shares the cache's tiles) and walks tiles of 64 keys.
+// The codes are converted ONCE per workgroup on their way into LDS, as fp16 in the MFMA's operand order (two buffers, one barrier a tile); each
+// wave has 32 queries:
+//   S^T = K Q^T (32x32x16): row m of the product is key 16 * ((m >> 2) & 1) + 4 * (m >> 3) + (m & 3) of a half tile, so that a lane (query
+//   column c = lane & 31, group g = lane >> 5) gets keys 16 g .. 16 g + 15 in order;   O^T = V^T P^T: the lane's own weights are the operand.
+// LDS pieces of 16 bytes are laid out by XOR so that neither the writes (one key, all columns) nor the reads (linear) meet in a bank.
+#define PM_ROWS 128
+
+// Which query tiles the kernel for many queries walks, and how their keys are cut (in `pieces` equal parts for every tile of a row)
+struct PmItem { int row, tile, piece, pieces; };
+
+__device__ __forceinline__ int pm_tiles(const PagedAttn& a, int few, int b, PaRow& r)
+{
+    r = pa_row(a, b);
+    const int64_t queries = (int64_t) r.fresh * (a.heads / a.kv_heads);
+    return queries > few ? (int) ((queries + PM_ROWS - 1) / PM_ROWS) : 0;
+}
+
+// Item `w` of the launch; row < 0: none.  Tiles of a row come with the last (the longest) first.  lds: 80 bytes, free again afterwards.
+__device__ __forceinline__ PmItem pm_find(const PagedAttn& a, const PaCut& cut, int w, void* lds)
+{
+    int64_t (*sums)[PA_WAVES] = (int64_t (*)[PA_WAVES]) lds;
+    PmItem& found = *(PmItem*) (sums + 2);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    PaRow r;
+    int64_t cost = 0, count = 0;
+    for (int b = tid; b < a.n; b += PA_WAVES * 64) {
+        const int q = pm_tiles(a, cut.few, b, r);
+        count += q;
+        cost += (int64_t) q * ((r.keys + PA_KEYS - 1) / PA_KEYS);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) { cost += __shfl_xor(cost, off, 64); count += __shfl_xor(count, off, 64); }
+    if (lane == 0) { sums[0][wave] = cost; sums[1][wave] = count; }
+    if (tid == 0) found = {-1, 0, 0, 0};
+    __syncthreads();
+    cost = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+    count = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+    // enough tiles to fill the machine are not cut; pieces number at most target + count <= 2 * target
+    int64_t piece = (cost + cut.target - 1) / cut.target;
+    piece = count >= cut.target || !cut.split ? (int64_t) 1 << 40 : piece > cut.min_piece ? piece : cut.min_piece;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < a.n; b0 += PA_WAVES * 64) {
+        const int b = b0 + tid;
+        const int q = b < a.n ? pm_tiles(a, cut.few, b, r) : 0;
+        const int np = q ? (int) (((r.keys + PA_KEYS - 1) / PA_KEYS + piece - 1) / piece) : 0;
+        const int64_t mine = (int64_t) q * np;
+        int64_t inc = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) { const int64_t o = __shfl_up(inc, off, 64); if (lane >= off) inc += o; }
+        __syncthreads();
+        if (lane == 63) sums[0][wave] = inc;
+        __syncthreads();
+        int64_t base = before + inc - mine;
+        for (int u = 0; u < wave; ++u) base += sums[0][u];
+        if (w >= base && w < base + mine) {
+            const int k = (int) (w - base);
+            found = {b, q - 1 - k / np, k % np, np};
+        }
+        before += sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+        if (before > w) break;
+    }
+    __syncthreads();
+    const PmItem it = found;
+    __syncthreads();                                              // `lds` is the caller's again
+    return it;
+}
+
+template <int CODE, int DP>
+__global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_many_kernel(PagedAttn a, PaCut cut, float* __restrict__ parts,
+                                                                                        PmItem* __restrict__ items, int part_items)
+{
+    constexpr int KB = DP / 16, DT = DP / 32, PIECES = PA_KEYS * KB / 256;       // 16-byte pieces of codes per thread: keys, and as many of values
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // [2][keys: 2 * KB * 1024 bytes, values: 4 * DT * 1024 bytes]
+    constexpr int K_BYTES = 2 * KB * 1024, BUF = 2 * K_BYTES;
+    const int kvh = blockIdx.y, w = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, g = lane >> 5;
+    const PmItem it = pm_find(a, cut, w, lds);
+    if (kvh == 0 && tid == 0 && w < part_items) items[w] = it;                   // for the joining kernel
+    if (it.row < 0) return;
+    const PaRow row = pa_row(a, it.row);
+    const int group = a.heads / a.kv_heads, lbs = 31 - __clz(a.block);
+    const int64_t queries = (int64_t) row.fresh * group, q0 = (int64_t) it.tile * PM_ROWS;
+    const int last_token = (int) ((min(q0 + PM_ROWS, queries) - 1) / group);
+    const int all_tiles = (int) ((min((int64_t) row.past + last_token + 1, (int64_t) row.keys) + PA_KEYS - 1) / PA_KEYS);
+    const int t_first = (int) ((int64_t) all_tiles * it.piece / it.pieces), t_last = (int) ((int64_t) all_tiles * (it.piece + 1) / it.pieces);
+
+    // this lane's query
+    const int64_t r = q0 + wave * 32 + c;
+    const bool in = r < queries;
+    const int token = in ? (int) (r / group) : 0, head = kvh * group + (in ? (int) (r % group) : 0);
+    const int limit = in ? (int) min((int64_t) row.past + token, (int64_t) row.keys - 1) : -1;
+    // the first and the last key that bound what this wave has to mask and to walk
+    const int64_t wave_q0 = q0 + wave * 32;
+    const int wave_free = wave_q0 < queries ? (int) min((int64_t) row.past + (int) (wave_q0 / group), (int64_t) row.keys - 1) : -1;
+    const int wave_end = wave_q0 < queries ? (int) min((int64_t) row.past + (int) ((min(wave_q0 + 32, queries) - 1) / group), (int64_t) row.keys - 1) : -1;
+    f16x8 qf[KB];
+    {
+        const f16* q = a.q + (size_t) (row.start + token) * a.q_stride + (size_t) head * a.hd;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            f16x8 x = pa_query(a, q, (int64_t) row.past + token, 16 * kb + 8 * g);
+            if (!in) x = (f16x8) {};
+            qf[kb] = x;
+        }
+    }
+
+    const int32_t* table = a.table + (size_t) it.row * a.width;
+    const size_t page_bytes = (size_t) a.block * a.hd16;
+    // staging roles: keys: piece i of this thread is column chunk k_ch of key k_key + (256 / KB) * i; values: 16 keys v_kc of column v_d + 64 * i
+    const int k_ch = tid % KB, k_key = tid / KB, v_kc = tid & 3, v_d = tid >> 2;
+    constexpr int K_STEP = 256 / KB;
+    struct Ids { int k[PIECES]; int v; };
+    struct Stage { uint4 k[PIECES], v[PIECES]; float ks[PIECES], vs; int n; uint32_t there; };   // n: valid keys of the value pieces; there: a bit for each 16 keys
+    auto look = [&](int tile) -> Ids {
+        Ids id;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int p = (tile * PA_KEYS + k_key + K_STEP * i) >> lbs;
+            id.k[i] = p < a.width ? table[p] : -1;
+        }
+        const int p = (tile * PA_KEYS + 16 * v_kc) >> lbs;
+        id.v = p < a.width ? table[p] : -1;
+        return id;
+    };
+    auto fetch = [&](int tile, const Ids& id, Stage& st) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int key = tile * PA_KEYS + k_key + K_STEP * i;
+            const size_t kb = (size_t) (id.k[i] >= 0 && id.k[i] < a.blocks ? id.k[i] : 0) * a.kv_heads + kvh;
+            st.k[i] = *(const uint4*) (a.kp + kb * page_bytes + (size_t) (key & (a.block - 1)) * a.hd16 + (16 * k_ch < a.hd16 ? 16 * k_ch : 0));
+            st.ks[i] = paged_pow2(paged_scale_exp<CODE>(a.ks[kb]));
+        }
+        const bool ok = id.v >= 0 && id.v < a.blocks;
+        const size_t vb = (size_t) (ok ? id.v : 0) * a.kv_heads + kvh;
+        const int key = tile * PA_KEYS + 16 * v_kc;
+        const uint8_t* vp = a.vp + vb * page_bytes + (key & (a.block - 1));
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) st.v[i] = *(const uint4*) (vp + (size_t) (v_d + 64 * i < a.hd16 ? v_d + 64 * i : 0) * a.block);
+        st.vs = paged_pow2(paged_scale_exp<CODE>(a.vs[vb]));
+        st.n = ok ? min(max(row.keys - key, 0), 16) : 0;
+        st.there = (uint32_t) __ballot(ok) & 15;
+    };
+    auto store = [&](Stage& st, unsigned char* buf) {
+        if (st.n < 16) {                                          // bytes that hold no value may be anything, NaN too: a weight of 0 does not hide it
+            uint32_t mask[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mask[i] = st.n >= 4 * i + 4 ? 0xffffffffu : st.n <= 4 * i ? 0u : (1u << (8 * (st.n - 4 * i))) - 1;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) { st.v[i].x &= mask[0]; st.v[i].y &= mask[1]; st.v[i].z &= mask[2]; st.v[i].w &= mask[3]; }
+        }
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int key = k_key + K_STEP * i, kt = key >> 5, m = 8 * ((key >> 2) & 3) + 4 * ((key >> 4) & 1) + (key & 3);
+            unsigned char* p = buf + (kt * KB + k_ch) * 1024;
+            *(f16x8*) (p + ((m ^ (k_ch & 7)) << 4)) = pa_numbers<CODE>(st.k[i].x, st.k[i].y, st.ks[i]);
+            *(f16x8*) (p + (((32 + m) ^ (k_ch & 7)) << 4)) = pa_numbers<CODE>(st.k[i].z, st.k[i].w, st.ks[i]);
+            const int d = v_d + 64 * i;
+            const int slot = ((v_kc & 1) * 32 + (d & 31)) ^ (v_kc << 1);
+            unsigned char* q = buf + K_BYTES + ((v_kc >> 1) * 2 * DT + (d >> 5)) * 1024 + (slot << 4);
+            *(f16x8*) q = pa_numbers<CODE>(st.v[i].x, st.v[i].y, st.vs);
+            *(f16x8*) (q + DT * 1024) = pa_numbers<CODE>(st.v[i].z, st.v[i].w, st.vs);
+        }
+    };
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[t][j] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float c1 = a.scale * 1.44269504f;
+
+    Stage st;
+    Ids id;
+    uint32_t there = 15;
+    if (t_first < t_last) {
+        fetch(t_first, look(t_first), st);
+        there = st.there;
+        store(st, lds);
+        if (t_first + 1 < t_last) fetch(t_first + 1, look(t_first + 1), st);
+        if (t_first + 2 < t_last) id = look(t_first + 2);
+    }
+    for (int tile = t_first; tile < t_last; ++tile) {
+        unsigned char* buf = lds + ((tile - t_first) & 1) * BUF;
+        const uint32_t now = there;
+        __syncthreads();                                          // this tile is in `buf`, and every wave is through with the other one
+        if (tile + 1 < t_last) {
+            there = st.there;
+            store(st, lds + ((tile + 1 - t_first) & 1) * BUF);
+            if (tile + 2 < t_last) {
+                fetch(tile + 2, id, st);
+                if (tile + 3 < t_last) id = look(tile + 3);
+            }
+        }
+        if (tile * PA_KEYS > wave_end) continue;
+        const bool border = tile * PA_KEYS + PA_KEYS - 1 > wave_free || now != 15;
+        f32x16 s[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[kt][j] = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const f16x8 k = *(const f16x8*) (buf + (kt * KB + kb) * 1024 + ((lane ^ (kb & 7)) << 4));
+                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[kb], s[kt], 0, 0, 0);
+            }
+        }
+        float mx = -INFINITY;
+        if (border) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (!(now >> (2 * kt + g) & 1) || tile * PA_KEYS + 32 * kt + 16 * g + j > limit) s[kt][j] = -INFINITY;
+        }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[kt][j]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c1;
+        const float mn = fmaxf(m, mx);
+        if (__any(mn > m)) {
+            const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= keep;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[t][j] *= keep;
+            m = mn;
+        }
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        f16x8 p[2][2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[kt][j], c1, -ref));
+                l += e;
+                p[kt][j >> 3][j & 7] = (f16) e;
+            }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    const f16x8 v = *(const f16x8*) (buf + K_BYTES + ((kt * 2 + h) * DT + t) * 1024 + ((lane ^ (4 * kt + 2 * g)) << 4));
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[kt][h], o[t], 0, 0, 0);
+                }
+    }
+
+    // ---- out: row j of a product is column 32 t + 8 * (j >> 2) + 4 g + (j & 3)
+    l += __shfl_xor(l, 32, 64);
+    if (!in) return;
+    if (it.pieces == 1) {
+        f16* out = a.out + (size_t) (row.start + token) * a.heads * a.hd + (size_t) head * a.hd;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d = 32 * t + 8 * j + 4 * g;
+                if (d >= a.hd) continue;                              // (head_dim is a multiple of four)
+                f16x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (f16) (o[t][4 * j + e] * inv);
+                *(f16x4*) (out + d) = x;
+            }
+    } else {
+        float* part = parts + (((size_t) w * a.kv_heads + kvh) * PM_ROWS + wave * 32 + c) * (DP + 4);
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *(f32x4*) (part + 32 * t + 8 * j + 4 * g) = (f32x4) {o[t][4 * j], o[t][4 * j + 1], o[t][4 * j + 2], o[t][4 * j + 3]};
+        if (g == 0) { part[DP] = m; part[DP + 1] = l; }
+    }
+}
+
+// The pieces of a query tile joined, in order: one wave per query.
+__global__ __launch_bounds__(256) void paged_attn_join_many_kernel(PagedAttn a, const float* __restrict__ parts, const PmItem* __restrict__ items, int dp)
+{
+    const int w = blockIdx.x, kvh = blockIdx.y, q = blockIdx.z * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const PmItem it = items[w];
+    if (it.row < 0 || it.piece != 0 || it.pieces < 2) return;
+    const PaRow row = pa_row(a, it.row);
+    const int group = a.heads / a.kv_heads;
+    const int64_t r = (int64_t) it.tile * PM_ROWS + q;
+    if (r >= (int64_t) row.fresh * group) return;
+    const size_t step = (size_t) a.kv_heads * PM_ROWS * (dp + 4);
+    const float* p0 = parts + (((size_t) w * a.kv_heads + kvh) * PM_ROWS + q) * (dp + 4);
+    float top = -INFINITY;
+    for (int k = lane; k < it.pieces; k += 64) top = fmaxf(top, p0[k * step + dp]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int k = 0; k < it.pieces; ++k) {
+        const float* p = p0 + k * step;
+        const float f = p[dp] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[dp] - top);
+        sum += f * p[dp + 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (64 * j < dp) o[j] += f * p[64 * j + lane];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    f16* out = a.out + (size_t) (row.start + (int) (r / group)) * a.heads * a.hd + (size_t) (kvh * group + (int) (r % group)) * a.hd;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) if (64 * j + lane < a.hd) out[64 * j + lane] = (f16) (o[j] * inv);
+}
+
+// How a call is cut, from what the host knows: the kernel for few queries takes rows of up to `few` of them (NT tiles of 16)
+struct PaPlan {
+    int dp, nt, group, items, rows_y; PaCut cut; size_t first_bytes, part_bytes;          // few queries
+    bool many; int many_items, many_parts; PaCut many_cut; size_t many_item_bytes, many_part_bytes;
+    size_t bytes() const { return first_bytes + part_bytes + many_item_bytes + many_part_bytes; }
+};
+static size_t pa_round(size_t n) { return (n + 255) / 256 * 256; }
+
+static PaPlan pa_plan(int n, int rows, int max_new, int heads, int kv_heads, int hd, int width, int block)
+{
+    PaPlan p;
+    p.dp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+    p.group = heads / kv_heads;
+    const int64_t queries = (int64_t) (max_new < rows ? max_new : rows) * p.group;
+    const int most = p.dp == 256 ? 16 : 32;
+    p.nt = queries <= 16 || queries > most ? 1 : 2;
+    p.many = queries > most;
+    p.cut.few = 16 * p.nt;
+    p.rows_y = (int) (queries < p.cut.few ? queries : p.cut.few);
+    p.cut.target = kv_heads >= 1024 ? 1 : 1024 / kv_heads;
+    p.cut.min_piece = PA_WAVES;
+    p.cut.split = n <= PA_MAX_ROWS && (int64_t) width * block > p.cut.min_piece * PA_KEYS;
+    p.items = n > PA_MAX_ROWS || !p.cut.split ? n : p.cut.target + n;
+    p.first_bytes = pa_round((size_t) n * sizeof(int2));
+    p.part_bytes = p.cut.split ? pa_round((size_t) p.items * kv_heads * pa_part_floats(p.dp, p.nt) * sizeof(float)) : 0;
+    p.many_items = p.many_parts = 0;
+    p.many_item_bytes = p.many_part_bytes = 0;
+    if (p.many) {
+        const int64_t fresh = (int64_t) n * max_new < rows ? (int64_t) n * max_new : rows, tiles = (fresh * p.group + PM_ROWS - 1) / PM_ROWS + n;
+        p.many_cut = {p.cut.few, kv_heads >= 512 ? 1 : 512 / kv_heads, 8, (int64_t) width * block > 8 * PA_KEYS};
+        p.many_parts = p.many_cut.split ? 2 * p.many_cut.target : 0;
+        p.many_items = (int) (tiles > p.many_parts ? tiles : p.many_parts);
+        p.many_item_bytes = pa_round((size_t) p.many_parts * sizeof(PmItem));
+        p.many_part_bytes = pa_round((size_t) p.many_parts * kv_heads * PM_ROWS * (p.dp + 4) * sizeof(float));
+    }
+    return p;
+}
+
+template <int CODE> static int pa_launch(const PagedAttn& a, const PaPlan& p, void* workspace, hipStream_t s)
+{
+    int2* firsts = (int2*) workspace;
+    float* parts = (float*) ((char*) workspace + p.first_bytes);
+    const dim3 grid((unsigned) p.items, (unsigned) a.kv_heads);
+#define PA_FEW(DP, NT) hipLaunchKernelGGL((paged_attn_few_kernel<CODE, DP, NT>), grid, dim3(PA_WAVES * 64), 0, s, a, p.cut, parts, firsts)
+    if (p.dp == 64)       { if (p.nt == 1) PA_FEW(64, 1); else PA_FEW(64, 2); }
+    else if (p.dp == 128) { if (p.nt == 1) PA_FEW(128, 1); else PA_FEW(128, 2); }
+    else                  PA_FEW(256, 1);
+#undef PA_FEW
+    EXL_LAUNCH_CHECK();
+    if (p.cut.split) {
+        hipLaunchKernelGGL(paged_attn_join_kernel, dim3((unsigned) a.n, (unsigned) p.rows_y, (unsigned) a.kv_heads), dim3(256), 0, s, a, p.cut, parts, firsts, p.dp,
+                           p.nt);
+        EXL_LAUNCH_CHECK();
+    }
+    if (p.many) {
+        PmItem* items = (PmItem*) ((char*) parts + p.part_bytes);
+        float* more = (float*) ((char*) items + p.many_item_bytes);
+        const dim3 mgrid((unsigned) p.many_items, (unsigned) a.kv_heads);
+#define PA_MANY(DP) do { static bool done[EXL_MAX_DEVICES] = {};                                                                             \
+        EXL_TRY(exl_lds_opt_in((const void*) paged_attn_many_kernel<CODE, DP>, done));                                                        \
+        hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP>), mgrid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4, s, a, p.many_cut, more, items, p.many_parts); } while (0)
+        if (p.dp == 64) PA_MANY(64); else if (p.dp == 128) PA_MANY(128); else PA_MANY(256);
+#undef PA_MANY
+        EXL_LAUNCH_CHECK();
+        if (p.many_parts) {
+            hipLaunchKernelGGL(paged_attn_join_many_kernel, dim3((unsigned) p.many_parts, (unsigned) a.kv_heads, PM_ROWS / 4), dim3(256), 0, s, a, more, items, p.dp);
+            EXL_LAUNCH_CHECK();
+        }
+    }
+    return 0;
 }
 
 extern "C" size_t exl_paged_attention_workspace(int n_rows, int rows, int max_new, int num_heads, int num_kv_heads, int head_dim, int table_width,
                                                 int block_size)
 {
-    return 0;
+    if (n_rows <= 0 || rows <= 0 || max_new <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 || table_width <= 0 ||
+        block_size <= 0) return 0;
+    const PaPlan p = pa_plan(n_rows, rows, max_new, num_heads, num_kv_heads, head_dim, table_width, block_size);
+    return p.bytes();
 }
 
 extern "C" int exl_paged_attention(const void* q, long q_stride, const int32_t* starts, const int32_t* past_lens, const int32_t* new_lens, int n_rows,
@@ -127,8 +817,8 @@ extern "C" int exl_paged_attention(const void* q, long q_stride, const int32_t* 
                    value_scales, (const f16*) sin, (const f16*) cos, (f16*) out, n_rows, rows, max_new, table_width, num_blocks, block_size, num_heads,
                    num_kv_heads, head_dim, (head_dim + 15) / 16 * 16, angle_rows, q_stride, scale > 0.f ? scale : 1.f / sqrtf((float) head_dim)};
     hipStream_t s = (hipStream_t) stream;
-    if (code == EXL_PAGE_FP8) hipLaunchKernelGGL((paged_attn_row_kernel<EXL_PAGE_FP8>), dim3(rows, num_heads), dim3(PA_TILE), 0, s, a);
-    else                   hipLaunchKernelGGL((paged_attn_row_kernel<EXL_PAGE_INT8>), dim3(rows, num_heads), dim3(PA_TILE), 0, s, a);
-    EXL_LAUNCH_CHECK();
-    return 0;
+    const PaPlan p = pa_plan(n_rows, rows, max_new, num_heads, num_kv_heads, head_dim, table_width, block_size);
+    EXL_REQUIRE(workspace && (uintptr_t) workspace % 16 == 0 && workspace_bytes >= p.bytes(), EXL_E_TOO_SMALL,
+                "paged_attention: the workspace is too small (%zu < %zu bytes) or not 16-byte aligned", workspace_bytes, p.bytes());
+    return code == EXL_PAGE_FP8 ? pa_launch<EXL_PAGE_FP8>(a, p, workspace, s) : pa_launch<EXL_PAGE_INT8>(a, p, workspace, s);
 }

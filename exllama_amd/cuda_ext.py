@@ -667,7 +667,8 @@ if not _env_on("EXL_NO_FAST_BINDING"):
             raise RuntimeError(_msg) from e
         _warnings.warn(_msg + " -- continuing on the ctypes path (same kernels, 12-18 us more host time per op call)", RuntimeWarning)
     if FAST_BINDING is not None:
-        for _name in ("q4_matmul", "rms_norm", "rope_", "q4_attn", "q4_attn_2", "q4_mlp", "attention"):
+        for _name in ("q4_matmul", "rms_norm", "rope_", "q4_attn", "q4_attn_2", "q4_mlp", "attention", "paged_slots", "paged_append",
+                      "paged_attention"):
             setattr(exllama_ext, _name, getattr(FAST_BINDING, _name))
 
 # re-exports at module level, as the reference does (cuda_ext.py:66-77)
