@@ -202,13 +202,17 @@ int paged_check_block(const char* what, int block_size, int num_blocks)
 //   amax = max |x| (x clamped to +-top * 2^hi, NaN left out), e = the least exponent with amax <= top * 2^e; a run that does not start
 //   its page keeps the page's earlier tokens: e = max(e, the page's), their codes move by 2^(e_old - e);  code = round(x / 2^e)
 // Keys are rotated first when sin / cos are given: lo * cos - hi * sin in 64 bits and rounded to odd in 32, so that the code is one
-// rounding of the exact rotation.  One wave does a run of one head; nothing is shared between waves.
+// rounding of the exact rotation.  Short runs (single tokens, a few drafted ones) take a wave each; from APPEND_LONG tokens on, and
+// head_dim % 16 == 0, the whole workgroup takes the run: every number is read once and stays in registers between the maximum and the
+// rounding, and the values' codes are transposed in LDS.
 struct AppendArgs {
     const f16* k; const f16* v; const int32_t* slots; const int32_t* positions; const f16* sin; const f16* cos;
     uint8_t* kp; uint8_t* vp; float* ks; float* vs;
     int rows, kv_heads, hd, hd16, block, blocks, chunk, angle_rows;
     long k_stride, v_stride;
 };
+
+#define APPEND_LONG 8
 
 // a * b - c * d (sign = -1) or a * b + c * d of fp16 numbers: exact products, the sum in 64 bits, rounded to odd (a later rounding to
 // fewer bits then is the exact value's)
@@ -306,12 +310,140 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int h, int t, in
     }
 }
 
-template <int CODE, bool ROPE> __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
+// The exponent of a page that a run of largest magnitude `amax` at offset `off` joins; `old`: the exponent before (== the new one: nothing moves)
+template <int CODE> __device__ __forceinline__ int append_exp(float amax, int off, const float* scale, int& old)
 {
-    const int h = blockIdx.y, lane = threadIdx.x & 63;
-    const int t0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * a.chunk;
-    const int t1 = min(t0 + a.chunk, a.rows);
-    for (int t = t0; t < t1; ++t) {
+    const float cap = PagedRange<CODE>::top * paged_pow2(PagedRange<CODE>::hi);
+    const int e = paged_exp_for<CODE>(fminf(amax, cap));
+    old = off > 0 ? paged_scale_exp<CODE>(*scale) : e;
+    return max(e, old);
+}
+
+// A run of n tokens by the whole workgroup (256 threads).  `per` = head_dim / 16 threads share a token, each with 16 of its numbers: columns
+// 8 j .. 8 j + 7 of both halves of a key (what a rotation pairs), columns 16 j .. 16 j + 15 of a value.  P: passes over the tokens.
+template <int CODE, bool ROPE, int P>
+__device__ __forceinline__ void append_run_wide(const AppendArgs& a, int h, int t, int n, int page, int off, uint8_t* lds, float* red)
+{
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per = a.hd >> 4, step = 256 / per, half = a.hd >> 1;
+    const int j = tid % per, i0 = tid / per;
+    const bool on = i0 < step;                                    // (256 is no multiple of head_dim / 16: 80, 96, ...)
+    float k[P][16];
+    f16x8 v[P][2];
+    float kmax = 0.f, vmax = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int i = i0 + p * step;
+        if (!on || i >= n) continue;
+        const f16* kr = a.k + (size_t) (t + i) * a.k_stride + (size_t) h * a.hd + 8 * j;
+        const f16* vr = a.v + (size_t) (t + i) * a.v_stride + (size_t) h * a.hd + 16 * j;
+        const f16x8 lo = *(const f16x8_a8*) kr, hi = *(const f16x8_a8*) (kr + half);
+        v[p][0] = *(const f16x8_a8*) vr;
+        v[p][1] = *(const f16x8_a8*) (vr + 8);
+        if (ROPE) {
+            const size_t at = (size_t) min(max(a.positions[t + i], 0), a.angle_rows - 1) * a.hd + 8 * j;
+            const f16x8 sl = *(const f16x8_a8*) (a.sin + at), sh = *(const f16x8_a8*) (a.sin + at + half);
+            const f16x8 cl = *(const f16x8_a8*) (a.cos + at), ch = *(const f16x8_a8*) (a.cos + at + half);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                k[p][e] = rot_odd(lo[e], cl[e], hi[e], sl[e], -1.f);
+                k[p][8 + e] = rot_odd(hi[e], ch[e], lo[e], sh[e], 1.f);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { k[p][e] = (float) lo[e]; k[p][8 + e] = (float) hi[e]; }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            kmax = fmaxf(kmax, fabsf(k[p][e]));
+            vmax = fmaxf(vmax, fabsf((float) v[p][e >> 3][e & 7]));
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { kmax = fmaxf(kmax, __shfl_xor(kmax, o, 64)); vmax = fmaxf(vmax, __shfl_xor(vmax, o, 64)); }
+    __syncthreads();                                              // (the last run's LDS is free)
+    if (lane == 0) { red[wave] = kmax; red[4 + wave] = vmax; }
+    __syncthreads();
+    kmax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    vmax = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+    const size_t ph = (size_t) page * a.kv_heads + h, at = ph * a.block * a.hd16;
+    uint8_t* kc = a.kp + at;
+    uint8_t* vc = a.vp + at;
+    int kold, vold;
+    const int ke = append_exp<CODE>(kmax, off, a.ks + ph, kold), ve = append_exp<CODE>(vmax, off, a.vs + ph, vold);
+    __syncthreads();                                              // every thread has read the scales
+    if (tid == 0) { a.ks[ph] = paged_pow2(ke); a.vs[ph] = paged_pow2(ve); }
+    if (ke != kold) {                                             // the earlier tokens' codes under the new scale
+        const float f = paged_pow2(kold - ke);
+        for (int w = tid; w < off * (a.hd16 >> 2); w += 256) {
+            float x[4];
+            paged_decode4<CODE>(((const uint32_t*) kc)[w], x);
+            ((uint32_t*) kc)[w] = paged_encode4<CODE>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+        }
+    }
+    if (ve != vold) {
+        const float f = paged_pow2(vold - ve);
+        const int words = a.block >> 2;
+        for (int w = tid; w < a.hd16 * words; w += 256) {
+            const int first = (w % words) * 4;
+            if (first >= off) continue;
+            float x[4];
+            paged_decode4<CODE>(((const uint32_t*) vc)[w], x);
+            const uint32_t now = paged_encode4<CODE>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+            if (first + 4 <= off) ((uint32_t*) vc)[w] = now;
+            else for (int b = 0; b < off - first; ++b) vc[4 * w + b] = (uint8_t) (now >> (8 * b));       // (the word's other bytes belong to the new tokens)
+        }
+    }
+    const float kinv = paged_pow2(-ke), vinv = paged_pow2(-ve);
+    const int row = a.block + 4;                                  // bytes of a value column in LDS: the columns of a wave's threads lie in different banks
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int i = i0 + p * step;
+        if (!on || i >= n) continue;
+        uint32_t c[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) c[w] = paged_encode4<CODE>(k[p][4 * w] * kinv, k[p][4 * w + 1] * kinv, k[p][4 * w + 2] * kinv, k[p][4 * w + 3] * kinv);
+        uint8_t* kr = kc + (size_t) (off + i) * a.hd16 + 8 * j;
+        *(uint2*) kr = make_uint2(c[0], c[1]);
+        *(uint2*) (kr + half) = make_uint2(c[2], c[3]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const f16x8 x = v[p][w >> 1];
+            const int e = (w & 1) * 4;
+            const uint32_t u = paged_encode4<CODE>((float) x[e] * vinv, (float) x[e + 1] * vinv, (float) x[e + 2] * vinv, (float) x[e + 3] * vinv);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) lds[(16 * j + 4 * w + b) * row + off + i] = (uint8_t) (u >> (8 * b));
+        }
+    }
+    __syncthreads();
+    const int pieces = a.block >> 4;                              // 16 tokens of a column at a time
+    for (int w = tid; w < a.hd * pieces; w += 256) {
+        const int d = w / pieces, first = (w % pieces) * 16;
+        const uint8_t* src = lds + d * row + first;
+        uint8_t* dst = vc + (size_t) d * a.block + first;
+        if (first >= off && first + 16 <= off + n) {
+            const uint32_t* x = (const uint32_t*) src;
+            *(uint4*) dst = make_uint4(x[0], x[1], x[2], x[3]);
+        } else {
+            for (int b = max(first, off); b < min(first + 16, off + n); ++b) dst[b - first] = src[b - first];
+        }
+    }
+}
+
+// One workgroup = `chunk` token rows of one head: it does the runs that begin there.  P = 0: a wave for every run.
+template <int CODE, bool ROPE, int P> __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
+{
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ float red[8];
+    __shared__ int longs[16][4];                                  // the long runs: token row, tokens, page, offset
+    __shared__ int count;
+    const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int t0 = blockIdx.x * a.chunk, t1 = min(t0 + a.chunk, a.rows);
+    if (P) {
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+    }
+    for (int t = t0 + wave; t < t1; t += 4) {
         const int slot = a.slots[t];
         if (slot < 0 || slot / a.block >= a.blocks) continue;
         const int page = slot / a.block, off = slot % a.block;
@@ -325,8 +457,17 @@ template <int CODE, bool ROPE> __global__ __launch_bounds__(256) void paged_appe
             if (m) break;
         }
         n = min(n, a.block - off);
+        if (P && n >= APPEND_LONG) {
+            if (lane == 0) { const int x = atomicAdd(&count, 1); longs[x][0] = t; longs[x][1] = n; longs[x][2] = page; longs[x][3] = off; }
+            continue;
+        }
         append_run<CODE, ROPE, true>(a, h, t, n, page, off);
         append_run<CODE, ROPE, false>(a, h, t, n, page, off);
+    }
+    if (P) {
+        __syncthreads();
+        for (int x = 0; x < count; ++x)                           // (runs of different pages: their order does not matter)
+            append_run_wide<CODE, ROPE, P ? P : 1>(a, h, longs[x][0], longs[x][1], longs[x][2], longs[x][3], lds, red);
     }
 }
 
@@ -347,18 +488,20 @@ extern "C" int exl_paged_append(const void* key_states, const void* value_states
     if (rows == 0) return 0;
     AppendArgs a = {(const f16*) key_states, (const f16*) value_states, slots, positions, (const f16*) sin, (const f16*) cos,
                     (uint8_t*) key_pages, (uint8_t*) value_pages, key_scales, value_scales, rows, num_kv_heads, head_dim, (head_dim + 15) / 16 * 16,
-                    block_size, num_blocks, 1, angle_rows, key_stride, value_stride};
-    const long waves = (long) rows * num_kv_heads;
-    a.chunk = waves <= 4096 ? 1 : (int) (waves / 4096 < 16 ? waves / 4096 : 16);
-    const dim3 grid((unsigned) ((rows + 4L * a.chunk - 1) / (4L * a.chunk)), (unsigned) num_kv_heads);
+                    block_size, num_blocks, 4, angle_rows, key_stride, value_stride};
+    const int passes = head_dim % 16 ? 0 : (block_size * (head_dim / 16) + 255) / 256;       // (256 / (head_dim / 16) tokens a pass, or a few less)
+    a.chunk = (long) rows * num_kv_heads <= 16384 ? 4 : 16;       // few rows: a run for every wave at once
+    const dim3 grid((unsigned) ((rows + a.chunk - 1L) / a.chunk), (unsigned) num_kv_heads);
+    const size_t lds = passes ? (size_t) head_dim * (block_size + 4) : 0;
     hipStream_t s = (hipStream_t) stream;
-    if (code == EXL_PAGE_FP8) {
-        if (sin) hipLaunchKernelGGL((paged_append_kernel<EXL_PAGE_FP8, true>), grid, dim3(256), 0, s, a);
-        else     hipLaunchKernelGGL((paged_append_kernel<EXL_PAGE_FP8, false>), grid, dim3(256), 0, s, a);
-    } else {
-        if (sin) hipLaunchKernelGGL((paged_append_kernel<EXL_PAGE_INT8, true>), grid, dim3(256), 0, s, a);
-        else     hipLaunchKernelGGL((paged_append_kernel<EXL_PAGE_INT8, false>), grid, dim3(256), 0, s, a);
-    }
+    const int p = !passes ? 0 : passes * (256 / (head_dim / 16)) >= block_size ? passes : passes + 1;
+#define APPEND(C, R, P) hipLaunchKernelGGL((paged_append_kernel<C, R, P>), grid, dim3(256), lds, s, a)
+#define APPEND_P(C, R) do { if (p == 0) APPEND(C, R, 0); else if (p == 1) APPEND(C, R, 1); else if (p == 2) APPEND(C, R, 2); else if (p <= 4) APPEND(C, R, 4); \
+                            else APPEND(C, R, 8); } while (0)
+    if (code == EXL_PAGE_FP8) { if (sin) APPEND_P(EXL_PAGE_FP8, true); else APPEND_P(EXL_PAGE_FP8, false); }
+    else                      { if (sin) APPEND_P(EXL_PAGE_INT8, true); else APPEND_P(EXL_PAGE_INT8, false); }
+#undef APPEND_P
+#undef APPEND
     EXL_LAUNCH_CHECK();
     return 0;
 }
