@@ -38,18 +38,24 @@ template <int CODE> __device__ __forceinline__ int paged_exp_for(float amax)
     return min(max(e, R::lo), R::hi);
 }
 
-// four codes of y = x / scale: one rounding to nearest even, saturating; NaN stays NaN (e4m3) or becomes 0 (int8)
-template <int CODE> __device__ __forceinline__ uint32_t paged_encode4(float a, float b, float c, float d)
+// four codes of x * inv, inv = 1 / scale: one rounding to nearest even; NaN stays NaN (e4m3) or becomes 0 (int8).  |x| * inv <= top, unless
+// SATURATE (one instruction or two for a number where every comparison counts: the clamp is for pages with numbers beyond the last scale's)
+template <int CODE, bool SATURATE> __device__ __forceinline__ uint32_t paged_encode4(float a, float b, float c, float d, float inv)
 {
-    const float t = PagedRange<CODE>::top;
-    auto clamp = [&](float y) { return y > t ? t : y < -t ? -t : y; };
-    a = clamp(a); b = clamp(b); c = clamp(c); d = clamp(d);
-    if (CODE == EXL_PAGE_FP8) {
-        int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-        return (uint32_t) __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+    if (SATURATE) {
+        const float t = PagedRange<CODE>::top / inv;
+        auto clamp = [&](float y) { return y > t ? t : y < -t ? -t : y; };
+        a = clamp(a); b = clamp(b); c = clamp(c); d = clamp(d);
     }
-    auto whole = [](float y) { return (uint32_t) (uint8_t) (int8_t) (y == y ? (int) rintf(y) : 0); };
-    return whole(a) | whole(b) << 8 | whole(c) << 16 | whole(d) << 24;
+    if (CODE == EXL_PAGE_FP8) {
+        const int r = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+        return (uint32_t) __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, r, true);
+    }
+    // 1.5 * 2^23 + y has the nearest whole number in its low byte (two's complement); a NaN of fp16 or fp32 arithmetic has zeros there
+    const float base = 12582912.f;
+    const uint32_t ab = __builtin_amdgcn_perm(__float_as_uint(fmaf(b, inv, base)), __float_as_uint(fmaf(a, inv, base)), 0x0c0c0400u);
+    const uint32_t cd = __builtin_amdgcn_perm(__float_as_uint(fmaf(d, inv, base)), __float_as_uint(fmaf(c, inv, base)), 0x04000c0cu);
+    return ab | cd;
 }
 
 // the four numbers of a word of codes

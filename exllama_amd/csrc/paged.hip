@@ -1,5 +1,6 @@
 // The paged 8-bit cache (paged.h): block tables and slot maps from request lengths, and the append of new keys and values.
 #include "paged.h"
+#include <type_traits>
 
 // ---- block tables and slot maps ---------------------------------------------------------------------------------------------------
 // For every row b, in order (all sums exclusive prefix sums over the rows):
@@ -201,32 +202,39 @@ int paged_check_block(const char* what, int block_size, int num_blocks)
 // A RUN is the longest stretch of token rows whose slots are consecutive inside one page.  Per run and kv head, keys and values each:
 //   amax = max |x| (x clamped to +-top * 2^hi, NaN left out), e = the least exponent with amax <= top * 2^e; a run that does not start
 //   its page keeps the page's earlier tokens: e = max(e, the page's), their codes move by 2^(e_old - e);  code = round(x / 2^e)
-// Keys are rotated first when sin / cos are given: lo * cos - hi * sin in 64 bits and rounded to odd in 32, so that the code is one
-// rounding of the exact rotation.  Short runs (single tokens, a few drafted ones) take a wave each; from APPEND_LONG tokens on, and
+// Keys are rotated first when sin / cos are given; the code is one rounding of the exact rotation.  Short runs (single tokens, a few drafted ones) take a wave each; from APPEND_LONG tokens on, and
 // head_dim % 16 == 0, the whole workgroup takes the run: every number is read once and stays in registers between the maximum and the
 // rounding, and the values' codes are transposed in LDS.
 struct AppendArgs {
     const f16* k; const f16* v; const int32_t* slots; const int32_t* positions; const f16* sin; const f16* cos;
     uint8_t* kp; uint8_t* vp; float* ks; float* vs;
-    int rows, kv_heads, hd, hd16, block, blocks, chunk, angle_rows;
-    long k_stride, v_stride;
+    int rows, kv_heads, hd, hd16, lbs, blocks, chunk, angle_rows;  // lbs: log2 of the block size
+    int k_stride, v_stride;
+    uint32_t by_words, by_16, by_4;                               // dividing thread numbers by hd16 / 4, hd / 16 and hd / 4: n * by >> 32
 };
+
+// n / d for n < 2^16, d <= 64 (by = 2^32 / d rounded up, 0 for d = 1); a division by a number in a register is twenty instructions
+__device__ __forceinline__ int over(int n, uint32_t by) { return by ? (int) __umulhi((uint32_t) n, by) : n; }
 
 #define APPEND_LONG 8
 
-// a * b - c * d (sign = -1) or a * b + c * d of fp16 numbers: exact products, the sum in 64 bits, rounded to odd (a later rounding to
-// fewer bits then is the exact value's)
-__device__ __forceinline__ float rot_odd(f16 a, f16 b, f16 c, f16 d, float sign)
+// a * b + sign * c * d of fp16 numbers as a 32-bit number that rounds to a code (7 bits at most) and compares with a scale's border as the
+// exact one does.  One fma of an exact product rounds once; a second rounding can only go wrong where the first ended on a border, that
+// is with 15 zeros below: there the sum is rounded to odd instead (its error is exact by Knuth's two-sum; an inexact even sum moves one
+// step towards the exact one).  Rounding every sum to odd made 16 instructions a number instead of 5.
+__device__ __forceinline__ float rot_code(f16 a, f16 b, f16 c, f16 d, float sign)
 {
-    const float p = (float) a * (float) b, q = (float) c * (float) d * sign;
-    const double s = (double) p + (double) q;
-    float r = (float) s;
-    if ((double) r != s && s == s) {
-        uint32_t u = __float_as_uint(r);
-        if (fabs((double) r) > fabs(s)) u -= 1;                // towards zero
-        r = __uint_as_float(u | 1);
+#pragma clang fp contract(off)
+    const float q = (float) c * (float) d * sign;
+    float s = __builtin_fmaf((float) a, (float) b, q);
+    if (__any((__float_as_uint(s) & 0x7fff) == 0)) {
+        const float p = (float) a * (float) b;
+        const float bb = s - p;
+        const float err = (p - (s - bb)) + (q - bb);
+        const uint32_t u = __float_as_uint(s);
+        if (!(u & 1) && (err < 0.f || err > 0.f)) s = __uint_as_float((err < 0.f) == (s < 0.f) ? u + 1 : u - 1);
     }
-    return r;
+    return s;
 }
 
 // x of four columns d .. d + 3 of a key or value row; zeros behind head_dim
@@ -246,181 +254,185 @@ template <bool ROPE> __device__ __forceinline__ void append_load(const f16* row,
     for (int i = 0; i < 4; ++i) {
         const int c = d + i;
         const f16 o = row[c < half ? c + half : c - half];
-        x[i] = rot_odd(v[i], cos[c], o, sin[c], c < half ? -1.f : 1.f);
+        x[i] = rot_code(v[i], cos[c], o, sin[c], c < half ? -1.f : 1.f);
     }
 }
 
-template <int CODE, bool ROPE, bool IS_KEY>
-__device__ __forceinline__ void append_run(const AppendArgs& a, int h, int t, int n, int page, int off)
-{
-    const int lane = threadIdx.x & 63;
-    const f16* x0 = IS_KEY ? a.k + (size_t) t * a.k_stride + (size_t) h * a.hd : a.v + (size_t) t * a.v_stride + (size_t) h * a.hd;
-    const long stride = IS_KEY ? a.k_stride : a.v_stride;
-    uint8_t* codes = (IS_KEY ? a.kp : a.vp) + ((size_t) page * a.kv_heads + h) * a.block * a.hd16;
-    float* scale = (IS_KEY ? a.ks : a.vs) + (size_t) page * a.kv_heads + h;
-    const int per = a.hd16 >> 2, words = n * per;
-    const float cap = PagedRange<CODE>::top * paged_pow2(PagedRange<CODE>::hi);
-    auto fetch = [&](int w, float (&x)[4], int& i, int& d) {
-        i = w / per;
-        d = (w - i * per) * 4;
-        const int pos = ROPE ? min(max(a.positions[t + i], 0), a.angle_rows - 1) : 0;
-        append_load<ROPE && IS_KEY>(x0 + (size_t) i * stride, a.sin + (size_t) pos * a.hd, a.cos + (size_t) pos * a.hd, d, a.hd, x);
-    };
-    float amax = 0.f;
-    for (int w = lane; w < words; w += 64) {
-        float x[4]; int i, d;
-        fetch(w, x, i, d);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fabsf(x[j]));           // (fmaxf leaves a NaN out)
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-    int e = paged_exp_for<CODE>(fminf(amax, cap));
-    if (off > 0) {
-        const int old = paged_scale_exp<CODE>(*scale);
-        if (e <= old) e = old;
-        else {                                                  // the earlier tokens' codes under the new scale
-            const float f = paged_pow2(old - e);
-            const int old_words = IS_KEY ? off * per : a.hd16 * (a.block >> 2);
-            for (int w = lane; w < old_words; w += 64) {
-                uint32_t* p = (uint32_t*) codes + w;
-                const int first = IS_KEY ? 0 : (w % (a.block >> 2)) * 4;       // values: tokens first .. first + 3 of one column
-                if (!IS_KEY && first >= off) continue;
-                const uint32_t was = *p;
-                float x[4];
-                paged_decode4<CODE>(was, x);
-                const uint32_t now = paged_encode4<CODE>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
-                const int left = IS_KEY ? 4 : off - first;
-                const uint32_t mask = left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1;
-                *p = (now & mask) | (was & ~mask);
-            }
-        }
-    }
-    if (lane == 0) *scale = paged_pow2(e);
-    const float inv = paged_pow2(-e);
-    for (int w = lane; w < words; w += 64) {
-        float x[4]; int i, d;
-        fetch(w, x, i, d);
-        const uint32_t c = paged_encode4<CODE>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-        if (IS_KEY) *(uint32_t*) (codes + (size_t) (off + i) * a.hd16 + d) = c;
-        else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) codes[(size_t) (d + j) * a.block + off + i] = (uint8_t) (c >> (8 * j));
-        }
-    }
-}
-
-// The exponent of a page that a run of largest magnitude `amax` at offset `off` joins; `old`: the exponent before (== the new one: nothing moves)
-template <int CODE> __device__ __forceinline__ int append_exp(float amax, int off, const float* scale, int& old)
+// The exponent of a page that numbers of largest magnitude `amax` join at offset `off`; `old`: the exponent before (== the new one: nothing moves)
+template <int CODE> __device__ __forceinline__ int append_exp(float amax, int off, float scale, int& old)
 {
     const float cap = PagedRange<CODE>::top * paged_pow2(PagedRange<CODE>::hi);
     const int e = paged_exp_for<CODE>(fminf(amax, cap));
-    old = off > 0 ? paged_scale_exp<CODE>(*scale) : e;
+    old = off > 0 ? paged_scale_exp<CODE>(scale) : e;
     return max(e, old);
 }
 
-// A run of n tokens by the whole workgroup (256 threads).  `per` = head_dim / 16 threads share a token, each with 16 of its numbers: columns
-// 8 j .. 8 j + 7 of both halves of a key (what a rotation pairs), columns 16 j .. 16 j + 15 of a value.  P: passes over the tokens.
+// The codes of a page's first `off` tokens under a scale that is 1 / f of what it was, by `threads` threads
+template <int CODE> __device__ __forceinline__ void append_move_keys(uint8_t* codes, int off, int hd16, float f, int thread, int threads)
+{
+    for (int w = thread; w < off * (hd16 >> 2); w += threads) {
+        float x[4];
+        paged_decode4<CODE>(((const uint32_t*) codes)[w], x);
+        ((uint32_t*) codes)[w] = paged_encode4<CODE, false>(x[0], x[1], x[2], x[3], f);
+    }
+}
+template <int CODE> __device__ __forceinline__ void append_move_values(uint8_t* codes, int off, int hd16, int lbs, float f, int thread, int threads)
+{
+    for (int w = thread; w < hd16 << (lbs - 2); w += threads) {
+        const int first = (w & ((1 << (lbs - 2)) - 1)) * 4;
+        if (first >= off) continue;
+        float x[4];
+        paged_decode4<CODE>(((const uint32_t*) codes)[w], x);
+        const uint32_t now = paged_encode4<CODE, false>(x[0], x[1], x[2], x[3], f);
+        if (first + 4 <= off) ((uint32_t*) codes)[w] = now;
+        else for (int b = 0; b < off - first; ++b) codes[4 * w + b] = (uint8_t) (now >> (8 * b));          // (the word's other bytes belong to the new tokens)
+    }
+}
+
+// A short run by one wave: a lane has four columns of a token, of the key and of the value at once (one round of loads and one of shuffles).
+template <int CODE, bool ROPE> __device__ __forceinline__ void append_run(const AppendArgs& a, int h, int t, int n, int page, int off)
+{
+    const int lane = threadIdx.x & 63;
+    const f16* k0 = a.k + (size_t) t * a.k_stride + (size_t) h * a.hd;
+    const f16* v0 = a.v + (size_t) t * a.v_stride + (size_t) h * a.hd;
+    const size_t ph = (size_t) page * a.kv_heads + h, at = ph * a.hd16 << a.lbs;
+    uint8_t* kc = a.kp + at;
+    uint8_t* vc = a.vp + at;
+    const float kscale = a.ks[ph], vscale = a.vs[ph];
+    const int per = a.hd16 >> 2, words = n * per;
+    const float cap = PagedRange<CODE>::top * paged_pow2(PagedRange<CODE>::hi);
+    auto fetch = [&](int w, float (&k)[4], float (&v)[4], int& i, int& d) {
+        i = over(w, a.by_words);
+        d = (w - i * per) * 4;
+        const int pos = ROPE ? min(max(a.positions[t + i], 0), a.angle_rows - 1) : 0;
+        append_load<false>(v0 + (size_t) i * a.v_stride, nullptr, nullptr, d, a.hd, v);
+        append_load<ROPE>(k0 + (size_t) i * a.k_stride, a.sin + (size_t) pos * a.hd, a.cos + (size_t) pos * a.hd, d, a.hd, k);
+    };
+    float k[4], v[4], kmax = 0.f, vmax = 0.f;
+    int i, d;
+    for (int w = lane; w < words; w += 64) {
+        fetch(w, k, v, i, d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { kmax = fmaxf(kmax, fabsf(k[j])); vmax = fmaxf(vmax, fabsf(v[j])); }       // (fmaxf leaves a NaN out)
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { kmax = fmaxf(kmax, __shfl_xor(kmax, o, 64)); vmax = fmaxf(vmax, __shfl_xor(vmax, o, 64)); }
+    int kold, vold;
+    const int ke = append_exp<CODE>(kmax, off, kscale, kold), ve = append_exp<CODE>(vmax, off, vscale, vold);
+    if (ke != kold) append_move_keys<CODE>(kc, off, a.hd16, paged_pow2(kold - ke), lane, 64);
+    if (ve != vold) append_move_values<CODE>(vc, off, a.hd16, a.lbs, paged_pow2(vold - ve), lane, 64);
+    if (lane == 0) { a.ks[ph] = paged_pow2(ke); a.vs[ph] = paged_pow2(ve); }
+    const float kinv = paged_pow2(-ke), vinv = paged_pow2(-ve);
+    const bool big = kmax > cap || vmax > cap;
+    for (int w = lane; w < words; w += 64) {
+        if (words > 64) fetch(w, k, v, i, d);
+        const uint32_t x = big ? paged_encode4<CODE, true>(k[0], k[1], k[2], k[3], kinv) : paged_encode4<CODE, false>(k[0], k[1], k[2], k[3], kinv);
+        const uint32_t y = big ? paged_encode4<CODE, true>(v[0], v[1], v[2], v[3], vinv) : paged_encode4<CODE, false>(v[0], v[1], v[2], v[3], vinv);
+        *(uint32_t*) (kc + (off + i) * a.hd16 + d) = x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vc[((d + j) << a.lbs) + off + i] = (uint8_t) (y >> (8 * j));
+    }
+}
+
+// A run of n tokens by the whole workgroup (256 threads).  Keys: head_dim / 16 threads share a token, each with columns 8 j .. 8 j + 7 of both
+// halves (what a rotation pairs).  Values: a thread has four columns of four tokens that make up one word of each column in the page,
+// so that they are transposed by the encoding itself.  P: passes of 256 threads over the page, keys and values alike.
 template <int CODE, bool ROPE, int P>
 __device__ __forceinline__ void append_run_wide(const AppendArgs& a, int h, int t, int n, int page, int off, uint8_t* lds, float* red)
 {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = a.hd >> 4, step = 256 / per, half = a.hd >> 1;
-    const int j = tid % per, i0 = tid / per;
-    const bool on = i0 < step;                                    // (256 is no multiple of head_dim / 16: 80, 96, ...)
-    float k[P][16];
-    f16x8 v[P][2];
-    float kmax = 0.f, vmax = 0.f;
+    const int per = a.hd >> 4, half = a.hd >> 1, cols = a.hd >> 2, step = over(256, a.by_16);
+    const int i0 = over(tid, a.by_16), j = tid - i0 * per;        // (256 need not be a multiple of head_dim / 16: the last threads then repeat)
+    const int w0 = off >> 2, words = ((off + n - 1) >> 2) - w0 + 1;
+    const f16* k0 = a.k + (size_t) t * a.k_stride + (size_t) h * a.hd + 8 * j;
+    const f16* v0 = a.v + (size_t) t * a.v_stride + (size_t) h * a.hd;
+    const size_t ph = (size_t) page * a.kv_heads + h, at = ph * a.hd16 << a.lbs;
+    uint8_t* kc = a.kp + at;
+    uint8_t* vc = a.vp + at;
+    const float kscale = a.ks[ph], vscale = a.vs[ph];
+    // all loads go out before anything is computed; threads behind the run's end repeat its last token, which changes no maximum
+    f16x8 lo[P], hi[P];
+    f16x4 v[P][4];
+    int pos[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        const int i = i0 + p * step;
-        if (!on || i >= n) continue;
-        const f16* kr = a.k + (size_t) (t + i) * a.k_stride + (size_t) h * a.hd + 8 * j;
-        const f16* vr = a.v + (size_t) (t + i) * a.v_stride + (size_t) h * a.hd + 16 * j;
-        const f16x8 lo = *(const f16x8_a8*) kr, hi = *(const f16x8_a8*) (kr + half);
-        v[p][0] = *(const f16x8_a8*) vr;
-        v[p][1] = *(const f16x8_a8*) (vr + 8);
+        const int i = min(i0 + p * step, n - 1);
+        lo[p] = *(const f16x8_a8*) (k0 + i * a.k_stride);
+        hi[p] = *(const f16x8_a8*) (k0 + i * a.k_stride + half);
+        if (ROPE) pos[p] = a.positions[t + i];
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int x = tid + 256 * p, w = over(x, a.by_4), d = 4 * (x - w * cols), i = 4 * (w0 + min(w, words - 1)) - off;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) v[p][b] = *(const f16x4_a4*) (v0 + min(max(i + b, 0), n - 1) * a.v_stride + d);
+    }
+    float k[P][16], kmax = 0.f, vmax = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
         if (ROPE) {
-            const size_t at = (size_t) min(max(a.positions[t + i], 0), a.angle_rows - 1) * a.hd + 8 * j;
-            const f16x8 sl = *(const f16x8_a8*) (a.sin + at), sh = *(const f16x8_a8*) (a.sin + at + half);
-            const f16x8 cl = *(const f16x8_a8*) (a.cos + at), ch = *(const f16x8_a8*) (a.cos + at + half);
+            const size_t to = (size_t) min(max(pos[p], 0), a.angle_rows - 1) * a.hd + 8 * j;
+            const f16x8 sl = *(const f16x8_a8*) (a.sin + to), sh = *(const f16x8_a8*) (a.sin + to + half);
+            const f16x8 cl = *(const f16x8_a8*) (a.cos + to), ch = *(const f16x8_a8*) (a.cos + to + half);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                k[p][e] = rot_odd(lo[e], cl[e], hi[e], sl[e], -1.f);
-                k[p][8 + e] = rot_odd(hi[e], ch[e], lo[e], sh[e], 1.f);
+                k[p][e] = rot_code(lo[p][e], cl[e], hi[p][e], sl[e], -1.f);
+                k[p][8 + e] = rot_code(hi[p][e], ch[e], lo[p][e], sh[e], 1.f);
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { k[p][e] = (float) lo[e]; k[p][8 + e] = (float) hi[e]; }
+            for (int e = 0; e < 8; ++e) { k[p][e] = (float) lo[p][e]; k[p][8 + e] = (float) hi[p][e]; }
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             kmax = fmaxf(kmax, fabsf(k[p][e]));
-            vmax = fmaxf(vmax, fabsf((float) v[p][e >> 3][e & 7]));
+            vmax = fmaxf(vmax, fabsf((float) v[p][e >> 2][e & 3]));
         }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) { kmax = fmaxf(kmax, __shfl_xor(kmax, o, 64)); vmax = fmaxf(vmax, __shfl_xor(vmax, o, 64)); }
-    __syncthreads();                                              // (the last run's LDS is free)
+    __syncthreads();                                              // (the last run's LDS is free; every thread has read the scales)
     if (lane == 0) { red[wave] = kmax; red[4 + wave] = vmax; }
     __syncthreads();
     kmax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     vmax = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
-    const size_t ph = (size_t) page * a.kv_heads + h, at = ph * a.block * a.hd16;
-    uint8_t* kc = a.kp + at;
-    uint8_t* vc = a.vp + at;
     int kold, vold;
-    const int ke = append_exp<CODE>(kmax, off, a.ks + ph, kold), ve = append_exp<CODE>(vmax, off, a.vs + ph, vold);
-    __syncthreads();                                              // every thread has read the scales
+    const int ke = append_exp<CODE>(kmax, off, kscale, kold), ve = append_exp<CODE>(vmax, off, vscale, vold);
+    if (ke != kold) append_move_keys<CODE>(kc, off, a.hd16, paged_pow2(kold - ke), tid, 256);
+    if (ve != vold) append_move_values<CODE>(vc, off, a.hd16, a.lbs, paged_pow2(vold - ve), tid, 256);
     if (tid == 0) { a.ks[ph] = paged_pow2(ke); a.vs[ph] = paged_pow2(ve); }
-    if (ke != kold) {                                             // the earlier tokens' codes under the new scale
-        const float f = paged_pow2(kold - ke);
-        for (int w = tid; w < off * (a.hd16 >> 2); w += 256) {
-            float x[4];
-            paged_decode4<CODE>(((const uint32_t*) kc)[w], x);
-            ((uint32_t*) kc)[w] = paged_encode4<CODE>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+    const float kinv = paged_pow2(-ke), vinv = paged_pow2(-ve), cap = PagedRange<CODE>::top * paged_pow2(PagedRange<CODE>::hi);
+    const int row = (1 << a.lbs) + 4;                             // bytes of a value column in LDS: the columns of a wave's threads lie in different banks
+    auto encode = [&](auto saturate) {
+        constexpr bool S = decltype(saturate)::value;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int i = i0 + p * step;
+            uint32_t c[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) c[w] = paged_encode4<CODE, S>(k[p][4 * w], k[p][4 * w + 1], k[p][4 * w + 2], k[p][4 * w + 3], kinv);
+            uint8_t* kr = kc + (off + i) * a.hd16 + 8 * j;
+            if (i0 < step && i < n) {
+                *(uint2*) kr = make_uint2(c[0], c[1]);
+                *(uint2*) (kr + half) = make_uint2(c[2], c[3]);
+            }
         }
-    }
-    if (ve != vold) {
-        const float f = paged_pow2(vold - ve);
-        const int words = a.block >> 2;
-        for (int w = tid; w < a.hd16 * words; w += 256) {
-            const int first = (w % words) * 4;
-            if (first >= off) continue;
-            float x[4];
-            paged_decode4<CODE>(((const uint32_t*) vc)[w], x);
-            const uint32_t now = paged_encode4<CODE>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
-            if (first + 4 <= off) ((uint32_t*) vc)[w] = now;
-            else for (int b = 0; b < off - first; ++b) vc[4 * w + b] = (uint8_t) (now >> (8 * b));       // (the word's other bytes belong to the new tokens)
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int x = tid + 256 * p, w = over(x, a.by_4);
+            uint8_t* dst = lds + 4 * (x - w * cols) * row + 4 * (w0 + w);
+            if (w < words)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    *(uint32_t*) (dst + e * row) = paged_encode4<CODE, S>((float) v[p][0][e], (float) v[p][1][e], (float) v[p][2][e], (float) v[p][3][e], vinv);
         }
-    }
-    const float kinv = paged_pow2(-ke), vinv = paged_pow2(-ve);
-    const int row = a.block + 4;                                  // bytes of a value column in LDS: the columns of a wave's threads lie in different banks
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const int i = i0 + p * step;
-        if (!on || i >= n) continue;
-        uint32_t c[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) c[w] = paged_encode4<CODE>(k[p][4 * w] * kinv, k[p][4 * w + 1] * kinv, k[p][4 * w + 2] * kinv, k[p][4 * w + 3] * kinv);
-        uint8_t* kr = kc + (size_t) (off + i) * a.hd16 + 8 * j;
-        *(uint2*) kr = make_uint2(c[0], c[1]);
-        *(uint2*) (kr + half) = make_uint2(c[2], c[3]);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const f16x8 x = v[p][w >> 1];
-            const int e = (w & 1) * 4;
-            const uint32_t u = paged_encode4<CODE>((float) x[e] * vinv, (float) x[e + 1] * vinv, (float) x[e + 2] * vinv, (float) x[e + 3] * vinv);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) lds[(16 * j + 4 * w + b) * row + off + i] = (uint8_t) (u >> (8 * b));
-        }
-    }
+    };
+    if (kmax > cap || vmax > cap) encode(std::true_type()); else encode(std::false_type());
     __syncthreads();
-    const int pieces = a.block >> 4;                              // 16 tokens of a column at a time
-    for (int w = tid; w < a.hd * pieces; w += 256) {
-        const int d = w / pieces, first = (w % pieces) * 16;
+    for (int w = tid; w < a.hd << (a.lbs - 4); w += 256) {         // 16 tokens of a column at a time
+        const int d = w >> (a.lbs - 4), first = (w & ((1 << (a.lbs - 4)) - 1)) * 16;
         const uint8_t* src = lds + d * row + first;
-        uint8_t* dst = vc + (size_t) d * a.block + first;
+        uint8_t* dst = vc + (d << a.lbs) + first;
         if (first >= off && first + 16 <= off + n) {
             const uint32_t* x = (const uint32_t*) src;
             *(uint4*) dst = make_uint4(x[0], x[1], x[2], x[3]);
@@ -430,44 +442,50 @@ __device__ __forceinline__ void append_run_wide(const AppendArgs& a, int h, int 
     }
 }
 
-// One workgroup = `chunk` token rows of one head: it does the runs that begin there.  P = 0: a wave for every run.
+// One workgroup = `chunk` (at most 32) token rows of one head: it does the runs that begin there.  Every wave reads the chunk's slots and the page
+// that may follow (at most 32 + 128 of them) in one round of loads; a bit for each row says whether it continues the row before it.
+// P = 0: a wave for every run.
 template <int CODE, bool ROPE, int P> __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ float red[8];
-    __shared__ int longs[16][4];                                  // the long runs: token row, tokens, page, offset
-    __shared__ int count;
-    const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t0 = blockIdx.x * a.chunk, t1 = min(t0 + a.chunk, a.rows);
-    if (P) {
-        if (threadIdx.x == 0) count = 0;
-        __syncthreads();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // heads next to each other in launch order: what runs at one time reads whole token rows
+    const int h = blockIdx.x % a.kv_heads, t0 = (int) (blockIdx.x / a.kv_heads) * a.chunk, count = min(a.chunk, a.rows - t0);
+    int slot[3];                                                  // of token rows t0 - 1 + lane + 64 i
+    uint64_t on[4];                                               // bit: the row continues the one before it
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const int64_t t = (int64_t) t0 - 1 + lane + 64 * i;
+        slot[i] = t >= 0 && t < a.rows ? a.slots[t] : -1;
     }
-    for (int t = t0 + wave; t < t1; t += 4) {
-        const int slot = a.slots[t];
-        if (slot < 0 || slot / a.block >= a.blocks) continue;
-        const int page = slot / a.block, off = slot % a.block;
-        if (t > 0 && off > 0 && a.slots[t - 1] == slot - 1) continue;          // not the first of its run
-        int n = 1;                                              // lanes look at the following rows
-        for (int base = 1; base < a.block - off; base += 64) {
-            const int i = base + lane;
-            const bool on = i < a.block - off && t + i < a.rows && a.slots[t + i] == slot + i;
-            const uint64_t m = __ballot(!on);
-            n = base + (m ? __ffsll((unsigned long long) m) - 1 : 64);
-            if (m) break;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        int before = __shfl_up(slot[i], 1, 64);
+        if (i) { const int last = __shfl(slot[i ? i - 1 : 0], 63, 64); if (lane == 0) before = last; }
+        else if (lane == 0) before = -2;
+        on[i] = __ballot(slot[i] > 0 && (slot[i] & ((1 << a.lbs) - 1)) != 0 && slot[i] == before + 1);
+    }
+    on[3] = 0;
+    const int page_here = slot[0] >> a.lbs;
+    const uint64_t starts = __ballot(slot[0] >= 0 && page_here < a.blocks) & ~on[0];
+    for (int x = 0, nth = 0; x < count; ++x) {
+        if (!(starts >> (x + 1) & 1)) continue;
+        const int s = __shfl(slot[0], x + 1, 64), page = s >> a.lbs, off = s & ((1 << a.lbs) - 1);
+        int n = 1, at = x + 2;                                    // the ones that follow
+        while (at < 192) {
+            const uint64_t rest = ~(on[at >> 6] >> (at & 63));    // (zeros come in from above: the word ends the stretch at the latest)
+            const int ones = rest ? __ffsll((unsigned long long) rest) - 1 : 64, room = 64 - (at & 63);
+            n += min(ones, room);
+            at += min(ones, room);
+            if (ones < room) break;
         }
-        n = min(n, a.block - off);
+        n = min(n, (1 << a.lbs) - off);
         if (P && n >= APPEND_LONG) {
-            if (lane == 0) { const int x = atomicAdd(&count, 1); longs[x][0] = t; longs[x][1] = n; longs[x][2] = page; longs[x][3] = off; }
-            continue;
+            append_run_wide<CODE, ROPE, P ? P : 1>(a, h, t0 + x, n, page, off, lds, red);
+        } else if ((nth++ & 3) == wave) {
+            append_run<CODE, ROPE>(a, h, t0 + x, n, page, off);
         }
-        append_run<CODE, ROPE, true>(a, h, t, n, page, off);
-        append_run<CODE, ROPE, false>(a, h, t, n, page, off);
-    }
-    if (P) {
-        __syncthreads();
-        for (int x = 0; x < count; ++x)                           // (runs of different pages: their order does not matter)
-            append_run_wide<CODE, ROPE, P ? P : 1>(a, h, longs[x][0], longs[x][1], longs[x][2], longs[x][3], lds, red);
     }
 }
 
@@ -486,15 +504,22 @@ extern "C" int exl_paged_append(const void* key_states, const void* value_states
                 "paged_append: key / value rows must be 8-byte aligned and at least kv_heads * head_dim apart");
     EXL_REQUIRE(((uintptr_t) key_pages | (uintptr_t) value_pages) % 16 == 0, EXL_E_INVALID, "paged_append: pages must be 16-byte aligned");
     if (rows == 0) return 0;
+    EXL_REQUIRE(key_stride <= 1 << 22 && value_stride <= 1 << 22, EXL_E_UNSUPPORTED, "paged_append: key / value rows more than 2^22 elements apart");
+    auto by = [](int d) { return (uint32_t) ((0x100000000ull + d - 1) / d); };
+    const int hd16 = (head_dim + 15) / 16 * 16;
     AppendArgs a = {(const f16*) key_states, (const f16*) value_states, slots, positions, (const f16*) sin, (const f16*) cos,
-                    (uint8_t*) key_pages, (uint8_t*) value_pages, key_scales, value_scales, rows, num_kv_heads, head_dim, (head_dim + 15) / 16 * 16,
-                    block_size, num_blocks, 4, angle_rows, key_stride, value_stride};
-    const int passes = head_dim % 16 ? 0 : (block_size * (head_dim / 16) + 255) / 256;       // (256 / (head_dim / 16) tokens a pass, or a few less)
-    a.chunk = (long) rows * num_kv_heads <= 16384 ? 4 : 16;       // few rows: a run for every wave at once
-    const dim3 grid((unsigned) ((rows + a.chunk - 1L) / a.chunk), (unsigned) num_kv_heads);
-    const size_t lds = passes ? (size_t) head_dim * (block_size + 4) : 0;
+                    (uint8_t*) key_pages, (uint8_t*) value_pages, key_scales, value_scales, rows, num_kv_heads, head_dim, hd16,
+                    31 - __builtin_clz((unsigned) block_size), num_blocks, 4, angle_rows, (int) key_stride, (int) value_stride, by(hd16 / 4),
+                    head_dim % 16 ? 0u : by(head_dim / 16), by(head_dim / 4)};
+    // passes of the wide form over a page: block tokens x head_dim / 16 threads (256 / (head_dim / 16) whole tokens at a time)
+    const int step = head_dim % 16 ? 0 : 256 / (head_dim / 16), p = step ? (block_size + step - 1) / step : 0;
+    const int64_t work = (int64_t) rows * num_kv_heads;           // few rows: a run for every wave at once; many: fewer workgroups that find no run's beginning
+    a.chunk = work <= 16384 ? 4 : work <= 131072 ? 16 : 32;
+    const int64_t groups = ((int64_t) rows + a.chunk - 1) / a.chunk * num_kv_heads;
+    EXL_REQUIRE(groups <= 0x7fffffff, EXL_E_UNSUPPORTED, "paged_append: too many rows for %d kv heads", num_kv_heads);
+    const dim3 grid((unsigned) groups);
+    const size_t lds = p ? (size_t) head_dim * (block_size + 4) : 0;
     hipStream_t s = (hipStream_t) stream;
-    const int p = !passes ? 0 : passes * (256 / (head_dim / 16)) >= block_size ? passes : passes + 1;
 #define APPEND(C, R, P) hipLaunchKernelGGL((paged_append_kernel<C, R, P>), grid, dim3(256), lds, s, a)
 #define APPEND_P(C, R) do { if (p == 0) APPEND(C, R, 0); else if (p == 1) APPEND(C, R, 1); else if (p == 2) APPEND(C, R, 2); else if (p <= 4) APPEND(C, R, 4); \
                             else APPEND(C, R, 8); } while (0)

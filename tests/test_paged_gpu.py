@@ -121,16 +121,18 @@ def _runs(rng, blocks, block, spec):
 @pytest.mark.parametrize("hd,kvh,block,spec,rope", [
     (128, 8, 64, [(0, 1)], True), (128, 2, 16, [(5, 1), (15, 1), (0, 1), (9, 1)], True), (64, 3, 32, [(0, 100), (-1, -3), (31, 2), (7, 70)], True),
     (100, 4, 16, [(3, 40), (0, 16), (0, 1)], True), (80, 1, 128, [(0, 128), (100, 60)], False), (256, 2, 64, [(60, 9), (0, 64), (-1, -1)], True),
-    (4, 5, 16, [(0, 3), (15, 18)], True), (128, 32, 64, [(0, 200)], False), (20, 2, 128, [(64, 64), (127, 130)], True)])
+    (4, 5, 16, [(0, 3), (15, 18)], True), (128, 32, 64, [(0, 200)], False), (20, 2, 128, [(64, 64), (127, 130)], True),
+    (16, 3, 128, [(0, 128), (90, 50), (1, 1)], True), (48, 2, 32, [(2, 30), (0, 9), (31, 40)], True), (240, 1, 128, [(0, 128), (127, 9)], True),
+    (96, 40, 64, [(0, 700), (-1, -40), (9, 8)], False)])
 def test_append(ext, code, hd, kvh, block, spec, rope):
     rng = np.random.default_rng(hd + kvh)
-    pool = _pool(rng, 12, kvh, block, hd, code)
+    pool = _pool(rng, 16, kvh, block, hd, code)
     dev = _pool_dev(pool, code)
-    slots, pos = _runs(rng, 12, block, spec)
+    slots, pos = _runs(rng, 16, block, spec)
     t = len(slots)
     x = (rng.normal(0, 1, (2, t, kvh, hd)) * np.exp(rng.normal(0, 1.5, (2, 1, kvh, hd)))).astype(np.float16)
     x[:, rng.random(t) < 0.2] *= 30                            # tokens that raise their page's scale
-    sin, cos = _angles(300, hd)
+    sin, cos = _angles(800, hd)
     wide = torch.zeros(t, 2 * kvh * hd + 4, dtype=torch.float16, device=DEV)      # keys and values as two views of one projection's output
     k, v = wide[:, 4:4 + kvh * hd], wide[:, 4 + kvh * hd:]
     k.copy_(torch.from_numpy(x[0]).reshape(t, -1))
