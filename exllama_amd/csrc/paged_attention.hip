@@ -1,6 +1,7 @@
 // Attention over the paged 8-bit cache (paged.h).
 //   o[t, h] = sum_j p_j V[j] / sum_j p_j,   p_j = exp(s_j - max s),   s_j = scale * rope(q[t, h]) . K[j],   j <= past + i, j < past + new
 #include "paged.h"
+#include <type_traits>
 
 struct PagedAttn {
     const f16* q; const int32_t* starts; const int32_t* past; const int32_t* fresh; const int32_t* table;
@@ -35,29 +36,45 @@ __device__ __forceinline__ PaRow pa_row(const PagedAttn& a, int b)
 #define PA_KEYS 64
 #define PA_MAX_ROWS 1024                                       // rows of the batch up to which their keys are cut into pieces of equal size
 
-template <int CODE> __device__ __forceinline__ f16x8 pa_numbers(uint32_t lo, uint32_t hi, float scale)     // 8 codes * scale (a power of two)
+// A page's scale as the conversions take it.  int8: 2^e is the exponent field of the fp16 numbers that a code's byte becomes the mantissa of:
+// (1024 + u) * 2^e with u = code + 128, minus 1152 * 2^e -- up to e = 5; beyond (`big`, for every lane as soon as one has it) a product follows.
+struct PaScale { float f; uint32_t top; f16x2 sub, mul; };
+template <int CODE> __device__ __forceinline__ PaScale pa_scale(float s)
 {
-    f16x8 r;
-    if (CODE == EXL_PAGE_FP8) {
-        f16x2* p = (f16x2*) &r;
-        p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) lo, scale, false);
-        p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) lo, scale, true);
-        p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) hi, scale, false);
-        p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) hi, scale, true);
-    } else {
-        // 0x6400 | u is the fp16 number 1024 + u: the bytes with the sign bit flipped (u = code + 128), minus 1152
-        const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
-        union { uint32_t u[4]; f16x2 h[4]; f16x8 v; } x;
-        x.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
-        x.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
-        x.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
-        x.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
-        const f16 s = (f16) scale;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x.h[i] = (x.h[i] - (f16) 1152.f) * s;
-        r = x.v;
+    PaScale r = {};
+    const int e = paged_scale_exp<CODE>(s);
+    r.f = paged_pow2(e);
+    if (CODE == EXL_PAGE_INT8) {
+        const uint32_t field = (uint32_t) (min(e, 5) + 25) << 2;
+        r.top = field * 0x01010101u;
+        r.sub = __builtin_bit_cast(f16x2, (field << 8 | 0x80) * 0x00010001u);
+        r.mul = (f16x2) ((f16) paged_pow2(max(e - 5, 0)));
     }
     return r;
+}
+template <int CODE> __device__ __forceinline__ bool pa_big(const PaScale& s) { return CODE == EXL_PAGE_INT8 && __any((float) s.mul[0] != 1.f); }
+
+template <int CODE, bool BIG> __device__ __forceinline__ f16x8 pa_numbers(uint32_t lo, uint32_t hi, const PaScale& scale)     // 8 codes * scale, exact
+{
+    union { uint32_t u[4]; f16x2 h[4]; f16x8 v; } x;
+    if (CODE == EXL_PAGE_FP8) {
+        x.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) lo, scale.f, false);
+        x.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) lo, scale.f, true);
+        x.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) hi, scale.f, false);
+        x.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) hi, scale.f, true);
+    } else {
+        const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
+        x.u[0] = __builtin_amdgcn_perm(scale.top, a, 0x04010400u);
+        x.u[1] = __builtin_amdgcn_perm(scale.top, a, 0x04030402u);
+        x.u[2] = __builtin_amdgcn_perm(scale.top, b, 0x04010400u);
+        x.u[3] = __builtin_amdgcn_perm(scale.top, b, 0x04030402u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x.h[i] = x.h[i] - scale.sub;
+            if (BIG) x.h[i] = x.h[i] * scale.mul;
+        }
+    }
+    return x.v;
 }
 
 // Query elements d .. d + 7 of one token and head (zeros behind head_dim), rotated at `pos` when there are tables
@@ -213,7 +230,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
         if (iv < a.width) r.v = table[iv];
         return r;
     };
-    struct Stage { uint4 k[4][KS]; uint4 v[DT]; float ks, vs; bool there; };
+    struct Stage { uint4 k[4][KS]; uint4 v[DT]; float ks, vs; bool there; };      // (scales as they are: looking at one here would wait for every load before it)
     auto fetch = [&](int tile, Ids id, Stage& st) {
         const bool kok = id.k >= 0 && id.k < a.blocks, vok = id.v >= 0 && id.v < a.blocks;
         const size_t kb = (size_t) (kok ? id.k : 0) * a.kv_heads + kvh, vb = (size_t) (vok ? id.v : 0) * a.kv_heads + kvh;
@@ -226,8 +243,8 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
         const uint8_t* vp = a.vp + vb * kpage + ((tile * PA_KEYS + 16 * g) & (a.block - 1));
 #pragma unroll
         for (int t = 0; t < DT; ++t) st.v[t] = *(const uint4*) (vp + vd[t]);
-        st.ks = paged_pow2(paged_scale_exp<CODE>(a.ks[vb]));
-        st.vs = paged_pow2(paged_scale_exp<CODE>(a.vs[vb]));
+        st.ks = a.ks[vb];
+        st.vs = a.vs[vb];
         st.there = vok;
     };
 
@@ -240,6 +257,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
         for (int t = 0; t < DT; ++t) o[nt][t] = (f32x4) {0.f, 0.f, 0.f, 0.f};
     }
     const float c1 = a.scale * 1.44269504f;                       // scores in powers of two
+    const PaScale one = pa_scale<CODE>(1.f);
 
     auto work = [&](int tile, Stage& st) {
         const int key0 = tile * PA_KEYS + 16 * g;
@@ -261,7 +279,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
         for (int t4 = 0; t4 < 4; ++t4)
 #pragma unroll
             for (int u = 0; u < KS; ++u) {
-                const f16x8 k0 = pa_numbers<CODE>(st.k[t4][u].x, st.k[t4][u].y, 1.f), k1 = pa_numbers<CODE>(st.k[t4][u].z, st.k[t4][u].w, 1.f);
+                const f16x8 k0 = pa_numbers<CODE, false>(st.k[t4][u].x, st.k[t4][u].y, one), k1 = pa_numbers<CODE, false>(st.k[t4][u].z, st.k[t4][u].w, one);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     s[nt][t4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[nt][u][0], s[nt][t4], 0, 0, 0);
@@ -269,7 +287,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
                 }
             }
         f16x8 p[NT][2];
-        const float sc = st.ks * c1;
+        const float sc = paged_pow2(paged_scale_exp<CODE>(st.ks)) * c1;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float x[16], mx = -INFINITY;
@@ -281,8 +299,9 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
             }
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float mn = fmaxf(m[nt], mx);
-            if (__any(mn > m[nt])) {
+            // the reference moves only when a score passes it by 2^8: the weights are relative to it, fp16 holds them up to 2^16
+            if (__any(mx > m[nt] + 8.f)) {
+                const float mn = fmaxf(m[nt], mx);
                 const float keep = m[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[nt] - mn);
                 l[nt] *= keep;
 #pragma unroll
@@ -291,7 +310,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
                     for (int j = 0; j < 4; ++j) o[nt][t][j] *= keep;
                 m[nt] = mn;
             }
-            const float ref = mn == -INFINITY ? 0.f : mn;
+            const float ref = m[nt] == -INFINITY ? 0.f : m[nt];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float e = __builtin_amdgcn_exp2f(x[i] - ref);
@@ -299,9 +318,10 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
                 p[nt][i >> 3][i & 7] = (f16) e;
             }
         }
+        const PaScale vs = pa_scale<CODE>(st.vs);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            const f16x8 v0 = pa_numbers<CODE>(st.v[t].x, st.v[t].y, st.vs), v1 = pa_numbers<CODE>(st.v[t].z, st.v[t].w, st.vs);
+            const f16x8 v0 = pa_numbers<CODE, true>(st.v[t].x, st.v[t].y, vs), v1 = pa_numbers<CODE, true>(st.v[t].z, st.v[t].w, vs);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 o[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[nt][0], o[nt][t], 0, 0, 0);
@@ -471,7 +491,8 @@ __device__ __forceinline__ PmItem pm_find(const PagedAttn& a, const PaCut& cut, 
     return it;
 }
 
-template <int CODE, int DP>
+// WIDE: pages of 64 or 128 tokens, a tile lies in one: its page is looked up once, in scalar registers.
+template <int CODE, int DP, bool WIDE>
 __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_many_kernel(PagedAttn a, PaCut cut, float* __restrict__ parts,
                                                                                         PmItem* __restrict__ items, int part_items)
 {
@@ -479,16 +500,17 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // [2][keys: 2 * KB * 1024 bytes, values: 4 * DT * 1024 bytes]
     constexpr int K_BYTES = 2 * KB * 1024, BUF = 2 * K_BYTES;
     const int kvh = blockIdx.y, w = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, g = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, g = lane >> 5;
     const PmItem it = pm_find(a, cut, w, lds);
     if (kvh == 0 && tid == 0 && w < part_items) items[w] = it;                   // for the joining kernel
     if (it.row < 0) return;
-    const PaRow row = pa_row(a, it.row);
+    const PaRow row = pa_row(a, __builtin_amdgcn_readfirstlane(it.row));
     const int group = a.heads / a.kv_heads, lbs = 31 - __clz(a.block);
     const int64_t queries = (int64_t) row.fresh * group, q0 = (int64_t) it.tile * PM_ROWS;
     const int last_token = (int) ((min(q0 + PM_ROWS, queries) - 1) / group);
     const int all_tiles = (int) ((min((int64_t) row.past + last_token + 1, (int64_t) row.keys) + PA_KEYS - 1) / PA_KEYS);
-    const int t_first = (int) ((int64_t) all_tiles * it.piece / it.pieces), t_last = (int) ((int64_t) all_tiles * (it.piece + 1) / it.pieces);
+    const int t_first = __builtin_amdgcn_readfirstlane((int) ((int64_t) all_tiles * it.piece / it.pieces));
+    const int t_last = __builtin_amdgcn_readfirstlane((int) ((int64_t) all_tiles * (it.piece + 1) / it.pieces));
 
     // this lane's query
     const int64_t r = q0 + wave * 32 + c;
@@ -510,62 +532,97 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
         }
     }
 
-    const int32_t* table = a.table + (size_t) it.row * a.width;
+    const int32_t* table = a.table + (size_t) __builtin_amdgcn_readfirstlane(it.row) * a.width;
     const size_t page_bytes = (size_t) a.block * a.hd16;
     // staging roles: keys: piece i of this thread is column chunk k_ch of key k_key + (256 / KB) * i; values: 16 keys v_kc of column v_d + 64 * i
     const int k_ch = tid % KB, k_key = tid / KB, v_kc = tid & 3, v_d = tid >> 2;
     constexpr int K_STEP = 256 / KB;
-    struct Ids { int k[PIECES]; int v; };
-    struct Stage { uint4 k[PIECES], v[PIECES]; float ks[PIECES], vs; int n; uint32_t there; };   // n: valid keys of the value pieces; there: a bit for each 16 keys
+    struct Ids { int k[WIDE ? 1 : PIECES]; int v; };
+    struct Stage { uint4 k[PIECES], v[PIECES]; float ks[WIDE ? 1 : PIECES], vs; int n; uint32_t there; };   // n: valid keys of the value pieces; there: a bit for each 16 keys
     auto look = [&](int tile) -> Ids {
         Ids id;
+        if (WIDE) {
+            const int p = (tile * PA_KEYS) >> lbs;
+            id.k[0] = id.v = p < a.width ? ((const __attribute__((address_space(4))) int32_t*) table)[p] : -1;     // a scalar load
+        } else {
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int p = (tile * PA_KEYS + k_key + K_STEP * i) >> lbs;
-            id.k[i] = p < a.width ? table[p] : -1;
+            for (int i = 0; i < PIECES; ++i) {
+                const int p = (tile * PA_KEYS + k_key + K_STEP * i) >> lbs;
+                id.k[WIDE ? 0 : i] = p < a.width ? table[p] : -1;
+            }
+            const int p = (tile * PA_KEYS + 16 * v_kc) >> lbs;
+            id.v = p < a.width ? table[p] : -1;
         }
-        const int p = (tile * PA_KEYS + 16 * v_kc) >> lbs;
-        id.v = p < a.width ? table[p] : -1;
         return id;
     };
-    auto fetch = [&](int tile, const Ids& id, Stage& st) {
+    // offsets of this thread's pieces inside a page, for WIDE: from the tile's first key on
+    const int k_at = k_key * a.hd16 + (16 * k_ch < a.hd16 ? 16 * k_ch : 0);
+    int v_at[PIECES];
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int key = tile * PA_KEYS + k_key + K_STEP * i;
-            const size_t kb = (size_t) (id.k[i] >= 0 && id.k[i] < a.blocks ? id.k[i] : 0) * a.kv_heads + kvh;
-            st.k[i] = *(const uint4*) (a.kp + kb * page_bytes + (size_t) (key & (a.block - 1)) * a.hd16 + (16 * k_ch < a.hd16 ? 16 * k_ch : 0));
-            st.ks[i] = paged_pow2(paged_scale_exp<CODE>(a.ks[kb]));
-        }
+    for (int i = 0; i < PIECES; ++i) v_at[i] = ((v_d + 64 * i < a.hd16 ? v_d + 64 * i : 0) << lbs) + (WIDE ? 16 * v_kc : 0);
+    auto fetch = [&](int tile, const Ids& id, Stage& st) {
         const bool ok = id.v >= 0 && id.v < a.blocks;
         const size_t vb = (size_t) (ok ? id.v : 0) * a.kv_heads + kvh;
         const int key = tile * PA_KEYS + 16 * v_kc;
-        const uint8_t* vp = a.vp + vb * page_bytes + (key & (a.block - 1));
+        if (WIDE) {
+            const int first = (tile * PA_KEYS) & (a.block - 1);
+            const uint8_t* kp = a.kp + vb * page_bytes + first * a.hd16;
+            const uint8_t* vp = a.vp + vb * page_bytes + first;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) st.v[i] = *(const uint4*) (vp + (size_t) (v_d + 64 * i < a.hd16 ? v_d + 64 * i : 0) * a.block);
-        st.vs = paged_pow2(paged_scale_exp<CODE>(a.vs[vb]));
+            for (int i = 0; i < PIECES; ++i) {
+                st.k[i] = *(const uint4*) (kp + (uint32_t) (k_at + K_STEP * i * a.hd16));
+                st.v[i] = *(const uint4*) (vp + (uint32_t) v_at[i]);
+            }
+            st.ks[0] = a.ks[vb];
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int at = tile * PA_KEYS + k_key + K_STEP * i, kid = id.k[WIDE ? 0 : i];
+                const size_t kb = (size_t) (kid >= 0 && kid < a.blocks ? kid : 0) * a.kv_heads + kvh;
+                st.k[i] = *(const uint4*) (a.kp + kb * page_bytes + (size_t) ((at & (a.block - 1)) * a.hd16 + (16 * k_ch < a.hd16 ? 16 * k_ch : 0)));
+                st.ks[WIDE ? 0 : i] = a.ks[kb];
+            }
+            const uint8_t* vp = a.vp + vb * page_bytes + (key & (a.block - 1));
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) st.v[i] = *(const uint4*) (vp + v_at[i]);
+        }
+        st.vs = a.vs[vb];                                         // (as it is: looking at it here would wait for every load before it)
         st.n = ok ? min(max(row.keys - key, 0), 16) : 0;
-        st.there = (uint32_t) __ballot(ok) & 15;
+        st.there = WIDE ? (ok ? 15u : 0u) : (uint32_t) __ballot(ok) & 15;
     };
+    // where this thread's pieces go in a buffer
+    int k_to[PIECES], v_to[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int key = k_key + K_STEP * i, kt = key >> 5, m = 8 * ((key >> 2) & 3) + 4 * ((key >> 4) & 1) + (key & 3), d = v_d + 64 * i;
+        k_to[i] = (kt * KB + k_ch) * 1024 + ((m ^ (k_ch & 7)) << 4);
+        v_to[i] = K_BYTES + ((v_kc >> 1) * 2 * DT + (d >> 5)) * 1024 + ((((v_kc & 1) * 32 + (d & 31)) ^ (v_kc << 1)) << 4);
+    }
     auto store = [&](Stage& st, unsigned char* buf) {
-        if (st.n < 16) {                                          // bytes that hold no value may be anything, NaN too: a weight of 0 does not hide it
+        if (__any(st.n < 16)) {                                   // bytes that hold no value may be anything, NaN too: a weight of 0 does not hide it
             uint32_t mask[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) mask[i] = st.n >= 4 * i + 4 ? 0xffffffffu : st.n <= 4 * i ? 0u : (1u << (8 * (st.n - 4 * i))) - 1;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) { st.v[i].x &= mask[0]; st.v[i].y &= mask[1]; st.v[i].z &= mask[2]; st.v[i].w &= mask[3]; }
         }
+        const PaScale vscale = pa_scale<CODE>(st.vs);
+        PaScale kscale[WIDE ? 1 : PIECES];
+        bool big = pa_big<CODE>(vscale);
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int key = k_key + K_STEP * i, kt = key >> 5, m = 8 * ((key >> 2) & 3) + 4 * ((key >> 4) & 1) + (key & 3);
-            unsigned char* p = buf + (kt * KB + k_ch) * 1024;
-            *(f16x8*) (p + ((m ^ (k_ch & 7)) << 4)) = pa_numbers<CODE>(st.k[i].x, st.k[i].y, st.ks[i]);
-            *(f16x8*) (p + (((32 + m) ^ (k_ch & 7)) << 4)) = pa_numbers<CODE>(st.k[i].z, st.k[i].w, st.ks[i]);
-            const int d = v_d + 64 * i;
-            const int slot = ((v_kc & 1) * 32 + (d & 31)) ^ (v_kc << 1);
-            unsigned char* q = buf + K_BYTES + ((v_kc >> 1) * 2 * DT + (d >> 5)) * 1024 + (slot << 4);
-            *(f16x8*) q = pa_numbers<CODE>(st.v[i].x, st.v[i].y, st.vs);
-            *(f16x8*) (q + DT * 1024) = pa_numbers<CODE>(st.v[i].z, st.v[i].w, st.vs);
-        }
+        for (int i = 0; i < (WIDE ? 1 : PIECES); ++i) { kscale[i] = pa_scale<CODE>(st.ks[i]); big = big || pa_big<CODE>(kscale[i]); }
+        auto convert = [&](auto big) {
+            constexpr bool BIG = decltype(big)::value;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const PaScale& ks = kscale[WIDE ? 0 : i];
+                *(f16x8*) (buf + k_to[i]) = pa_numbers<CODE, BIG>(st.k[i].x, st.k[i].y, ks);
+                *(f16x8*) (buf + k_to[i] + 512) = pa_numbers<CODE, BIG>(st.k[i].z, st.k[i].w, ks);       // (columns 8 .. 15 of the chunk: lanes 32 .. 63)
+                *(f16x8*) (buf + v_to[i]) = pa_numbers<CODE, BIG>(st.v[i].x, st.v[i].y, vscale);
+                *(f16x8*) (buf + v_to[i] + DT * 1024) = pa_numbers<CODE, BIG>(st.v[i].z, st.v[i].w, vscale);
+            }
+        };
+        if (big) convert(std::true_type()); else convert(std::false_type());
     };
 
     f32x16 o[DT];
@@ -612,20 +669,22 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
             }
         }
         float mx = -INFINITY;
-        if (border) {
+        if (__builtin_amdgcn_readfirstlane(border)) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int kt = 0; kt < 2; ++kt) {
+                const int left = now >> (2 * kt + g) & 1 ? limit - (tile * PA_KEYS + 32 * kt + 16 * g) : -1;      // the last visible of these 16 keys
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (!(now >> (2 * kt + g) & 1) || tile * PA_KEYS + 32 * kt + 16 * g + j > limit) s[kt][j] = -INFINITY;
+                for (int j = 0; j < 16; ++j) if (j > left) s[kt][j] = -INFINITY;
+            }
         }
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[kt][j]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c1;
-        const float mn = fmaxf(m, mx);
-        if (__any(mn > m)) {
+        // the reference moves only when a score passes it by 2^8: the weights are relative to it, fp16 holds them up to 2^16
+        if (__any(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx);
             const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             l *= keep;
 #pragma unroll
@@ -634,7 +693,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
                 for (int j = 0; j < 16; ++j) o[t][j] *= keep;
             m = mn;
         }
-        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float ref = m == -INFINITY ? 0.f : m;
         f16x8 p[2][2];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -771,10 +830,12 @@ template <int CODE> static int pa_launch(const PagedAttn& a, const PaPlan& p, vo
         PmItem* items = (PmItem*) ((char*) parts + p.part_bytes);
         float* more = (float*) ((char*) items + p.many_item_bytes);
         const dim3 mgrid((unsigned) p.many_items, (unsigned) a.kv_heads);
-#define PA_MANY(DP) do { static bool done[EXL_MAX_DEVICES] = {};                                                                             \
-        EXL_TRY(exl_lds_opt_in((const void*) paged_attn_many_kernel<CODE, DP>, done));                                                        \
-        hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP>), mgrid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4, s, a, p.many_cut, more, items, p.many_parts); } while (0)
-        if (p.dp == 64) PA_MANY(64); else if (p.dp == 128) PA_MANY(128); else PA_MANY(256);
+#define PA_MANY(DP, WIDE) do { static bool done[EXL_MAX_DEVICES] = {};                                                                       \
+        EXL_TRY(exl_lds_opt_in((const void*) paged_attn_many_kernel<CODE, DP, WIDE>, done));                                                  \
+        hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE>), mgrid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4, s, a, p.many_cut, more, items, \
+                           p.many_parts); } while (0)
+        if (a.block >= PA_KEYS) { if (p.dp == 64) PA_MANY(64, true); else if (p.dp == 128) PA_MANY(128, true); else PA_MANY(256, true); }
+        else                    { if (p.dp == 64) PA_MANY(64, false); else if (p.dp == 128) PA_MANY(128, false); else PA_MANY(256, false); }
 #undef PA_MANY
         EXL_LAUNCH_CHECK();
         if (p.many_parts) {
