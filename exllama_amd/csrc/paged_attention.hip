@@ -108,15 +108,10 @@ __device__ __forceinline__ f16x8 pa_query(const PagedAttn& a, const f16* q, int6
     return r;
 }
 
-// Which rows of the batch the kernel for few queries takes, and how their keys are cut: `tiles` tiles of a row in pieces of `piece` tiles
-struct PaCut { int few, target, min_piece, split; };             // few: queries of a row (tokens * group) up to which it is taken
+// How the keys of all rows are cut: pieces of equal size, about `target` of them, none of less than `min_piece` tiles
+struct PaCut { int target, min_piece; };
 
-__device__ __forceinline__ int pa_few_tiles(const PagedAttn& a, const PaCut& cut, int b, PaRow& r)
-{
-    r = pa_row(a, b);
-    const int64_t queries = (int64_t) r.fresh * (a.heads / a.kv_heads);
-    return queries > 0 && queries <= cut.few ? (r.keys + PA_KEYS - 1) / PA_KEYS : 0;
-}
+__device__ __forceinline__ int pa_tiles(const PagedAttn& a, int b) { return (pa_row(a, b).keys + PA_KEYS - 1) / PA_KEYS; }
 
 struct PaItem { int row, first, last, piece, pieces; };          // tiles first .. last - 1, piece number `piece` of `pieces`
 
@@ -126,17 +121,16 @@ __device__ __forceinline__ PaItem pa_find(const PagedAttn& a, const PaCut& cut, 
     __shared__ int64_t sums[PA_WAVES];
     __shared__ PaItem found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    PaRow r;
     PaItem it = {-1, 0, 0, 0, 0};
     if (a.n > PA_MAX_ROWS) {
-        const int tiles = pa_few_tiles(a, cut, w, r);
+        const int tiles = pa_tiles(a, w);
         if (tiles > 0) it = {w, 0, tiles, 0, 1};
         return it;
     }
     int64_t total = 0;
     int tiles0 = 0;
     for (int b = tid; b < a.n; b += PA_WAVES * 64) {
-        const int tiles = pa_few_tiles(a, cut, b, r);
+        const int tiles = pa_tiles(a, b);
         if (b == tid) tiles0 = tiles;
         total += tiles;
     }
@@ -151,7 +145,7 @@ __device__ __forceinline__ PaItem pa_find(const PagedAttn& a, const PaCut& cut, 
     int before = 0;
     for (int b0 = 0; b0 < a.n; b0 += PA_WAVES * 64) {
         const int b = b0 + tid;
-        const int tiles = b >= a.n ? 0 : b0 == 0 ? tiles0 : pa_few_tiles(a, cut, b, r);
+        const int tiles = b >= a.n ? 0 : b0 == 0 ? tiles0 : pa_tiles(a, b);
         const int mine = (tiles + piece - 1) / piece;
         int inc = mine;
 #pragma unroll
@@ -186,7 +180,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
     constexpr bool AHEAD = DP <= 128;
     __shared__ __attribute__((aligned(16))) float joined[PA_WAVES][16 * ROW];
     __shared__ float stat[PA_WAVES][2][16];
-    const int kvh = blockIdx.y, w = blockIdx.x;
+    const int kvh = blockIdx.x % a.kv_heads, w = blockIdx.x / a.kv_heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const PaItem it = pa_find(a, cut, w);
     if (it.row < 0) return;
@@ -386,13 +380,13 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
 }
 
 // The pieces of a row joined, in order: one workgroup per row of the batch, query and kv head.
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, PaCut cut, const float* __restrict__ parts, const int2* __restrict__ firsts, int dp, int nt)
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const float* __restrict__ parts, const int2* __restrict__ firsts, int dp, int nt)
 {
     __shared__ float part_o[16][256 + 4];
     __shared__ float part_l[16];
     const int b = blockIdx.x, r = blockIdx.y, kvh = blockIdx.z, group = a.heads / a.kv_heads, tid = threadIdx.x;
-    PaRow row;
-    if (pa_few_tiles(a, cut, b, row) == 0 || r >= row.fresh * group) return;
+    const PaRow row = pa_row(a, b);
+    if (row.keys == 0 || r >= row.fresh * group) return;
     const int2 first = firsts[b];                                 // (the row had a first piece: it was written)
     if (first.y < 2) return;
     const size_t step = a.kv_heads * pa_part_floats(dp, nt);
@@ -431,58 +425,64 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, PaCut
 // LDS pieces of 16 bytes are laid out by XOR so that neither the writes (one key, all columns) nor the reads (linear) meet in a bank.
 #define PM_ROWS 128
 
-// Which query tiles the kernel for many queries walks, and how their keys are cut (in `pieces` equal parts for every tile of a row)
+// A tile of queries and a piece of its keys (all tiles of a row are cut in the same number of `pieces`)
 struct PmItem { int row, tile, piece, pieces; };
 
-__device__ __forceinline__ int pm_tiles(const PagedAttn& a, int few, int b, PaRow& r)
-{
-    r = pa_row(a, b);
-    const int64_t queries = (int64_t) r.fresh * (a.heads / a.kv_heads);
-    return queries > few ? (int) ((queries + PM_ROWS - 1) / PM_ROWS) : 0;
-}
-
-// Item `w` of the launch; row < 0: none.  Tiles of a row come with the last (the longest) first.  lds: 80 bytes, free again afterwards.
+// Item `w` of the launch; row < 0: none.  The cost of a row is tiles of queries * tiles of keys; with `piece` = a `target`-th of all rows' cost
+// (or min_piece), rows of 1.5 times as many keys or more are cut into pieces of about that size -- 4 / 3 * target items at most, and these come first: an item's number is its place
+// among the partial results.  Tiles of a row come with the last (the longest) first; where every item of the launch is resident at once, the
+// second half comes shortest first: the two workgroups of a compute unit, half a launch apart, then have equal work together.
+// lds: 80 bytes, free again afterwards.
 __device__ __forceinline__ PmItem pm_find(const PagedAttn& a, const PaCut& cut, int w, void* lds)
 {
-    int64_t (*sums)[PA_WAVES] = (int64_t (*)[PA_WAVES]) lds;
-    PmItem& found = *(PmItem*) (sums + 2);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    PaRow r;
-    int64_t cost = 0, count = 0;
-    for (int b = tid; b < a.n; b += PA_WAVES * 64) {
-        const int q = pm_tiles(a, cut.few, b, r);
-        count += q;
-        cost += (int64_t) q * ((r.keys + PA_KEYS - 1) / PA_KEYS);
-    }
+    int64_t* sums = (int64_t*) lds;
+    PmItem& found = *(PmItem*) (sums + 2 * PA_WAVES);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, step = PA_WAVES * 64;
+    struct Size { int q, keys; };
+    auto size = [&](int b) -> Size {
+        const PaRow r = pa_row(a, b);
+        const int64_t queries = (int64_t) r.fresh * (a.heads / a.kv_heads);
+        return {(int) ((queries + PM_ROWS - 1) / PM_ROWS), (r.keys + PA_KEYS - 1) / PA_KEYS};
+    };
+    auto total = [&](int64_t v, int at) -> int64_t {               // over the workgroup
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) { cost += __shfl_xor(cost, off, 64); count += __shfl_xor(count, off, 64); }
-    if (lane == 0) { sums[0][wave] = cost; sums[1][wave] = count; }
+        for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+        if (lane == 0) sums[at * PA_WAVES + wave] = v;
+        __syncthreads();
+        return sums[at * PA_WAVES] + sums[at * PA_WAVES + 1] + sums[at * PA_WAVES + 2] + sums[at * PA_WAVES + 3];
+    };
+    const Size mine = tid < a.n ? size(tid) : Size{0, 0};           // (of the first 256 rows, kept)
+    int64_t cost = 0;
+    for (int b = tid; b < a.n; b += step) { const Size z = b == tid ? mine : size(b); cost += (int64_t) z.q * z.keys; }
     if (tid == 0) found = {-1, 0, 0, 0};
-    __syncthreads();
-    cost = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
-    count = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
-    // enough tiles to fill the machine are not cut; pieces number at most target + count <= 2 * target
-    int64_t piece = (cost + cut.target - 1) / cut.target;
-    piece = count >= cut.target || !cut.split ? (int64_t) 1 << 40 : piece > cut.min_piece ? piece : cut.min_piece;
-    int64_t before = 0;
-    for (int b0 = 0; b0 < a.n; b0 += PA_WAVES * 64) {
+    cost = total(cost, 0);
+    const int64_t even = (cost + cut.target - 1) / cut.target;
+    const int piece = (int) min(max(even, (int64_t) cut.min_piece), (int64_t) 1 << 30);
+    auto pieces = [&](const Size& z) { return max((int) (((int64_t) z.keys + piece / 2) / piece), 1); };
+    int64_t cuts = 0;
+    for (int b = tid; b < a.n; b += step) { const Size z = b == tid ? mine : size(b); const int np = pieces(z); if (np > 1) cuts += (int64_t) z.q * np; }
+    cuts = total(cuts, 1);
+    const bool first = w < cuts;                                  // among the rows that are cut, or behind them
+    int64_t before = first ? 0 : cuts, count = 0;
+    for (int b0 = 0; b0 < a.n; b0 += step) {
         const int b = b0 + tid;
-        const int q = b < a.n ? pm_tiles(a, cut.few, b, r) : 0;
-        const int np = q ? (int) (((r.keys + PA_KEYS - 1) / PA_KEYS + piece - 1) / piece) : 0;
-        const int64_t mine = (int64_t) q * np;
-        int64_t inc = mine;
+        const Size z = b >= a.n ? Size{0, 0} : b0 == 0 ? mine : size(b);
+        const int np = pieces(z);
+        const int64_t here = (np > 1) == first ? (int64_t) z.q * np : 0;
+        int64_t inc = here;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) { const int64_t o = __shfl_up(inc, off, 64); if (lane >= off) inc += o; }
         __syncthreads();
-        if (lane == 63) sums[0][wave] = inc;
+        if (lane == 63) sums[wave] = inc;
         __syncthreads();
-        int64_t base = before + inc - mine;
-        for (int u = 0; u < wave; ++u) base += sums[0][u];
-        if (w >= base && w < base + mine) {
-            const int k = (int) (w - base);
-            found = {b, q - 1 - k / np, k % np, np};
+        int64_t base = before + inc - here;
+        for (int u = 0; u < wave; ++u) base += sums[u];
+        if (w >= base && w < base + here) {
+            const int k = (int) (w - base), t = k / np, half = (z.q + 1) / 2;
+            const bool fold = !first && cost <= (int64_t) cut.target * z.keys;        // (as many tiles as fit at once, or fewer)
+            found = {b, fold && t >= half ? t - half : z.q - 1 - t, k % np, np};
         }
-        before += sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+        before += sums[0] + sums[1] + sums[2] + sums[3];
         if (before > w) break;
     }
     __syncthreads();
@@ -499,7 +499,9 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     constexpr int KB = DP / 16, DT = DP / 32, PIECES = PA_KEYS * KB / 256;       // 16-byte pieces of codes per thread: keys, and as many of values
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // [2][keys: 2 * KB * 1024 bytes, values: 4 * DT * 1024 bytes]
     constexpr int K_BYTES = 2 * KB * 1024, BUF = 2 * K_BYTES;
-    const int kvh = blockIdx.y, w = blockIdx.x;
+    // kv heads next to each other in launch order: consecutive workgroups go to different XCDs, so that those of one head (the same keys and
+    // values) share an XCD's L2 where kv_heads is a multiple of 8, and every XCD gets tiles of all lengths
+    const int kvh = blockIdx.x % a.kv_heads, w = blockIdx.x / a.kv_heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, g = lane >> 5;
     const PmItem it = pm_find(a, cut, w, lds);
     if (kvh == 0 && tid == 0 && w < part_items) items[w] = it;                   // for the joining kernel
@@ -741,43 +743,51 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     }
 }
 
-// The pieces of a query tile joined, in order: one wave per query.
-__global__ __launch_bounds__(256) void paged_attn_join_many_kernel(PagedAttn a, const float* __restrict__ parts, const PmItem* __restrict__ items, int dp)
+// The pieces of a query tile joined, in order: 16 lanes for a query, 32 queries of an item for a workgroup (most of which find nothing to do).
+template <int DP> __global__ __launch_bounds__(256) void paged_attn_join_many_kernel(PagedAttn a, const float* __restrict__ parts, const PmItem* __restrict__ items)
 {
-    const int w = blockIdx.x, kvh = blockIdx.y, q = blockIdx.z * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    constexpr int V = DP / 64;                                    // groups of four columns of a lane
+    const int w = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x & 15;
     const PmItem it = items[w];
     if (it.row < 0 || it.piece != 0 || it.pieces < 2) return;
     const PaRow row = pa_row(a, it.row);
     const int group = a.heads / a.kv_heads;
-    const int64_t r = (int64_t) it.tile * PM_ROWS + q;
-    if (r >= (int64_t) row.fresh * group) return;
-    const size_t step = (size_t) a.kv_heads * PM_ROWS * (dp + 4);
-    const float* p0 = parts + (((size_t) w * a.kv_heads + kvh) * PM_ROWS + q) * (dp + 4);
-    float top = -INFINITY;
-    for (int k = lane; k < it.pieces; k += 64) top = fmaxf(top, p0[k * step + dp]);
+    const size_t step = (size_t) a.kv_heads * PM_ROWS * (DP + 4);
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < 2; ++u) {
+        const int q = blockIdx.z * 32 + u * 16 + (threadIdx.x >> 4);
+        const int64_t r = (int64_t) it.tile * PM_ROWS + q;
+        if (r >= (int64_t) row.fresh * group) return;
+        const float* p0 = parts + (((size_t) w * a.kv_heads + kvh) * PM_ROWS + q) * (DP + 4);
+        float top = -INFINITY;
+        for (int k = lane; k < it.pieces; k += 16) top = fmaxf(top, p0[k * step + DP]);
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 16));
+        float sum = 0.f;
+        f32x4 o[V] = {};
 #pragma unroll 2
-    for (int k = 0; k < it.pieces; ++k) {
-        const float* p = p0 + k * step;
-        const float f = p[dp] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[dp] - top);
-        sum += f * p[dp + 1];
+        for (int k = 0; k < it.pieces; ++k) {
+            const float* p = p0 + k * step;
+            const float m = p[DP], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            sum += f * p[DP + 1];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) if (64 * j < dp) o[j] += f * p[64 * j + lane];
+            for (int j = 0; j < V; ++j) o[j] += f * *(const f32x4*) (p + 64 * j + 4 * lane);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        f16* out = a.out + (size_t) (row.start + (int) (r / group)) * a.heads * a.hd + (size_t) (kvh * group + (int) (r % group)) * a.hd;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int d = 64 * j + 4 * lane;
+            f16x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = (f16) (o[j][e] * inv);
+            if (d < a.hd) *(f16x4*) (out + d) = x;                  // (head_dim is a multiple of four)
+        }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    f16* out = a.out + (size_t) (row.start + (int) (r / group)) * a.heads * a.hd + (size_t) (kvh * group + (int) (r % group)) * a.hd;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) if (64 * j + lane < a.hd) out[64 * j + lane] = (f16) (o[j] * inv);
 }
 
-// How a call is cut, from what the host knows: the kernel for few queries takes rows of up to `few` of them (NT tiles of 16)
-struct PaPlan {
-    int dp, nt, group, items, rows_y; PaCut cut; size_t first_bytes, part_bytes;          // few queries
-    bool many; int many_items, many_parts; PaCut many_cut; size_t many_item_bytes, many_part_bytes;
-    size_t bytes() const { return first_bytes + part_bytes + many_item_bytes + many_part_bytes; }
-};
+// How a call is cut, from what the host knows: most queries of a row (max_new * group) up to 16 * NT: the kernel for few queries, else the other
+struct PaPlan { int dp, nt, group, items, parts, rows_y; bool many, split; PaCut cut; size_t item_bytes, part_bytes; };
 static size_t pa_round(size_t n) { return (n + 255) / 256 * 256; }
 
 static PaPlan pa_plan(int n, int rows, int max_new, int heads, int kv_heads, int hd, int width, int block)
@@ -785,63 +795,61 @@ static PaPlan pa_plan(int n, int rows, int max_new, int heads, int kv_heads, int
     PaPlan p;
     p.dp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
     p.group = heads / kv_heads;
-    const int64_t queries = (int64_t) (max_new < rows ? max_new : rows) * p.group;
-    const int most = p.dp == 256 ? 16 : 32;
-    p.nt = queries <= 16 || queries > most ? 1 : 2;
-    p.many = queries > most;
-    p.cut.few = 16 * p.nt;
-    p.rows_y = (int) (queries < p.cut.few ? queries : p.cut.few);
-    p.cut.target = kv_heads >= 1024 ? 1 : 1024 / kv_heads;
-    p.cut.min_piece = PA_WAVES;
-    p.cut.split = n <= PA_MAX_ROWS && (int64_t) width * block > p.cut.min_piece * PA_KEYS;
-    p.items = n > PA_MAX_ROWS || !p.cut.split ? n : p.cut.target + n;
-    p.first_bytes = pa_round((size_t) n * sizeof(int2));
-    p.part_bytes = p.cut.split ? pa_round((size_t) p.items * kv_heads * pa_part_floats(p.dp, p.nt) * sizeof(float)) : 0;
-    p.many_items = p.many_parts = 0;
-    p.many_item_bytes = p.many_part_bytes = 0;
-    if (p.many) {
+    const int64_t queries = (int64_t) (max_new < rows ? max_new : rows) * p.group, longest = (int64_t) width * block;
+    p.many = queries > (p.dp == 256 ? 16 : 32);
+    p.nt = queries <= 16 ? 1 : 2;
+    p.rows_y = (int) queries;
+    if (!p.many) {
+        p.cut = {kv_heads >= 1024 ? 1 : 1024 / kv_heads, PA_WAVES};
+        p.split = n <= PA_MAX_ROWS && longest > p.cut.min_piece * PA_KEYS;
+        p.items = p.parts = p.split ? p.cut.target + n : n;
+        p.item_bytes = pa_round((size_t) n * sizeof(int2));
+        p.part_bytes = p.split ? pa_round((size_t) p.parts * kv_heads * pa_part_floats(p.dp, p.nt) * sizeof(float)) : 0;
+    } else {
         const int64_t fresh = (int64_t) n * max_new < rows ? (int64_t) n * max_new : rows, tiles = (fresh * p.group + PM_ROWS - 1) / PM_ROWS + n;
-        p.many_cut = {p.cut.few, kv_heads >= 512 ? 1 : 512 / kv_heads, 8, (int64_t) width * block > 8 * PA_KEYS};
-        p.many_parts = p.many_cut.split ? 2 * p.many_cut.target : 0;
-        p.many_items = (int) (tiles > p.many_parts ? tiles : p.many_parts);
-        p.many_item_bytes = pa_round((size_t) p.many_parts * sizeof(PmItem));
-        p.many_part_bytes = pa_round((size_t) p.many_parts * kv_heads * PM_ROWS * (p.dp + 4) * sizeof(float));
+        p.cut = {kv_heads >= 512 ? 1 : 512 / kv_heads, 8};
+        p.split = longest > p.cut.min_piece * PA_KEYS;
+        p.parts = p.split ? 2 * p.cut.target : 0;
+        p.items = (int) (tiles + p.parts < 0x7fffffff ? tiles + p.parts : 0x7fffffff);
+        p.item_bytes = pa_round((size_t) p.parts * sizeof(PmItem));
+        p.part_bytes = pa_round((size_t) p.parts * kv_heads * PM_ROWS * (p.dp + 4) * sizeof(float));
     }
     return p;
 }
 
 template <int CODE> static int pa_launch(const PagedAttn& a, const PaPlan& p, void* workspace, hipStream_t s)
 {
-    int2* firsts = (int2*) workspace;
-    float* parts = (float*) ((char*) workspace + p.first_bytes);
-    const dim3 grid((unsigned) p.items, (unsigned) a.kv_heads);
+    float* parts = (float*) ((char*) workspace + p.item_bytes);
+    EXL_REQUIRE((int64_t) p.items * a.kv_heads <= 0x7fffffff, EXL_E_UNSUPPORTED, "paged_attention: too many rows for %d kv heads", a.kv_heads);
+    const dim3 grid((unsigned) p.items * (unsigned) a.kv_heads);
+    if (!p.many) {
+        int2* firsts = (int2*) workspace;
 #define PA_FEW(DP, NT) hipLaunchKernelGGL((paged_attn_few_kernel<CODE, DP, NT>), grid, dim3(PA_WAVES * 64), 0, s, a, p.cut, parts, firsts)
-    if (p.dp == 64)       { if (p.nt == 1) PA_FEW(64, 1); else PA_FEW(64, 2); }
-    else if (p.dp == 128) { if (p.nt == 1) PA_FEW(128, 1); else PA_FEW(128, 2); }
-    else                  PA_FEW(256, 1);
+        if (p.dp == 64)       { if (p.nt == 1) PA_FEW(64, 1); else PA_FEW(64, 2); }
+        else if (p.dp == 128) { if (p.nt == 1) PA_FEW(128, 1); else PA_FEW(128, 2); }
+        else                  PA_FEW(256, 1);
 #undef PA_FEW
-    EXL_LAUNCH_CHECK();
-    if (p.cut.split) {
-        hipLaunchKernelGGL(paged_attn_join_kernel, dim3((unsigned) a.n, (unsigned) p.rows_y, (unsigned) a.kv_heads), dim3(256), 0, s, a, p.cut, parts, firsts, p.dp,
-                           p.nt);
         EXL_LAUNCH_CHECK();
-    }
-    if (p.many) {
-        PmItem* items = (PmItem*) ((char*) parts + p.part_bytes);
-        float* more = (float*) ((char*) items + p.many_item_bytes);
-        const dim3 mgrid((unsigned) p.many_items, (unsigned) a.kv_heads);
-#define PA_MANY(DP, WIDE) do { static bool done[EXL_MAX_DEVICES] = {};                                                                       \
-        EXL_TRY(exl_lds_opt_in((const void*) paged_attn_many_kernel<CODE, DP, WIDE>, done));                                                  \
-        hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE>), mgrid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4, s, a, p.many_cut, more, items, \
-                           p.many_parts); } while (0)
-        if (a.block >= PA_KEYS) { if (p.dp == 64) PA_MANY(64, true); else if (p.dp == 128) PA_MANY(128, true); else PA_MANY(256, true); }
-        else                    { if (p.dp == 64) PA_MANY(64, false); else if (p.dp == 128) PA_MANY(128, false); else PA_MANY(256, false); }
-#undef PA_MANY
-        EXL_LAUNCH_CHECK();
-        if (p.many_parts) {
-            hipLaunchKernelGGL(paged_attn_join_many_kernel, dim3((unsigned) p.many_parts, (unsigned) a.kv_heads, PM_ROWS / 4), dim3(256), 0, s, a, more, items, p.dp);
+        if (p.split) {
+            hipLaunchKernelGGL(paged_attn_join_kernel, dim3((unsigned) a.n, (unsigned) p.rows_y, (unsigned) a.kv_heads), dim3(256), 0, s, a, parts, firsts, p.dp, p.nt);
             EXL_LAUNCH_CHECK();
         }
+        return 0;
+    }
+    PmItem* items = (PmItem*) workspace;
+#define PA_MANY(DP, WIDE) do { static bool done[EXL_MAX_DEVICES] = {};                                                                       \
+    EXL_TRY(exl_lds_opt_in((const void*) paged_attn_many_kernel<CODE, DP, WIDE>, done));                                                      \
+    hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE>), grid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4, s, a, p.cut, parts, items, p.parts); } while (0)
+    if (a.block >= PA_KEYS) { if (p.dp == 64) PA_MANY(64, true); else if (p.dp == 128) PA_MANY(128, true); else PA_MANY(256, true); }
+    else                    { if (p.dp == 64) PA_MANY(64, false); else if (p.dp == 128) PA_MANY(128, false); else PA_MANY(256, false); }
+#undef PA_MANY
+    EXL_LAUNCH_CHECK();
+    if (p.split) {
+        const dim3 jgrid((unsigned) p.parts, (unsigned) a.kv_heads, PM_ROWS / 32);
+        if (p.dp == 64)       hipLaunchKernelGGL((paged_attn_join_many_kernel<64>), jgrid, dim3(256), 0, s, a, parts, items);
+        else if (p.dp == 128) hipLaunchKernelGGL((paged_attn_join_many_kernel<128>), jgrid, dim3(256), 0, s, a, parts, items);
+        else                  hipLaunchKernelGGL((paged_attn_join_many_kernel<256>), jgrid, dim3(256), 0, s, a, parts, items);
+        EXL_LAUNCH_CHECK();
     }
     return 0;
 }
@@ -852,7 +860,7 @@ extern "C" size_t exl_paged_attention_workspace(int n_rows, int rows, int max_ne
     if (n_rows <= 0 || rows <= 0 || max_new <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 || table_width <= 0 ||
         block_size <= 0) return 0;
     const PaPlan p = pa_plan(n_rows, rows, max_new, num_heads, num_kv_heads, head_dim, table_width, block_size);
-    return p.bytes();
+    return p.item_bytes + p.part_bytes;
 }
 
 extern "C" int exl_paged_attention(const void* q, long q_stride, const int32_t* starts, const int32_t* past_lens, const int32_t* new_lens, int n_rows,
@@ -879,7 +887,7 @@ extern "C" int exl_paged_attention(const void* q, long q_stride, const int32_t* 
                    num_kv_heads, head_dim, (head_dim + 15) / 16 * 16, angle_rows, q_stride, scale > 0.f ? scale : 1.f / sqrtf((float) head_dim)};
     hipStream_t s = (hipStream_t) stream;
     const PaPlan p = pa_plan(n_rows, rows, max_new, num_heads, num_kv_heads, head_dim, table_width, block_size);
-    EXL_REQUIRE(workspace && (uintptr_t) workspace % 16 == 0 && workspace_bytes >= p.bytes(), EXL_E_TOO_SMALL,
-                "paged_attention: the workspace is too small (%zu < %zu bytes) or not 16-byte aligned", workspace_bytes, p.bytes());
+    EXL_REQUIRE(workspace && (uintptr_t) workspace % 16 == 0 && workspace_bytes >= p.item_bytes + p.part_bytes, EXL_E_TOO_SMALL,
+                "paged_attention: the workspace is too small (%zu < %zu bytes) or not 16-byte aligned", workspace_bytes, p.item_bytes + p.part_bytes);
     return code == EXL_PAGE_FP8 ? pa_launch<EXL_PAGE_FP8>(a, p, workspace, s) : pa_launch<EXL_PAGE_INT8>(a, p, workspace, s);
 }
