@@ -24,17 +24,18 @@ __device__ __forceinline__ PaRow pa_row(const PagedAttn& a, int b)
 }
 
 // ---- rows of few queries: the cache's bytes are all that counts ------------------------------------------------------------------------
-// One workgroup (4 waves) streams a piece of one row's keys and values of one kv head, in tiles of 64 keys, for all of the row's queries and
-// all query heads of that kv head (up to 16 * NT of them: GQA reads the cache once).  Both products are MFMAs on fp16 numbers converted from the
-// codes in registers; nothing goes through LDS in the loop:
+// The tiles of 64 keys of all rows lie in one line, row behind row (each with PA_BEGIN places before it, for what beginning a row costs), and
+// every wave takes an equal stretch of it for one kv head: whatever the rows' lengths, all waves end together, none waits for another, and the next row's first tile is on its way while the last one's last is worked on.
+// A wave does all queries of its row that read the kv head (up to 16 * NT: tokens * heads of the group, GQA reads the cache once).  A row
+// that lies in one stretch is written; the others leave one partial result for each stretch, joined in order by a second kernel -- the cut
+// depends on the lengths alone, so results do not depend on scheduling.
+// Both products are MFMAs on fp16 numbers converted from the codes in registers; nothing goes through LDS:
 //   S^T = K Q^T   (16x16x32): A = keys.  MFMA row m of product t4 is key 16 * (m >> 2) + 4 * t4 + (m & 3) of the tile, so that a lane (query
 //                 column c = lane & 15, group g = lane >> 4) gets the 16 scores of keys 16 g .. 16 g + 15, in order, over the four products;
 //   O^T = V^T P^T : A = value columns, 16 bytes = keys 16 g .. 16 g + 15 of one column, as the page holds them; B = the lane's own 16 weights.
-// Running maximum and sum stay in the lane of the query; the four waves (64 keys each in turn) join through LDS at the end.  A piece's key range is
-// a function of the lengths alone, and the pieces of a row are joined in order: results do not depend on scheduling.
 #define PA_WAVES 4
 #define PA_KEYS 64
-#define PA_MAX_ROWS 1024                                       // rows of the batch up to which their keys are cut into pieces of equal size
+#define PA_BEGIN 1
 
 // A page's scale as the conversions take it.  int8: 2^e is the exponent field of the fp16 numbers that a code's byte becomes the mantissa of:
 // (1024 + u) * 2^e with u = code + 128, minus 1152 * 2^e -- up to e = 5; beyond (`big`, for every lane as soon as one has it) a product follows.
@@ -101,77 +102,81 @@ __device__ __forceinline__ PaQuery pa_query(const PagedAttn& a, const f16* q, in
         }
         return r;
     }
-    for (int i = 0; i < 8; ++i) {                                // head_dim not a multiple of 16: the halves meet inside eight elements
-        const int e = d + i;
+#pragma unroll
+    for (int u = 0; u < 8; u += 4) {                             // head_dim a multiple of 4: in fours, whose other halves lie in fours too, but for the four in the middle
+        const int e = d + u;
         if (e >= a.hd) break;
-        float x = (float) q[e];
-        if (sin) x = fmaf(x, (float) cos[e], (e < half ? -(float) q[e + half] : (float) q[e - half]) * (float) sin[e]);
-        put(i, x);
+        const f16x4 x = *(const f16x4_a4*) (q + e);
+        f16x4 o = {}, si = {}, co = {};
+        if (sin) {
+            si = *(const f16x4_a4*) (sin + e);
+            co = *(const f16x4_a4*) (cos + e);
+            if (e + 4 <= half || e >= half) o = *(const f16x4_a4*) (q + (e < half ? e + half : e - half));
+            else for (int i = 0; i < 4; ++i) o[i] = q[e + i < half ? e + i + half : e + i - half];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put(u + i, sin ? fmaf((float) x[i], (float) co[i], (e + i < half ? -(float) o[i] : (float) o[i]) * (float) si[i]) : (float) x[i]);
     }
     return r;
 }
 
-// How the keys of all rows are cut: pieces of equal size, about `target` of them, none of less than `min_piece` tiles
+// How the work is cut: few queries: `target` waves for a kv head, no stretch of less than `min_piece` tiles; many queries: pm_find below
 struct PaCut { int target, min_piece; };
 
-__device__ __forceinline__ int pa_tiles(const PagedAttn& a, int b) { return (pa_row(a, b).keys + PA_KEYS - 1) / PA_KEYS; }
-
-struct PaItem { int row, first, last, piece, pieces; };          // tiles first .. last - 1, piece number `piece` of `pieces`
-
-// Item `w` of the launch; row < 0: none.  Every thread of the workgroup calls it.
-__device__ __forceinline__ PaItem pa_find(const PagedAttn& a, const PaCut& cut, int w)
+// A row by scalar loads (b is the same in every lane)
+__device__ __forceinline__ PaRow pa_row_of_wave(const PagedAttn& a, int b)
 {
-    __shared__ int64_t sums[PA_WAVES];
-    __shared__ PaItem found;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    PaItem it = {-1, 0, 0, 0, 0};
-    if (a.n > PA_MAX_ROWS) {
-        const int tiles = pa_tiles(a, w);
-        if (tiles > 0) it = {w, 0, tiles, 0, 1};
-        return it;
-    }
-    int64_t total = 0;
-    int tiles0 = 0;
-    for (int b = tid; b < a.n; b += PA_WAVES * 64) {
-        const int tiles = pa_tiles(a, b);
-        if (b == tid) tiles0 = tiles;
-        total += tiles;
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
-    if (lane == 0) sums[wave] = total;
-    if (tid == 0) found = it;
-    __syncthreads();
-    total = sums[0] + sums[1] + sums[2] + sums[3];
-    const int64_t even = (total + cut.target - 1) / cut.target;
-    const int piece = (int) (even > cut.min_piece ? even : cut.min_piece);
-    int before = 0;
-    for (int b0 = 0; b0 < a.n; b0 += PA_WAVES * 64) {
-        const int b = b0 + tid;
-        const int tiles = b >= a.n ? 0 : b0 == 0 ? tiles0 : pa_tiles(a, b);
-        const int mine = (tiles + piece - 1) / piece;
-        int inc = mine;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) { const int o = __shfl_up(inc, off, 64); if (lane >= off) inc += o; }
-        __syncthreads();
-        if (lane == 63) sums[wave] = inc;
-        __syncthreads();
-        int base = before + inc - mine;
-        for (int u = 0; u < wave; ++u) base += (int) sums[u];
-        if (w >= base && w < base + mine) {
-            const int k = w - base;
-            // equal pieces: their number is settled, the tiles are shared out evenly
-            found = {b, (int) ((int64_t) tiles * k / mine), (int) ((int64_t) tiles * (k + 1) / mine), k, mine};
-        }
-        before += (int) (sums[0] + sums[1] + sums[2] + sums[3]);
-        if (before > w) break;
-    }
-    __syncthreads();
-    return found;
+    typedef const __attribute__((address_space(4))) int32_t* scalar;
+    PaRow r;
+    r.start = min(max(((scalar) a.starts)[b], 0), a.rows);
+    r.fresh = min(min(max(((scalar) a.fresh)[b], 0), a.max_new), a.rows - r.start);
+    r.past = max(((scalar) a.past)[b], 0);
+    r.keys = r.fresh ? (int) min((int64_t) r.past + r.fresh, (int64_t) a.width * a.block) : 0;
+    return r;
 }
 
-// Partial results of an item that is one of several pieces: [item * kv_heads + kv_head][16 * NT queries][DP + 2] floats (o, then m and l)
-__host__ __device__ constexpr size_t pa_part_floats(int dp, int nt) { return (size_t) 16 * nt * (dp + 2); }
+// Stretch `w` of the line: `count` places from place `from` of row `row` on, the first of them number `at` of the line; `share`: places of a stretch
+struct PaStretch { int row, from, count, share; int64_t at; };
+__device__ __forceinline__ PaStretch pa_stretch(const PagedAttn& a, const PaCut& cut, int w)
+{
+    const int lane = threadIdx.x & 63;
+    auto places = [&](int b) { const int keys = b < a.n ? pa_row(a, b).keys : 0; return keys ? (keys + PA_KEYS - 1) / PA_KEYS + PA_BEGIN : 0; };
+    const int mine = places(lane);                                 // (of the first 64 rows, kept)
+    int64_t total = mine;
+    for (int b = lane + 64; b < a.n; b += 64) total += places(b);
+    if (a.n == 1) total = __builtin_amdgcn_readfirstlane(mine);
+    else {
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+    }
+    PaStretch st = {-1, 0, 0, 0, 0};
+    const int64_t even = (total + cut.target - 1) / cut.target;
+    st.share = (int) (even > cut.min_piece ? even : cut.min_piece);
+    st.at = (int64_t) w * st.share;
+    if (st.at >= total) return st;
+    st.count = (int) min((int64_t) st.share, total - st.at);
+    if (a.n == 1) { st.row = 0; st.from = (int) st.at; return st; }
+    int64_t before = 0;
+    for (int b0 = 0; b0 < a.n; b0 += 64) {
+        const int t = b0 == 0 ? mine : places(b0 + lane);
+        int64_t inc = t;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) { const int64_t o = __shfl_up(inc, off, 64); if (lane >= off) inc += o; }
+        const int64_t from = before + inc - t;
+        const uint64_t hit = __ballot(st.at >= from && st.at < from + t);
+        if (hit) {
+            const int l = __ffsll((unsigned long long) hit) - 1;
+            st.row = b0 + l;
+            st.from = __builtin_amdgcn_readlane((int) (st.at - from), l);
+            return st;
+        }
+        before += __shfl(inc, 63, 64);
+    }
+    return st;
+}
+
+// A partial result: [queries][DP + 4] floats (o, then m and l); a stretch has room for two: of the row that it continues, and of the one that goes on
+__host__ __device__ constexpr size_t pa_part_floats(int dp, int nt) { return (size_t) 16 * nt * (dp + 4); }
 
 // Registers (DP = 128, NT = 1): 64 for a tile's bytes, twice (the next tile is on its way while one is worked on), 32 of O, 32 of Q: two waves per
 // SIMD.  Twice the queries take one wave per SIMD, and so do wider heads, without the second set of bytes.
@@ -179,57 +184,19 @@ template <int CODE, int DP, int NT>
 __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_attn_few_kernel(PagedAttn a, PaCut cut, float* __restrict__ parts,
                                                                                             int2* __restrict__ firsts)
 {
-    constexpr int KS = DP / 64, DT = DP / 16, ROW = DP + 4;
+    constexpr int KS = DP / 64, DT = DP / 16;
     constexpr bool AHEAD = DP <= 128;
-    __shared__ __attribute__((aligned(16))) float joined[PA_WAVES][16 * ROW];
-    __shared__ float stat[PA_WAVES][2][16];
-    const int kvh = blockIdx.x % a.kv_heads, w = blockIdx.x / a.kv_heads;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-    const PaItem it = pa_find(a, cut, w);
-    if (it.row < 0) return;
-    if (kvh == 0 && tid == 0 && it.piece == 0) firsts[it.row] = make_int2(w, it.pieces);       // for the joining kernel
-    const PaRow row = pa_row(a, it.row);
-    const int group = a.heads / a.kv_heads, queries = row.fresh * group;
-    const int lbs = 31 - __clz(a.block);
-
-    f16x8 qf[NT][KS][2], ql[NT][KS][2];                          // (the query and what fp16 leaves of it: the matrix cores have time for both)
-    int limit[NT];                                               // the last key this lane's query sees
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int r = nt * 16 + c, i = r / group;
-        const bool in = r < queries;
-        limit[nt] = in ? (int) min((int64_t) row.past + i, (int64_t) row.keys - 1) : -1;
-        const f16* q = a.q + (size_t) (row.start + (in ? i : 0)) * a.q_stride + (size_t) (kvh * group + (in ? r % group : 0)) * a.hd;
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                PaQuery x = pa_query(a, q, (int64_t) row.past + i, 64 * s + 16 * g + 8 * half);
-                if (!in) x = {};
-                qf[nt][s][half] = x.hi;
-                ql[nt][s][half] = x.lo;
-            }
-    }
-
-    const int32_t* table = a.table + (size_t) it.row * a.width;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int worker = __builtin_amdgcn_readfirstlane(blockIdx.x * PA_WAVES + (threadIdx.x >> 6)), kvh = worker % a.kv_heads, w = worker / a.kv_heads;
+    const PaStretch to = pa_stretch(a, cut, w);
+    if (to.row < 0) return;
+    const int group = a.heads / a.kv_heads, lbs = 31 - __clz(a.block);
     const size_t kpage = (size_t) a.block * a.hd16;              // bytes of one page of one head, keys or values
-    // byte offsets inside a key row / inside a value page; columns behind head_dim read column 0 (their queries are zeros, their results unused)
-    int kd[KS], vd[DT];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) kd[s] = 64 * s + 16 * g < a.hd16 ? 64 * s + 16 * g : 0;
-#pragma unroll
-    for (int t = 0; t < DT; ++t) vd[t] = (16 * t + c < a.hd16 ? 16 * t + c : 0) * a.block;
-
-    struct Ids { int k, v; };
-    auto look = [&](int tile) -> Ids {                            // the pages of this lane's key rows and of its group's values
-        const int ik = (tile * PA_KEYS + 16 * (c >> 2)) >> lbs, iv = (tile * PA_KEYS + 16 * g) >> lbs;
-        Ids r = {-1, -1};
-        if (ik < a.width) r.k = table[ik];
-        if (iv < a.width) r.v = table[iv];
-        return r;
-    };
+    // (columns behind head_dim: key rows read column 0 again, value pages their last 16 columns; the queries there are zeros, the results unused)
     struct Stage { uint4 k[4][KS]; uint4 v[DT]; float ks, vs; bool there; };      // (scales as they are: looking at one here would wait for every load before it)
-    auto fetch = [&](int tile, Ids id, Stage& st) {
+    auto fetch = [&](int tile, const int32_t* table, Stage& st) {
+        const int ik = (tile * PA_KEYS + 16 * (c >> 2)) >> lbs, iv = (tile * PA_KEYS + 16 * g) >> lbs;      // the pages of this lane's key rows and of its group's values
+        struct { int k, v; } id = {ik < a.width ? table[ik] : -1, iv < a.width ? table[iv] : -1};
         const bool kok = id.k >= 0 && id.k < a.blocks, vok = id.v >= 0 && id.v < a.blocks;
         const size_t kb = (size_t) (kok ? id.k : 0) * a.kv_heads + kvh, vb = (size_t) (vok ? id.v : 0) * a.kv_heads + kvh;
         const int key = tile * PA_KEYS + 16 * (c >> 2) + (c & 3);
@@ -237,25 +204,47 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
 #pragma unroll
         for (int t4 = 0; t4 < 4; ++t4)
 #pragma unroll
-            for (int s = 0; s < KS; ++s) st.k[t4][s] = *(const uint4*) (kp + 4 * t4 * a.hd16 + kd[s]);
-        const uint8_t* vp = a.vp + vb * kpage + ((tile * PA_KEYS + 16 * g) & (a.block - 1));
+            for (int s = 0; s < KS; ++s) st.k[t4][s] = *(const uint4*) (kp + 4 * t4 * a.hd16 + (64 * s + 16 * g < a.hd16 ? 64 * s + 16 * g : 0));
+        const uint8_t* vp = a.vp + vb * kpage + c * a.block + ((tile * PA_KEYS + 16 * g) & (a.block - 1));
 #pragma unroll
-        for (int t = 0; t < DT; ++t) st.v[t] = *(const uint4*) (vp + vd[t]);
+        for (int t = 0; t < DT; ++t) st.v[t] = *(const uint4*) (vp + min(16 * t, a.hd16 - 16) * a.block);
         st.ks = a.ks[vb];
         st.vs = a.vs[vb];
         st.there = vok;
     };
 
-    f32x4 o[NT][DT];
-    float m[NT], l[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        m[nt] = -INFINITY; l[nt] = 0.f;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[nt][t] = (f32x4) {0.f, 0.f, 0.f, 0.f};
-    }
     const float c1 = a.scale * 1.44269504f;                       // scores in powers of two
     const PaScale one = pa_scale<CODE>(1.f);
+    f16x8 qf[NT][KS][2], ql[NT][KS][2];                          // the query and what fp16 leaves of it: the matrix cores have time for both
+    int limit[NT];                                               // the last key this lane's query sees
+    f32x4 o[NT][DT];
+    float m[NT], l[NT];
+    PaRow row;
+    auto begin = [&](int b) {                                     // the queries of row b
+        row = pa_row_of_wave(a, b);
+        const int queries = row.fresh * group;
+        int cc = c, gg = g;                                       // (opaque: what follows from them stays here and takes no registers in the loop over the tiles)
+        asm volatile("" : "+v"(cc), "+v"(gg));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * 16 + cc, i = r / group;
+            const bool in = r < queries;
+            limit[nt] = in ? (int) min((int64_t) row.past + i, (int64_t) row.keys - 1) : -1;
+            const f16* q = a.q + (size_t) (row.start + (in ? i : 0)) * a.q_stride + (size_t) (kvh * group + (in ? r - i * group : 0)) * a.hd;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    PaQuery x = pa_query(a, q, (int64_t) row.past + i, 64 * s + 16 * gg + 8 * half);
+                    if (!in) x = {};
+                    qf[nt][s][half] = x.hi;
+                    ql[nt][s][half] = x.lo;
+                }
+            m[nt] = -INFINITY; l[nt] = 0.f;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[nt][t] = (f32x4) {0.f, 0.f, 0.f, 0.f};
+        }
+    };
 
     auto work = [&](int tile, Stage& st) {
         const int key0 = tile * PA_KEYS + 16 * g;
@@ -330,96 +319,137 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
         }
     };
 
-    int tile = it.first + wave;
-    if (tile < it.last) {
-        Stage st;
-        fetch(tile, look(tile), st);
-        for (; tile < it.last; tile += PA_WAVES) {
-            const int next = tile + PA_WAVES;
-            if (AHEAD) {
-                Stage nx;
-                if (next < it.last) fetch(next, look(next), nx);
-                work(tile, st);
-                st = nx;
+    // a row's (or a stretch's) end: the sums of the four groups, and out.  `part`: where a partial result goes, or null
+    auto end = [&](float* part) {
+        int cc = c, gg = g;
+        asm volatile("" : "+v"(cc), "+v"(gg));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float sum = l[nt];
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            const int r = nt * 16 + cc, i = r / group;
+            if (r >= row.fresh * group) continue;
+            if (part) {
+                float* p = part + (size_t) r * (DP + 4);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) *(f32x4*) (p + 16 * t + 4 * gg) = o[nt][t];
+                if (gg == 0) { p[DP] = m[nt]; p[DP + 1] = sum; }
             } else {
-                work(tile, st);
-                if (next < it.last) fetch(next, look(next), st);
+                f16* out = a.out + (size_t) (row.start + i) * a.heads * a.hd + (size_t) (kvh * group + r - i * group) * a.hd;
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    f16x4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = (f16) (o[nt][t][e] * inv);
+                    if (16 * t + 4 * gg < a.hd) *(f16x4*) (out + 16 * t + 4 * gg) = x;      // (head_dim is a multiple of four)
+                }
             }
         }
-    }
+    };
 
-    // ---- the four waves' results, and out
-    float* part = parts + ((size_t) w * a.kv_heads + kvh) * pa_part_floats(DP, NT);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float ls = l[nt];
-        ls += __shfl_xor(ls, 16, 64);
-        ls += __shfl_xor(ls, 32, 64);
-        if (nt) __syncthreads();
-        if (g == 0) { stat[wave][0][c] = m[nt]; stat[wave][1][c] = ls; }
-        __syncthreads();
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int u = 0; u < PA_WAVES; ++u) top = fmaxf(top, stat[u][0][c]);
-        const float keep = m[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[nt] - top);
-#pragma unroll
-        for (int t = 0; t < DT; ++t) *(f32x4*) &joined[wave][c * ROW + 16 * t + 4 * g] = o[nt][t] * keep;
-        __syncthreads();
-        for (int x = tid; x < 16 * DP; x += PA_WAVES * 64) {
-            const int col = x / DP, d = x % DP, r = nt * 16 + col;
-            if (r >= queries) break;
-            const float v = joined[0][col * ROW + d] + joined[1][col * ROW + d] + joined[2][col * ROW + d] + joined[3][col * ROW + d];
-            top = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int u = 0; u < PA_WAVES; ++u) top = fmaxf(top, stat[u][0][col]);
-#pragma unroll
-            for (int u = 0; u < PA_WAVES; ++u) sum += stat[u][1][col] * (stat[u][0][col] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stat[u][0][col] - top));      // (0 * NaN: a NaN stays)
-            if (it.pieces == 1) {
-                if (d < a.hd)
-                    a.out[(size_t) (row.start + r / group) * a.heads * a.hd + (size_t) (kvh * group + r % group) * a.hd + d] = (f16) (sum == 0.f ? 0.f : v / sum);
-            } else {
-                part[(size_t) r * (DP + 2) + d] = v;
-                if (d == 0) { part[(size_t) r * (DP + 2) + DP] = top; part[(size_t) r * (DP + 2) + DP + 1] = sum; }
-            }
+    int b = to.row, from = to.from, left = to.count;              // the row, the first place of it that is this stretch's, places that are left
+    int64_t at = to.at - to.from;                                 // the row's first place in the line
+    if (from + left <= PA_BEGIN) return;                          // (no tile)
+    Stage st;
+    fetch(max(from - PA_BEGIN, 0), a.table + (size_t) b * a.width, st);
+    for (;;) {                                                    // the rows of the stretch
+        begin(b);
+        const int tiles = (row.keys + PA_KEYS - 1) / PA_KEYS, first = max(from - PA_BEGIN, 0), last = min(from + left - PA_BEGIN, tiles) - 1;
+        left -= tiles + PA_BEGIN - from;
+        int nb = b;                                               // the next row that has any keys, if it has a tile in this stretch
+        if (left > PA_BEGIN) do ++nb; while (nb < a.n - 1 && pa_row_of_wave(a, nb).keys == 0);
+        for (int tile = first; ; ++tile) {
+            const bool more = tile < last || nb != b;
+            const int32_t* table = a.table + (size_t) (tile < last ? b : nb) * a.width;
+            const int ntile = tile < last ? tile + 1 : 0;
+            Stage nx;
+            if (AHEAD && more) fetch(ntile, table, nx);
+            work(tile, st);
+            if (AHEAD) st = nx;
+            else if (more) fetch(ntile, table, st);
+            if (tile == last) break;
         }
+        const bool whole = first == 0 && last == tiles - 1;
+        float* part = parts + (((size_t) w * a.kv_heads + kvh) * 2 + (first == 0)) * pa_part_floats(DP, NT);
+        end(whole ? nullptr : part);
+        if (first == 0 && kvh == 0 && lane == 0)                  // for the joining kernel: where the row's parts begin, and how many there are
+            firsts[b] = make_int2(w, (int) ((at + PA_BEGIN + tiles - 1) / to.share) - w + 1);
+        if (nb == b) return;
+        at += tiles + PA_BEGIN;
+        b = nb;
+        from = 0;
     }
 }
 
-// The pieces of a row joined, in order: one workgroup per row of the batch, query and kv head.
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const float* __restrict__ parts, const int2* __restrict__ firsts, int dp, int nt)
+// The parts of a row joined: `each` (1, 2, 4, ...) queries of one row and kv head for a workgroup, dp / 4 lanes for a query; the lanes that are
+// left take every so many-th part each, with a maximum of their own, and meet in LDS -- in an order that depends on the lengths alone.
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const float* __restrict__ parts, const int2* __restrict__ firsts, int dp, int nt, int each)
 {
-    __shared__ float part_o[16][256 + 4];
-    __shared__ float part_l[16];
-    const int b = blockIdx.x, r = blockIdx.y, kvh = blockIdx.z, group = a.heads / a.kv_heads, tid = threadIdx.x;
+    __shared__ f32x4 slice_o[256];
+    __shared__ float slice_m[256], slice_l[256];
+    const int b = blockIdx.x, kvh = blockIdx.z, group = a.heads / a.kv_heads, tid = threadIdx.x;
     const PaRow row = pa_row(a, b);
-    if (row.keys == 0 || r >= row.fresh * group) return;
-    const int2 first = firsts[b];                                 // (the row had a first piece: it was written)
+    if (row.keys == 0 || (int) blockIdx.y * each >= row.fresh * group) return;
+    const int2 first = firsts[b];                                 // (the row had a first part: it was written)
     if (first.y < 2) return;
-    const size_t step = a.kv_heads * pa_part_floats(dp, nt);
-    const float* p0 = parts + ((size_t) first.x * a.kv_heads + kvh) * pa_part_floats(dp, nt) + (size_t) r * (dp + 2);
-    float top = -INFINITY;
-    for (int k = tid & 63; k < first.y; k += 64) top = fmaxf(top, p0[k * step + dp]);
+    const int lanes = dp >> 2, slices = 256 / (lanes * each), d = (tid % lanes) * 4, q = tid / lanes % each, sl = tid / (lanes * each);
+    const int r = blockIdx.y * each + q;
+    const size_t size = pa_part_floats(dp, nt), step = 2 * a.kv_heads * size;
+    const float* p0 = parts + (((size_t) first.x * a.kv_heads + kvh) * 2) * size + (size_t) r * (dp + 4);      // part 0 lies behind it, in the second place
+    float m = -INFINITY, sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (r < row.fresh * group) {
+        constexpr int U = 4;                                      // parts in flight
+        for (int k0 = sl; k0 < first.y; k0 += U * slices) {
+            float pm[U], pl[U];
+            f32x4 po[U];
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    const int lanes = dp >> 2, slices = 256 / lanes, sl = tid / lanes, d = (tid % lanes) * 4;      // dp 64, 128, 256: 16, 8, 4 slices of the pieces
-    float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-#pragma unroll 4
-    for (int k = sl; k < first.y; k += slices) {
-        const float* p = p0 + k * step;
-        const float m = p[dp], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-        sum += f * p[dp + 1];
+            for (int u = 0; u < U; ++u) {
+                const int k = min(k0 + u * slices, first.y - 1);
+                const float* p = p0 + (k ? k * step : size);
+                pm[u] = k0 + u * slices < first.y ? p[dp] : -INFINITY;
+                pl[u] = p[dp + 1];
+                po[u] = *(const f32x4*) (p + d);
+            }
+            float top = m;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] += f * p[d + j];
+            for (int u = 0; u < U; ++u) top = fmaxf(top, pm[u]);
+            const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            sum *= keep;
+            o *= keep;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k0 + u * slices >= first.y) break;
+                const float f = pm[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm[u] - top);
+                sum += f * pl[u];
+                o += f * po[u];
+            }
+            m = top;
+        }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) part_o[sl][d + j] = o[j];
-    if (d == 0) part_l[sl] = sum;
+    slice_o[tid] = o;
+    slice_m[tid] = m;
+    slice_l[tid] = sum;
     __syncthreads();
-    if (tid < a.hd) {
-        float v = 0.f, l = 0.f;
-        for (int u = 0; u < slices; ++u) { v += part_o[u][tid]; l += part_l[u]; }
-        a.out[(size_t) (row.start + r / group) * a.heads * a.hd + (size_t) (kvh * group + r % group) * a.hd + tid] = (f16) (l == 0.f ? 0.f : v / l);
+    if (sl || r >= row.fresh * group || d >= a.hd) return;
+    float top = m;
+    for (int u = 1; u < slices; ++u) top = fmaxf(top, slice_m[tid + u * lanes * each]);
+    const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    sum *= keep;
+    o *= keep;
+    for (int u = 1; u < slices; ++u) {
+        const int x = tid + u * lanes * each;
+        const float f = slice_m[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(slice_m[x] - top);
+        sum += f * slice_l[x];
+        o += f * slice_o[x];
     }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    f16x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (f16) (o[e] * inv);
+    *(f16x4*) (a.out + (size_t) (row.start + r / group) * a.heads * a.hd + (size_t) (kvh * group + r % group) * a.hd + d) = x;
 }
 
 // ---- rows of many queries: prompts and pieces of prompts --------------------------------------------------------------------------------
@@ -808,11 +838,12 @@ static PaPlan pa_plan(int n, int rows, int max_new, int heads, int kv_heads, int
     p.nt = queries <= 16 ? 1 : 2;
     p.rows_y = (int) queries;
     if (!p.many) {
-        p.cut = {kv_heads >= 1024 ? 1 : 1024 / kv_heads, PA_WAVES};
-        p.split = n <= PA_MAX_ROWS && longest > p.cut.min_piece * PA_KEYS;
-        p.items = p.parts = p.split ? p.cut.target + n : n;
+        const int waves = 1024 * (p.dp * p.nt <= 128 ? 2 : 1);     // of the whole machine
+        p.cut = {kv_heads >= waves ? 1 : waves / kv_heads, 2};
+        p.split = true;
+        p.items = p.parts = p.cut.target;
         p.item_bytes = pa_round((size_t) n * sizeof(int2));
-        p.part_bytes = p.split ? pa_round((size_t) p.parts * kv_heads * pa_part_floats(p.dp, p.nt) * sizeof(float)) : 0;
+        p.part_bytes = pa_round((size_t) p.parts * kv_heads * 2 * pa_part_floats(p.dp, p.nt) * sizeof(float));
     } else {
         const int64_t fresh = (int64_t) n * max_new < rows ? (int64_t) n * max_new : rows, tiles = (fresh * p.group + PM_ROWS - 1) / PM_ROWS + n;
         p.cut = {kv_heads >= 512 ? 1 : 512 / kv_heads, 8};
@@ -829,7 +860,8 @@ template <int CODE> static int pa_launch(const PagedAttn& a, const PaPlan& p, vo
 {
     float* parts = (float*) ((char*) workspace + p.item_bytes);
     EXL_REQUIRE((int64_t) p.items * a.kv_heads <= 0x7fffffff, EXL_E_UNSUPPORTED, "paged_attention: too many rows for %d kv heads", a.kv_heads);
-    const dim3 grid((unsigned) p.items * (unsigned) a.kv_heads);
+    const unsigned items = (unsigned) p.items * (unsigned) a.kv_heads;
+    const dim3 grid(p.many ? items : (items + PA_WAVES - 1) / PA_WAVES);
     if (!p.many) {
         int2* firsts = (int2*) workspace;
 #define PA_FEW(DP, NT) hipLaunchKernelGGL((paged_attn_few_kernel<CODE, DP, NT>), grid, dim3(PA_WAVES * 64), 0, s, a, p.cut, parts, firsts)
@@ -838,25 +870,26 @@ template <int CODE> static int pa_launch(const PagedAttn& a, const PaPlan& p, vo
         else                  PA_FEW(256, 1);
 #undef PA_FEW
         EXL_LAUNCH_CHECK();
-        if (p.split) {
-            hipLaunchKernelGGL(paged_attn_join_kernel, dim3((unsigned) a.n, (unsigned) p.rows_y, (unsigned) a.kv_heads), dim3(256), 0, s, a, parts, firsts, p.dp, p.nt);
-            EXL_LAUNCH_CHECK();
-        }
+        int each = 1;                                             // queries of a joining workgroup: as many as leave work for the whole machine
+        while (2 * each <= 1024 / p.dp && each < p.rows_y && (int64_t) a.n * a.kv_heads * ((p.rows_y + 2 * each - 1) / (2 * each)) >= 512) each *= 2;
+        hipLaunchKernelGGL(paged_attn_join_kernel, dim3((unsigned) a.n, (unsigned) ((p.rows_y + each - 1) / each), (unsigned) a.kv_heads), dim3(256), 0, s, a, parts, firsts,
+                           p.dp, p.nt, each);
+        EXL_LAUNCH_CHECK();
         return 0;
     }
-    PmItem* items = (PmItem*) workspace;
+    PmItem* list = (PmItem*) workspace;
 #define PA_MANY(DP, WIDE) do { static bool done[EXL_MAX_DEVICES] = {};                                                                       \
     EXL_TRY(exl_lds_opt_in((const void*) paged_attn_many_kernel<CODE, DP, WIDE>, done));                                                      \
-    hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE>), grid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4, s, a, p.cut, parts, items, p.parts); } while (0)
+    hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE>), grid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4, s, a, p.cut, parts, list, p.parts); } while (0)
     if (a.block >= PA_KEYS) { if (p.dp == 64) PA_MANY(64, true); else if (p.dp == 128) PA_MANY(128, true); else PA_MANY(256, true); }
     else                    { if (p.dp == 64) PA_MANY(64, false); else if (p.dp == 128) PA_MANY(128, false); else PA_MANY(256, false); }
 #undef PA_MANY
     EXL_LAUNCH_CHECK();
     if (p.split) {
         const dim3 jgrid((unsigned) p.parts, (unsigned) a.kv_heads, PM_ROWS / 32);
-        if (p.dp == 64)       hipLaunchKernelGGL((paged_attn_join_many_kernel<64>), jgrid, dim3(256), 0, s, a, parts, items);
-        else if (p.dp == 128) hipLaunchKernelGGL((paged_attn_join_many_kernel<128>), jgrid, dim3(256), 0, s, a, parts, items);
-        else                  hipLaunchKernelGGL((paged_attn_join_many_kernel<256>), jgrid, dim3(256), 0, s, a, parts, items);
+        if (p.dp == 64)       hipLaunchKernelGGL((paged_attn_join_many_kernel<64>), jgrid, dim3(256), 0, s, a, parts, list);
+        else if (p.dp == 128) hipLaunchKernelGGL((paged_attn_join_many_kernel<128>), jgrid, dim3(256), 0, s, a, parts, list);
+        else                  hipLaunchKernelGGL((paged_attn_join_many_kernel<256>), jgrid, dim3(256), 0, s, a, parts, list);
         EXL_LAUNCH_CHECK();
     }
     return 0;
