@@ -35,7 +35,7 @@ __device__ __forceinline__ PaRow pa_row(const PagedAttn& a, int b)
 //   O^T = V^T P^T : A = value columns, 16 bytes = keys 16 g .. 16 g + 15 of one column, as the page holds them; B = the lane's own 16 weights.
 #define PA_WAVES 4
 #define PA_KEYS 64
-#define PA_BEGIN 1
+#define PA_BEGIN 2
 
 // A page's scale as the conversions take it.  int8: 2^e is the exponent field of the fp16 numbers that a code's byte becomes the mantissa of:
 // (1024 + u) * 2^e with u = code + 128, minus 1152 * 2^e -- up to e = 5; beyond (`big`, for every lane as soon as one has it) a product follows.
@@ -135,43 +135,50 @@ __device__ __forceinline__ PaRow pa_row_of_wave(const PagedAttn& a, int b)
     return r;
 }
 
-// Stretch `w` of the line: `count` places from place `from` of row `row` on, the first of them number `at` of the line; `share`: places of a stretch
-struct PaStretch { int row, from, count, share; int64_t at; };
+// Stretch `w` of the line: `count` places from place `from` of row `row` on, the first of them number `at` of the line; `share`: places of a stretch.
+// (The host has made sure that the line has less than 2^30 places.)
+struct PaStretch { int row, from, count, share, at; };
 __device__ __forceinline__ PaStretch pa_stretch(const PagedAttn& a, const PaCut& cut, int w)
 {
+    constexpr int KEPT = 4;                                        // rows of the batch whose places stay in registers: 64 * KEPT
     const int lane = threadIdx.x & 63;
     auto places = [&](int b) { const int keys = b < a.n ? pa_row(a, b).keys : 0; return keys ? (keys + PA_KEYS - 1) / PA_KEYS + PA_BEGIN : 0; };
-    const int mine = places(lane);                                 // (of the first 64 rows, kept)
-    int64_t total = mine;
-    for (int b = lane + 64; b < a.n; b += 64) total += places(b);
-    if (a.n == 1) total = __builtin_amdgcn_readfirstlane(mine);
+    int kept[KEPT], total = 0;
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) {
+        kept[i] = 0;
+        if (64 * i < a.n) kept[i] = places(lane + 64 * i);
+        total += kept[i];
+    }
+    for (int b = lane + 64 * KEPT; b < a.n; b += 64) total += places(b);
+    if (a.n == 1) total = __builtin_amdgcn_readfirstlane(total);
     else {
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
     }
     PaStretch st = {-1, 0, 0, 0, 0};
-    const int64_t even = (total + cut.target - 1) / cut.target;
-    st.share = (int) (even > cut.min_piece ? even : cut.min_piece);
-    st.at = (int64_t) w * st.share;
-    if (st.at >= total) return st;
-    st.count = (int) min((int64_t) st.share, total - st.at);
-    if (a.n == 1) { st.row = 0; st.from = (int) st.at; return st; }
-    int64_t before = 0;
-    for (int b0 = 0; b0 < a.n; b0 += 64) {
-        const int t = b0 == 0 ? mine : places(b0 + lane);
-        int64_t inc = t;
+    st.share = max((total + cut.target - 1) / cut.target, cut.min_piece);
+    if ((int64_t) w * st.share >= total) return st;
+    st.at = w * st.share;
+    st.count = min(st.share, total - st.at);
+    if (a.n == 1) { st.row = 0; st.from = st.at; return st; }
+    int before = 0;
+    auto look = [&](int b0, int t) {                               // 64 rows; true: found
+        int inc = t;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) { const int64_t o = __shfl_up(inc, off, 64); if (lane >= off) inc += o; }
-        const int64_t from = before + inc - t;
+        for (int off = 1; off < 64; off <<= 1) { const int o = __shfl_up(inc, off, 64); if (lane >= off) inc += o; }
+        const int from = before + inc - t;
         const uint64_t hit = __ballot(st.at >= from && st.at < from + t);
-        if (hit) {
-            const int l = __ffsll((unsigned long long) hit) - 1;
-            st.row = b0 + l;
-            st.from = __builtin_amdgcn_readlane((int) (st.at - from), l);
-            return st;
-        }
-        before += __shfl(inc, 63, 64);
-    }
+        before += __builtin_amdgcn_readlane(inc, 63);
+        if (!hit) return false;
+        const int l = __ffsll((unsigned long long) hit) - 1;
+        st.row = b0 + l;
+        st.from = __builtin_amdgcn_readlane(st.at - from, l);
+        return true;
+    };
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) if (64 * i < a.n && look(64 * i, kept[i])) return st;
+    for (int b0 = 64 * KEPT; b0 < a.n; b0 += 64) if (look(b0, places(b0 + lane))) return st;
     return st;
 }
 
@@ -350,7 +357,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
     };
 
     int b = to.row, from = to.from, left = to.count;              // the row, the first place of it that is this stretch's, places that are left
-    int64_t at = to.at - to.from;                                 // the row's first place in the line
+    int at = to.at - to.from;                                     // the row's first place in the line
     if (from + left <= PA_BEGIN) return;                          // (no tile)
     Stage st;
     fetch(max(from - PA_BEGIN, 0), a.table + (size_t) b * a.width, st);
@@ -375,7 +382,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
         float* part = parts + (((size_t) w * a.kv_heads + kvh) * 2 + (first == 0)) * pa_part_floats(DP, NT);
         end(whole ? nullptr : part);
         if (first == 0 && kvh == 0 && lane == 0)                  // for the joining kernel: where the row's parts begin, and how many there are
-            firsts[b] = make_int2(w, (int) ((at + PA_BEGIN + tiles - 1) / to.share) - w + 1);
+            firsts[b] = make_int2(w, (at + PA_BEGIN + tiles - 1) / to.share - w + 1);
         if (nb == b) return;
         at += tiles + PA_BEGIN;
         b = nb;
@@ -922,6 +929,8 @@ extern "C" int exl_paged_attention(const void* q, long q_stride, const int32_t* 
                 "paged_attention: q rows must be 8-byte aligned and at least heads * head_dim apart");
     EXL_REQUIRE(((uintptr_t) key_pages | (uintptr_t) value_pages) % 16 == 0, EXL_E_INVALID, "paged_attention: pages must be 16-byte aligned");
     EXL_REQUIRE((int64_t) table_width * block_size <= 0x7fffffff, EXL_E_UNSUPPORTED, "paged_attention: the block table exceeds 2^31 tokens");
+    EXL_REQUIRE((int64_t) n_rows * ((int64_t) table_width * block_size / PA_KEYS + PA_BEGIN + 1) < 1 << 30, EXL_E_UNSUPPORTED,
+                "paged_attention: %d rows of %d blocks are too many", n_rows, table_width);
     if (rows == 0 || max_new == 0) return 0;
     PagedAttn a = {(const f16*) q, starts, past_lens, new_lens, block_table, (const uint8_t*) key_pages, (const uint8_t*) value_pages, key_scales,
                    value_scales, (const f16*) sin, (const f16*) cos, (f16*) out, n_rows, rows, max_new, table_width, num_blocks, block_size, num_heads,
