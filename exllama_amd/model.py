@@ -394,6 +394,19 @@ class ExLlamaAttention:
             hidden.add_(cfg.tp.all_reduce(self.o_proj.forward(attn, lora)))
 
 
+    def forward_paged(self, normed, hidden, cache, lora):
+        """The general path over an ExLlamaPagedCache: hidden += o_proj(attention over the pages), keys rotated and quantised by the append, queries
+        rotated by the attention kernel (each row of the batch at its own position)."""
+        cfg = self.config
+        q, k, v = (p.forward(normed, lora).view(-1, p.out_features) for p in (self.q_proj, self.k_proj, self.v_proj))
+        step, pages = cache.step[str(hidden.device)], cache.pages[self.index]
+        cuda_ext.ext_paged_append(k, v, step.slots, *pages, positions=step.positions, sin=self.sin, cos=self.cos)
+        attn = torch.zeros_like(q) if step.padded else torch.empty_like(q)            # (rows of padding are not written)
+        cuda_ext.ext_paged_attention(q, step.starts, step.past, step.new, step.table, *pages, cfg.num_attention_heads, max_new=step.max_new, sin=self.sin,
+                                     cos=self.cos, out=attn)
+        self.o_proj.forward(attn.view(hidden.shape[:-1] + (attn.shape[-1],)), lora, out=hidden, accumulate=True)
+
+
 def _rows(x):
     n = 1
     for d in x.shape[:-1]:
@@ -419,6 +432,14 @@ class ExLlamaDecoderLayer:
             self.self_attn.forward_residual(normed, hidden_states, cache, buffer, lora)
             normed = self.post_attention_layernorm.forward(hidden_states, buffer)
             self.mlp.forward_residual(normed, hidden_states, lora)
+            return hidden_states
+        self.took_layer_call = False
+        if isinstance(cache, ExLlamaPagedCache):
+            self.self_attn.forward_paged(self.input_layernorm.forward(hidden_states, buffer), hidden_states, cache, lora)
+            if cfg.fused_mlp_thd > 0 and rows <= cfg.fused_mlp_thd:
+                self.mlp.fused(hidden_states, buffer, self.post_attention_layernorm, lora)
+            else:
+                self.mlp.forward_residual(None, hidden_states, lora, norm=self.post_attention_layernorm)
             return hidden_states
         self.took_layer_call = 2 <= rows <= 256 and self._short_prompt(hidden_states, cache, buffer, lora)
         if self.took_layer_call:
@@ -515,6 +536,112 @@ class ExLlamaCache:
                 src = src_t.narrow(0, from_row, from_rows).narrow(2, from_column, from_columns)
                 dst = dst_t.narrow(0, to_row, to_rows).narrow(2, to_column, to_columns)
                 dst.copy_(src.expand_as(dst) if to_rows > 1 else src)
+
+
+class ExLlamaPagedCache:
+    """K/V cache in 8-bit pages, with a length of its own for every row of the batch (no counterpart in the reference).
+
+    Pages of `block_size` tokens (16, 32, 64 or 128) come from one pool of `num_blocks` (default: enough for every row to reach max_seq_len; fewer
+    serve rows that are not all long at once) and hold e4m3 or int8 codes with one power-of-two scale for each page and head: half the
+    memory of ExLlamaCache for the same tokens.  `ExLlama.forward(ids, cache, row_lens=[...])` takes right-padded rows; `release(row)`
+    gives a row's pages back.  `seq_lens` are the rows' lengths; `current_seq_len` is the longest of them, and setting it sets all rows."""
+
+    class _Step:
+        """What one forward pass needs on one device: token rows' starts, slots and positions (ext_paged_slots), lengths and table."""
+        __slots__ = ("starts", "slots", "positions", "past", "new", "table", "max_new", "padded")
+
+    def __init__(self, model, batch_size=1, max_seq_len=-1, block_size=64, num_blocks=None, dtype=torch.float8_e4m3fn):
+        cfg = model.config
+        if cfg.tp is not None:
+            raise RuntimeError("ExLlamaPagedCache: tensor-parallel shards are not supported")
+        if dtype not in cuda_ext.PAGE_CODES:
+            raise RuntimeError("ExLlamaPagedCache: dtype must be torch.float8_e4m3fn or torch.int8")
+        self.model, self.config, self.batch_size, self.block_size, self.dtype = model, cfg, batch_size, block_size, dtype
+        self.max_seq_len = max_seq_len if max_seq_len != -1 else cfg.max_seq_len
+        if self.max_seq_len > cfg.max_seq_len:
+            raise RuntimeError("ExLlamaPagedCache: cache is longer than the RoPE tables (config.max_seq_len)")
+        self.width = -(-self.max_seq_len // block_size)
+        self.num_blocks = batch_size * self.width if num_blocks is None else num_blocks
+        self.seq_lens = [0] * batch_size
+        self._held, self._free = [0] * batch_size, self.num_blocks      # the device's bookkeeping, as the host knows it: what cannot be held is refused
+        hd16 = (cfg.head_dim + 15) // 16 * 16
+        self.pages = []                                                  # per layer: key_pages, value_pages, key_scales, value_scales
+        for i in range(cfg.num_hidden_layers):
+            dev, shape = cfg.device_map.layers[i], (self.num_blocks, cfg.num_key_value_heads)
+            self.pages.append((torch.zeros(shape + (block_size, hd16), dtype=torch.uint8, device=dev).view(dtype),
+                               torch.zeros(shape + (hd16, block_size), dtype=torch.uint8, device=dev).view(dtype),
+                               torch.ones(shape, dtype=torch.float32, device=dev), torch.ones(shape, dtype=torch.float32, device=dev)))
+        self._dev = {}
+        for dev in sorted({str(torch.device(d)) for d in cfg.device_map.layers}):
+            ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+            self._dev[dev] = {"past": torch.zeros(batch_size, dtype=torch.int32, device=dev), "held": torch.zeros(batch_size, dtype=torch.int32, device=dev),
+                              "table": torch.full((batch_size, self.width), -1, dtype=torch.int32, device=dev),
+                              "ring": torch.arange(self.num_blocks, dtype=torch.int32, device=dev), "counters": ints(0, self.num_blocks, 0, 0)}
+        self.step = {}
+
+    @property
+    def current_seq_len(self):
+        return max(self.seq_lens)
+
+    @current_seq_len.setter
+    def current_seq_len(self, length):
+        """Every row to `length` tokens (0: start anew; shorter than now: the tokens behind are dropped).  The rows keep their pages."""
+        if any(length > n for n in self.seq_lens):
+            raise RuntimeError("ExLlamaPagedCache: a row cannot be longer than the tokens it has been given")
+        self.set_seq_lens([length] * self.batch_size)
+
+    def set_seq_lens(self, lengths):
+        """Rows to the given lengths, none longer than it is."""
+        if len(lengths) != self.batch_size or any(not 0 <= n <= m for n, m in zip(lengths, self.seq_lens)):
+            raise RuntimeError("ExLlamaPagedCache: one length for each row, none longer than the tokens the row has been given")
+        self.seq_lens = [int(n) for n in lengths]
+        for d in self._dev.values():
+            d["past"].copy_(torch.tensor(self.seq_lens, dtype=torch.int32))
+
+    def begin(self, new_lens, q_len):
+        """Blocks, slots and positions of a pass that brings new_lens[b] tokens to row b, token rows b * q_len ..; used by ExLlama.forward."""
+        new_lens = [int(n) for n in new_lens]
+        if len(new_lens) != self.batch_size or any(not 0 <= n <= q_len for n in new_lens):
+            raise RuntimeError(f"row_lens must give each of the {self.batch_size} rows 0 .. {q_len} tokens")
+        need = []
+        for past, n, held in zip(self.seq_lens, new_lens, self._held):
+            if past + n > self.max_seq_len:
+                raise RuntimeError(f"sequence ({past} + {n}) exceeds the cache length {self.max_seq_len}")
+            need.append(max(held, -(-(past + n) // self.block_size)))
+        if sum(need) - sum(self._held) > self._free:
+            raise RuntimeError(f"ExLlamaPagedCache: {sum(need) - sum(self._held)} more blocks are needed, {self._free} of {self.num_blocks} are free: release rows")
+        self._free -= sum(need) - sum(self._held)
+        self._held = need
+        for dev, d in self._dev.items():
+            st = self._Step()
+            st.new = torch.tensor(new_lens, dtype=torch.int32).to(dev)
+            st.past, st.table, st.max_new, st.padded = d["past"], d["table"], max(max(new_lens), 1), min(new_lens) < q_len
+            st.starts, st.slots, st.positions = cuda_ext.ext_paged_slots(d["past"], st.new, d["held"], d["table"], d["ring"], d["counters"], self.block_size,
+                                                                         self.batch_size * q_len, max_new=q_len, max_len=self.max_seq_len, row_stride=q_len)
+            self.step[dev] = st
+
+    def end(self, new_lens):
+        """The pass that begin() prepared has been enqueued: its tokens belong to the rows."""
+        self.seq_lens = [n + int(m) for n, m in zip(self.seq_lens, new_lens)]
+        for dev, d in self._dev.items():
+            d["past"].add_(self.step[dev].new)
+        self.step = {}
+
+    def release(self, *rows):
+        """The rows have ended: their pages go back to the pool, their lengths to 0."""
+        if any(not 0 <= b < self.batch_size for b in rows):
+            raise RuntimeError("ExLlamaPagedCache: no such row")
+        gone = [-1 if b in rows else 0 for b in range(self.batch_size)]
+        for dev, d in self._dev.items():
+            cuda_ext.ext_paged_slots(d["past"], torch.tensor(gone, dtype=torch.int32).to(dev), d["held"], d["table"], d["ring"], d["counters"], self.block_size, 0)
+        for b in set(rows):
+            self._free += self._held[b]
+            self._held[b] = 0
+        self.set_seq_lens([0 if g else n for g, n in zip(gone, self.seq_lens)])
+
+    def zero(self):
+        """Every row empty, every page back in the pool."""
+        self.release(*range(self.batch_size))
 
 
 class ExLlamaBuffer:
@@ -704,9 +831,15 @@ class ExLlama:
 
     # ---- forward -------------------------------------------------------------------------------------------
     def forward(self, input_ids, cache, last_id_only=True, preprocess_only=False, lora=None, output_device=None,
-                input_mask=None):
+                input_mask=None, row_lens=None):
         """Same contract as the reference (model.py:924-986): chunks long inputs by max_input_len, returns
-        fp32 logits [bsz, 1 or q_len, vocab] on `output_device` (default: input_ids' device), or None."""
+        fp32 logits [bsz, 1 or q_len, vocab] on `output_device` (default: input_ids' device), or None.
+        `row_lens` (an ExLlamaPagedCache only; default: q_len for every row): the tokens of each right-padded row that count, 0 for a row that
+        sits this pass out.  With last_id_only the logits are those of each row's last token (a row of none: its first padding's)."""
+        if isinstance(cache, ExLlamaPagedCache):
+            return self._forward_paged(input_ids, cache, last_id_only, preprocess_only, lora, output_device, input_mask, row_lens)
+        if row_lens is not None:
+            raise RuntimeError("row_lens needs an ExLlamaPagedCache")
         q_len = input_ids.shape[-1]
         bsz = input_ids.shape[0]
         if lora is not None and self.config.tp is not None:
@@ -769,6 +902,43 @@ class ExLlama:
         if preprocess_only:
             return None
         return _move_tensor(self.head(hidden, last_id_only), output_device, "logits", cfg)
+
+    @torch.no_grad()
+    def _forward_paged(self, input_ids, cache, last_id_only, preprocess_only, lora, output_device, input_mask, row_lens):
+        cfg = self.config
+        bsz, q_len = input_ids.shape
+        if input_mask is not None:
+            raise RuntimeError("an ExLlamaPagedCache takes row_lens instead of an input_mask")
+        if bsz != cache.batch_size:
+            raise RuntimeError(f"input_ids has {bsz} rows, the cache {cache.batch_size}")
+        row_lens = [q_len] * bsz if row_lens is None else [int(n) for n in row_lens]
+        if len(row_lens) != bsz or any(not 0 <= n <= q_len for n in row_lens):
+            raise RuntimeError(f"row_lens must give each of the {bsz} rows 0 .. {q_len} tokens")
+        if output_device is None:
+            output_device = input_ids.device
+        chunk_cap = max(1, cfg.max_input_len // bsz)
+        result = None
+        for begin in range(0, q_len, chunk_cap):
+            end = min(begin + chunk_cap, q_len)
+            new = [min(max(n - begin, 0), end - begin) for n in row_lens]
+            cache.begin(new, end - begin)
+            hidden = self.forward_layers(self.embed(input_ids[:, begin:end]), cache, None, lora)
+            cache.end(new)
+            self._count_path("ops_general")
+            if preprocess_only:
+                continue
+            if not last_id_only:
+                logits = self.head(hidden, False)
+                result = logits if result is None else torch.cat((result, logits), dim=1)
+                continue
+            here = [b for b in range(bsz) if begin < row_lens[b] <= end or (row_lens[b] == 0 and begin == 0)]      # rows whose last token lies in this chunk
+            if here:
+                at = torch.tensor([max(row_lens[b] - 1 - begin, 0) for b in here], device=hidden.device)
+                logits = self.head(hidden[torch.tensor(here, device=hidden.device), at].unsqueeze(1), False)
+                if result is None:
+                    result = torch.empty((bsz,) + logits.shape[1:], dtype=logits.dtype, device=logits.device)
+                result[torch.tensor(here, device=logits.device)] = logits
+        return None if result is None else _move_tensor(result, output_device, "logits", cfg)
 
     # The three stages of a forward pass, also used one stage per process by exllama_amd/pipeline.py (layer split
     # across processes: rank 0 embeds, every rank runs its own layers, the last rank applies norm + lm_head).
@@ -959,6 +1129,8 @@ class ExLlama:
         enable_decode_graph(lora=...) stays on the op-by-op path as before."""
         import ctypes as C
         cfg = self.config
+        if isinstance(cache, ExLlamaPagedCache):
+            raise RuntimeError("the native decode executor keeps an fp16 ExLlamaCache")
         if cache.batch_size != 1:
             raise RuntimeError("the native decode executor handles batch size 1")
         if cache.max_seq_len > cfg.max_seq_len:
