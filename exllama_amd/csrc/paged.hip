@@ -11,19 +11,21 @@
 // Then every token row's slot = table[pos / block] * block + pos % block.  Latency is all that matters (a step of 256 rows moves
 // 7 KB): one workgroup does both halves where the work is small, otherwise the scan runs in one workgroup and the filling in
 // many -- a second launch instead of a grid-wide wait.
-struct SlotRow { int start, take, past, kept, held, base, back, gone; };      // 32 bytes a row, in the caller's scratch
+struct SlotRow { int start, take, past, kept, held, base, back, gone; };      // 32 bytes a row
 
 struct SlotArgs {
     const int32_t* past; const int32_t* fresh; int32_t* held; int32_t* table; int32_t* ring; int32_t* counters;
-    int n, width, block, blocks, max_len, max_new, rows, row_stride;
-    int32_t* starts; int32_t* slots; int32_t* positions; SlotRow* desc;
+    int n, width, lbs, blocks, max_len, max_new, rows, row_stride;               // lbs: log2 of the block size
+    int32_t* starts; int32_t* slots; int32_t* positions;
 };
 
 #define SLOT_THREADS 1024
 #define SLOT_WAVES (SLOT_THREADS / 64)
+#define SLOT_SMALL_ROWS 1024                                      // rows and token rows up to which one workgroup does it all
+#define SLOT_SMALL_TOKENS 4096
 
-// exclusive prefix sum over the workgroup, and the total; `lds`: SLOT_WAVES + 1 entries of its own
-__device__ __forceinline__ int64_t slot_scan(int64_t v, int64_t* lds, int64_t& total)
+// exclusive prefix sum over the workgroup, and the total; `lds`: SLOT_WAVES entries.  Up to 64 rows only the first wave has numbers: no barrier.
+__device__ __forceinline__ int64_t slot_scan(int64_t v, int64_t* lds, bool one_wave, int64_t& total)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int64_t inc = v;
@@ -32,23 +34,27 @@ __device__ __forceinline__ int64_t slot_scan(int64_t v, int64_t* lds, int64_t& t
         const int64_t o = __shfl_up(inc, off, 64);
         if (lane >= off) inc += o;
     }
+    total = __shfl(inc, 63, 64);
+    if (one_wave) return inc - v;
+    __syncthreads();                                              // (the last sums have been read)
     if (lane == 63) lds[wave] = inc;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int64_t run = 0;
-        for (int w = 0; w < SLOT_WAVES; ++w) { const int64_t s = lds[w]; lds[w] = run; run += s; }
-        lds[SLOT_WAVES] = run;
+    int64_t before = lds[lane & (SLOT_WAVES - 1)];                // every wave scans the waves' sums for itself
+#pragma unroll
+    for (int off = 1; off < SLOT_WAVES; off <<= 1) {
+        const int64_t o = __shfl_up(before, off, SLOT_WAVES);
+        if ((lane & (SLOT_WAVES - 1)) >= off) before += o;
     }
-    __syncthreads();
-    const int64_t r = inc - v + lds[wave];
-    total = lds[SLOT_WAVES];
-    __syncthreads();
-    return r;
+    total = __shfl(before, SLOT_WAVES - 1, 64);
+    const int64_t mine = __shfl(before, wave ? wave - 1 : 0, 64);
+    return inc - v + (wave ? mine : 0);
 }
 
-__device__ __forceinline__ void slot_scan_rows(const SlotArgs& a)
+__device__ __forceinline__ void slot_scan_rows(const SlotArgs& a, SlotRow* desc)
 {
-    __shared__ int64_t lds[SLOT_WAVES + 1];
+    __shared__ int64_t lds[SLOT_WAVES];
+    const bool one_wave = a.n <= 64;
+    if (one_wave && threadIdx.x >= 64) return;
     const int head = (int) ((uint32_t) a.counters[0] % (uint32_t) a.blocks);
     const int avail = min(max(a.counters[1], 0), a.blocks);
     int64_t rows_before = 0, want_before = 0, back_before = 0;
@@ -61,23 +67,21 @@ __device__ __forceinline__ void slot_scan_rows(const SlotArgs& a)
         int take = min(max(fresh, 0), a.max_new), start = 0;
         int64_t total;
         if (a.row_stride > 0) {
-            const int64_t s = (int64_t) b * a.row_stride;
-            start = (int) min(s, (int64_t) a.rows);
+            start = (int) min((int64_t) b * a.row_stride, (int64_t) a.rows);
             take = min(min(take, a.row_stride), a.rows - start);
         } else {
-            const int64_t s = rows_before + slot_scan(take, lds, total);
+            const int64_t s = rows_before + slot_scan(take, lds, one_wave, total);
             rows_before += total;
             start = (int) min(s, (int64_t) a.rows);
             take = min(take, a.rows - start);
         }
         const bool gone = fresh < 0;
         const int end = (int) min((int64_t) past + take, (int64_t) a.max_len);
-        const int want = in && !gone ? max(0, (end + a.block - 1) / a.block - held) : 0;
-        const int64_t base = want_before + slot_scan(want, lds, total);
-        want_before += total;
-        const int back = gone ? held : 0;
-        const int64_t back_base = back_before + slot_scan(back, lds, total);
-        back_before += total;
+        const int want = in && !gone ? max(0, (int) (((int64_t) end + (1 << a.lbs) - 1) >> a.lbs) - held) : 0, back = gone ? held : 0;
+        const int64_t both = slot_scan((int64_t) want << 32 | back, lds, one_wave, total);      // (both sums are less than the table's entries: 2^31)
+        const int64_t base = want_before + (both >> 32), back_base = back_before + (both & 0xffffffff);
+        want_before += total >> 32;
+        back_before += total & 0xffffffff;
         if (in) {
             const int got = (int) min(max((int64_t) avail - base, (int64_t) 0), (int64_t) want);
             SlotRow r;
@@ -86,12 +90,12 @@ __device__ __forceinline__ void slot_scan_rows(const SlotArgs& a)
             r.base = (int) ((head + base) % a.blocks);
             r.back = (int) ((head + avail + back_base) % a.blocks);
             r.gone = gone;
-            a.desc[b] = r;
+            desc[b] = r;
             a.starts[b] = start;
             a.held[b] = r.kept;
         }
     }
-    __syncthreads();                                          // every thread has read the counters
+    if (!one_wave) __syncthreads();                               // every thread has read the counters
     if (threadIdx.x == 0) {
         const int got = (int) min(want_before, (int64_t) avail);
         a.counters[0] = (head + got) % a.blocks;
@@ -105,11 +109,11 @@ __device__ __forceinline__ void slot_scan_rows(const SlotArgs& a)
 __device__ __forceinline__ int slot_ring(const SlotArgs& a, int at) { return a.ring[at >= a.blocks ? at - a.blocks : at]; }
 
 // the table and the ring of rows first, first + step, ... (a wave each)
-__device__ __forceinline__ void slot_fill_rows(const SlotArgs& a, int first, int step)
+__device__ __forceinline__ void slot_fill_rows(const SlotArgs& a, const SlotRow* desc, int first, int step)
 {
     const int lane = threadIdx.x & 63;
     for (int b = first; b < a.n; b += step) {
-        const SlotRow r = a.desc[b];
+        const SlotRow r = desc[b];
         int32_t* row = a.table + (size_t) b * a.width;
         if (r.gone) {
             for (int i = lane; i < r.held; i += 64) {
@@ -124,22 +128,22 @@ __device__ __forceinline__ void slot_fill_rows(const SlotArgs& a, int first, int
 }
 
 // the slots and positions of token rows first, first + step, ...
-__device__ __forceinline__ void slot_fill_tokens(const SlotArgs& a, int first, int step)
+__device__ __forceinline__ void slot_fill_tokens(const SlotArgs& a, const SlotRow* desc, int first, int step)
 {
     for (int t = first; t < a.rows; t += step) {
         int lo = 0, hi = a.n;                                 // the last row that starts at or before t (rows of no token share a start: the last one)
         if (a.row_stride > 0) lo = min(t / a.row_stride, a.n - 1);
-        else while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (a.desc[mid].start <= t) lo = mid; else hi = mid; }
-        const SlotRow r = a.desc[lo];
+        else while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (desc[mid].start <= t) lo = mid; else hi = mid; }
+        const SlotRow r = desc[lo];
         const int i = t - r.start;
         int slot = -1, pos = 0;
         if (i < r.take) {
             pos = (int) min((int64_t) r.past + i, (int64_t) 0x7fffffff);
-            const int k = pos / a.block;
+            const int k = pos >> a.lbs;
             if (pos < a.max_len && k < r.kept) {
                 // (entries that this call adds are still being written by other waves: they are read where they come from)
                 const int id = k < r.held ? a.table[(size_t) lo * a.width + k] : slot_ring(a, r.base + k - r.held);
-                if (id >= 0 && id < a.blocks) slot = id * a.block + pos % a.block;
+                if (id >= 0 && id < a.blocks) slot = (id << a.lbs) + (pos & ((1 << a.lbs) - 1));
             }
         }
         a.slots[t] = slot;
@@ -149,18 +153,19 @@ __device__ __forceinline__ void slot_fill_tokens(const SlotArgs& a, int first, i
 
 __global__ __launch_bounds__(SLOT_THREADS) void paged_slots_small_kernel(SlotArgs a)
 {
-    slot_scan_rows(a);
-    __syncthreads();                                          // desc, of this workgroup alone
-    slot_fill_tokens(a, threadIdx.x, SLOT_THREADS);
-    slot_fill_rows(a, threadIdx.x >> 6, SLOT_WAVES);
+    __shared__ SlotRow desc[SLOT_SMALL_ROWS];
+    slot_scan_rows(a, desc);
+    __syncthreads();
+    slot_fill_tokens(a, desc, threadIdx.x, SLOT_THREADS);
+    slot_fill_rows(a, desc, threadIdx.x >> 6, SLOT_WAVES);
 }
 
-__global__ __launch_bounds__(SLOT_THREADS) void paged_slots_scan_kernel(SlotArgs a) { slot_scan_rows(a); }
+__global__ __launch_bounds__(SLOT_THREADS) void paged_slots_scan_kernel(SlotArgs a, SlotRow* desc) { slot_scan_rows(a, desc); }
 
-__global__ __launch_bounds__(256) void paged_slots_fill_kernel(SlotArgs a, int token_groups)
+__global__ __launch_bounds__(256) void paged_slots_fill_kernel(SlotArgs a, const SlotRow* desc, int token_groups)
 {
-    if ((int) blockIdx.x < token_groups) slot_fill_tokens(a, blockIdx.x * 256 + threadIdx.x, token_groups * 256);
-    else slot_fill_rows(a, (blockIdx.x - token_groups) * 4 + (threadIdx.x >> 6), (gridDim.x - token_groups) * 4);
+    if ((int) blockIdx.x < token_groups) slot_fill_tokens(a, desc, blockIdx.x * 256 + threadIdx.x, token_groups * 256);
+    else slot_fill_rows(a, desc, (blockIdx.x - token_groups) * 4 + (threadIdx.x >> 6), (gridDim.x - token_groups) * 4);
 }
 
 extern "C" int exl_paged_slots(const int32_t* past_lens, const int32_t* new_lens, int32_t* held, int32_t* block_table, int32_t* ring,
@@ -174,16 +179,17 @@ extern "C" int exl_paged_slots(const int32_t* past_lens, const int32_t* new_lens
     EXL_TRY(paged_check_block("paged_slots", block_size, num_blocks));
     EXL_REQUIRE((int64_t) max_len <= (int64_t) table_width * block_size, EXL_E_INVALID, "paged_slots: max_len (%d) exceeds the block table (%d blocks of %d)",
                 max_len, table_width, block_size);
-    SlotArgs a = {past_lens, new_lens, held, block_table, ring, counters, n_rows, table_width, block_size, num_blocks, max_len, max_new, rows,
-                  row_stride, starts, slots, positions, (SlotRow*) scratch};
+    EXL_REQUIRE((int64_t) n_rows * table_width < 0x7fffffff, EXL_E_UNSUPPORTED, "paged_slots: the block table exceeds 2^31 entries");
+    SlotArgs a = {past_lens, new_lens, held, block_table, ring, counters, n_rows, table_width, 31 - __builtin_clz((unsigned) block_size), num_blocks, max_len,
+                  max_new, rows, row_stride, starts, slots, positions};
     hipStream_t s = (hipStream_t) stream;
-    if (rows <= 4096 && n_rows <= 1024) {
+    if (rows <= SLOT_SMALL_TOKENS && n_rows <= SLOT_SMALL_ROWS) {
         hipLaunchKernelGGL(paged_slots_small_kernel, dim3(1), dim3(SLOT_THREADS), 0, s, a);
     } else {
-        hipLaunchKernelGGL(paged_slots_scan_kernel, dim3(1), dim3(SLOT_THREADS), 0, s, a);
+        hipLaunchKernelGGL(paged_slots_scan_kernel, dim3(1), dim3(SLOT_THREADS), 0, s, a, (SlotRow*) scratch);
         EXL_LAUNCH_CHECK();
         const int tg = (int) ((rows + 255L) / 256 < 2048 ? (rows + 255L) / 256 : 2048), rg = (n_rows + 3) / 4 < 2048 ? (n_rows + 3) / 4 : 2048;
-        hipLaunchKernelGGL(paged_slots_fill_kernel, dim3(tg + rg), dim3(256), 0, s, a, tg);
+        hipLaunchKernelGGL(paged_slots_fill_kernel, dim3(tg + rg), dim3(256), 0, s, a, (const SlotRow*) scratch, tg);
     }
     EXL_LAUNCH_CHECK();
     return 0;
