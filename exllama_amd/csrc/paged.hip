@@ -50,49 +50,73 @@ __device__ __forceinline__ int64_t slot_scan(int64_t v, int64_t* lds, bool one_w
     return inc - v + (wave ? mine : 0);
 }
 
-__device__ __forceinline__ void slot_scan_rows(const SlotArgs& a, SlotRow* desc)
+// R consecutive rows for a thread
+template <int R> __device__ __forceinline__ void slot_scan_rows(const SlotArgs& a, SlotRow* desc)
 {
     __shared__ int64_t lds[SLOT_WAVES];
-    const bool one_wave = a.n <= 64;
+    const bool one_wave = a.n <= 64 * R;
     if (one_wave && threadIdx.x >= 64) return;
     const int head = (int) ((uint32_t) a.counters[0] % (uint32_t) a.blocks);
     const int avail = min(max(a.counters[1], 0), a.blocks);
     int64_t rows_before = 0, want_before = 0, back_before = 0;
-    for (int b0 = 0; b0 < a.n; b0 += SLOT_THREADS) {
-        const int b = b0 + threadIdx.x;
-        const bool in = b < a.n;
-        const int fresh = in ? a.fresh[b] : 0;
-        const int held = in ? min(max(a.held[b], 0), a.width) : 0;
-        const int past = in ? max(a.past[b], 0) : 0;
-        int take = min(max(fresh, 0), a.max_new), start = 0;
-        int64_t total;
-        if (a.row_stride > 0) {
-            start = (int) min((int64_t) b * a.row_stride, (int64_t) a.rows);
-            take = min(min(take, a.row_stride), a.rows - start);
-        } else {
-            const int64_t s = rows_before + slot_scan(take, lds, one_wave, total);
-            rows_before += total;
-            start = (int) min(s, (int64_t) a.rows);
-            take = min(take, a.rows - start);
+    for (int b0 = 0; b0 < a.n; b0 += SLOT_THREADS * R) {
+        const int first = b0 + threadIdx.x * R;
+        int fresh[R], held[R], past[R], take[R], start[R], want[R], back[R];
+        int64_t mine = 0, total;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const bool in = first + i < a.n;
+            fresh[i] = in ? a.fresh[first + i] : 0;
+            held[i] = in ? a.held[first + i] : 0;
+            past[i] = in ? a.past[first + i] : 0;
         }
-        const bool gone = fresh < 0;
-        const int end = (int) min((int64_t) past + take, (int64_t) a.max_len);
-        const int want = in && !gone ? max(0, (int) (((int64_t) end + (1 << a.lbs) - 1) >> a.lbs) - held) : 0, back = gone ? held : 0;
-        const int64_t both = slot_scan((int64_t) want << 32 | back, lds, one_wave, total);      // (both sums are less than the table's entries: 2^31)
-        const int64_t base = want_before + (both >> 32), back_base = back_before + (both & 0xffffffff);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            held[i] = min(max(held[i], 0), a.width);
+            past[i] = max(past[i], 0);
+            take[i] = min(max(fresh[i], 0), a.max_new);
+            mine += take[i];
+        }
+        int64_t at = 0;
+        if (a.row_stride <= 0) {
+            at = rows_before + slot_scan(mine, lds, one_wave, total);
+            rows_before += total;
+        }
+        mine = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (a.row_stride > 0) {
+                at = (int64_t) (first + i) * a.row_stride;
+                take[i] = min(take[i], a.row_stride);
+            }
+            start[i] = (int) min(at, (int64_t) a.rows);
+            at += take[i];
+            take[i] = min(take[i], a.rows - start[i]);
+            const int end = (int) min((int64_t) past[i] + take[i], (int64_t) a.max_len);
+            const int need = (int) (((int64_t) end + (1 << a.lbs) - 1) >> a.lbs);
+            want[i] = first + i < a.n && fresh[i] >= 0 ? max(0, need - held[i]) : 0;
+            back[i] = fresh[i] < 0 ? held[i] : 0;
+            mine += (int64_t) want[i] << 32 | back[i];
+        }
+        const int64_t both = slot_scan(mine, lds, one_wave, total);      // (both sums are less than the table's entries: 2^31)
+        int64_t base = want_before + (both >> 32), back_base = back_before + (both & 0xffffffff);
         want_before += total >> 32;
         back_before += total & 0xffffffff;
-        if (in) {
-            const int got = (int) min(max((int64_t) avail - base, (int64_t) 0), (int64_t) want);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (first + i >= a.n) break;
+            const int got = (int) min(max((int64_t) avail - base, (int64_t) 0), (int64_t) want[i]);
             SlotRow r;
-            r.start = start; r.take = take; r.past = past; r.held = held;
-            r.kept = gone ? 0 : held + got;
-            r.base = (int) ((head + base) % a.blocks);
-            r.back = (int) ((head + avail + back_base) % a.blocks);
-            r.gone = gone;
-            desc[b] = r;
-            a.starts[b] = start;
-            a.held[b] = r.kept;
+            r.start = start[i]; r.take = take[i]; r.past = past[i]; r.held = held[i];
+            r.gone = fresh[i] < 0;
+            r.kept = r.gone ? 0 : held[i] + got;
+            r.base = got ? (int) (head + base < a.blocks ? head + base : head + base - a.blocks) : 0;      // (got: base < avail <= blocks)
+            r.back = r.gone ? (int) ((head + avail + back_base) % a.blocks) : 0;
+            desc[first + i] = r;
+            a.starts[first + i] = start[i];
+            a.held[first + i] = r.kept;
+            base += want[i];
+            back_base += back[i];
         }
     }
     if (!one_wave) __syncthreads();                               // every thread has read the counters
@@ -117,7 +141,7 @@ __device__ __forceinline__ void slot_fill_rows(const SlotArgs& a, const SlotRow*
         int32_t* row = a.table + (size_t) b * a.width;
         if (r.gone) {
             for (int i = lane; i < r.held; i += 64) {
-                const int at = (int) (((int64_t) r.back + i) % a.blocks);
+                const int at = (int) (((uint32_t) r.back + (uint32_t) i) % (uint32_t) a.blocks);
                 a.ring[at] = row[i];
                 row[i] = -1;
             }
@@ -154,13 +178,13 @@ __device__ __forceinline__ void slot_fill_tokens(const SlotArgs& a, const SlotRo
 __global__ __launch_bounds__(SLOT_THREADS) void paged_slots_small_kernel(SlotArgs a)
 {
     __shared__ SlotRow desc[SLOT_SMALL_ROWS];
-    slot_scan_rows(a, desc);
+    slot_scan_rows<1>(a, desc);
     __syncthreads();
     slot_fill_tokens(a, desc, threadIdx.x, SLOT_THREADS);
     slot_fill_rows(a, desc, threadIdx.x >> 6, SLOT_WAVES);
 }
 
-__global__ __launch_bounds__(SLOT_THREADS) void paged_slots_scan_kernel(SlotArgs a, SlotRow* desc) { slot_scan_rows(a, desc); }
+__global__ __launch_bounds__(SLOT_THREADS) void paged_slots_scan_kernel(SlotArgs a, SlotRow* desc) { slot_scan_rows<4>(a, desc); }
 
 __global__ __launch_bounds__(256) void paged_slots_fill_kernel(SlotArgs a, const SlotRow* desc, int token_groups)
 {
