@@ -472,13 +472,15 @@ __device__ __forceinline__ void append_run_wide(const AppendArgs& a, int h, int 
     }
 }
 
-// One workgroup = `chunk` (at most 32) token rows of one head: it does the runs that begin there.  Every wave reads the chunk's slots and the page
-// that may follow (at most 32 + 128 of them) in one round of loads; a bit for each row says whether it continues the row before it.
+// One workgroup = `chunk` (at most 32) token rows of one head: it does the runs that begin there.  The chunk's slots and the page that may follow
+// (at most 32 + 128 of them) are read in one round of loads, by one wave for all four (they have to agree on the runs whatever happens to the
+// slots meanwhile); a bit for each row says whether it continues the row before it.
 // P = 0: a wave for every run.
 template <int CODE, bool ROPE, int P> __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ float red[8];
+    __shared__ int slots[192];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // heads next to each other in launch order: what runs at one time reads whole token rows
     const int h = blockIdx.x % a.kv_heads, t0 = (int) (blockIdx.x / a.kv_heads) * a.chunk, count = min(a.chunk, a.rows - t0);
@@ -487,8 +489,11 @@ template <int CODE, bool ROPE, int P> __global__ __launch_bounds__(256) void pag
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
         const int64_t t = (int64_t) t0 - 1 + lane + 64 * i;
-        slot[i] = t >= 0 && t < a.rows ? a.slots[t] : -1;
+        if (wave == 0) slots[lane + 64 * i] = t >= 0 && t < a.rows ? a.slots[t] : -1;
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) slot[i] = slots[lane + 64 * i];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
         int before = __shfl_up(slot[i], 1, 64);
@@ -523,11 +528,12 @@ extern "C" int exl_paged_append(const void* key_states, const void* value_states
                                 void* key_pages, void* value_pages, float* key_scales, float* value_scales, int code, int num_blocks, int num_kv_heads,
                                 int block_size, int head_dim, const int32_t* positions, const void* sin, const void* cos, int angle_rows, void* stream)
 {
-    EXL_REQUIRE(key_states && value_states && slots && key_pages && value_pages && key_scales && value_scales, EXL_E_INVALID, "paged_append: null pointer");
+    EXL_REQUIRE(((key_states && value_states && slots) || rows == 0) && key_pages && value_pages && key_scales && value_scales, EXL_E_INVALID,
+                "paged_append: null pointer");                    // (empty tensors have no address)
     EXL_REQUIRE(rows >= 0 && num_blocks > 0 && num_kv_heads > 0 && num_kv_heads <= 65535, EXL_E_INVALID, "paged_append: bad shape");
     EXL_TRY(paged_check_block("paged_append", block_size, num_blocks));
     EXL_TRY(paged_check_head("paged_append", code, head_dim));
-    EXL_REQUIRE((sin == nullptr) == (cos == nullptr) && (!sin || (positions && angle_rows > 0)), EXL_E_INVALID,
+    EXL_REQUIRE((sin == nullptr) == (cos == nullptr) && (!sin || ((positions || rows == 0) && angle_rows > 0)), EXL_E_INVALID,
                 "paged_append: a rotation needs sin, cos and positions");
     EXL_REQUIRE(key_stride >= (long) num_kv_heads * head_dim && value_stride >= (long) num_kv_heads * head_dim && key_stride % 4 == 0 &&
                 value_stride % 4 == 0 && ((uintptr_t) key_states | (uintptr_t) value_states) % 8 == 0, EXL_E_INVALID,

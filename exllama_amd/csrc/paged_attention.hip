@@ -78,6 +78,11 @@ template <int CODE, bool BIG> __device__ __forceinline__ f16x8 pa_numbers(uint32
     return x.v;
 }
 
+// A value that is NaN and that only some of a tile's queries see (a token of this call, in e4m3 pages): a weight of 0 does not hide it from the
+// others.  In tiles on the border such codes become 0 in the product with the weights, and the sums that they belong to become NaN behind it.
+__device__ __forceinline__ uint32_t pa_nan4(uint32_t codes) { return (((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7; }       // 1 in each byte that is NaN
+__device__ __forceinline__ uint32_t pa_bits4(uint32_t ones) { return ones * 0x10204080u >> 28; }                                        // four bytes of 0 or 1 as four bits
+
 // Query elements d .. d + 7 of one token and head (zeros behind head_dim), rotated at `pos` when there are tables.  A rotated query is no fp16
 // number: hi is the nearest one, lo what it leaves (0 without a rotation).
 struct PaQuery { f16x8 hi, lo; };
@@ -151,11 +156,11 @@ __device__ __forceinline__ PaStretch pa_stretch(const PagedAttn& a, const PaCut&
         total += kept[i];
     }
     for (int b = lane + 64 * KEPT; b < a.n; b += 64) total += places(b);
-    if (a.n == 1) total = __builtin_amdgcn_readfirstlane(total);
-    else {
+    if (a.n > 1) {
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
     }
+    total = __builtin_amdgcn_readfirstlane(total);
     PaStretch st = {-1, 0, 0, 0, 0};
     st.share = max((total + cut.target - 1) / cut.target, cut.min_piece);
     if ((int64_t) w * st.share >= total) return st;
@@ -198,6 +203,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
     const PaStretch to = pa_stretch(a, cut, w);
     if (to.row < 0) return;
     const int group = a.heads / a.kv_heads, lbs = 31 - __clz(a.block);
+    const int by_group = __builtin_amdgcn_readfirstlane((65535 + group) / group);                 // n / group = n * by_group >> 16 (n, group <= 32)
     const size_t kpage = (size_t) a.block * a.hd16;              // bytes of one page of one head, keys or values
     // (columns behind head_dim: key rows read column 0 again, value pages their last 16 columns; the queries there are zeros, the results unused)
     struct Stage { uint4 k[4][KS]; uint4 v[DT]; float ks, vs; bool there; };      // (scales as they are: looking at one here would wait for every load before it)
@@ -227,14 +233,18 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
     f32x4 o[NT][DT];
     float m[NT], l[NT];
     PaRow row;
+    auto lane_here = [] {                                         // the lane once more, opaque: what follows from it takes no registers in the loop over the tiles
+        int zero = 0;
+        asm volatile("" : "+v"(zero));
+        return (int) __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+    };
     auto begin = [&](int b) {                                     // the queries of row b
         row = pa_row_of_wave(a, b);
         const int queries = row.fresh * group;
-        int cc = c, gg = g;                                       // (opaque: what follows from them stays here and takes no registers in the loop over the tiles)
-        asm volatile("" : "+v"(cc), "+v"(gg));
+        const int here = lane_here(), cc = here & 15, gg = here >> 4;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = nt * 16 + cc, i = r / group;
+            const int r = nt * 16 + cc, i = r * by_group >> 16;
             const bool in = r < queries;
             limit[nt] = in ? (int) min((int64_t) row.past + i, (int64_t) row.keys - 1) : -1;
             const f16* q = a.q + (size_t) (row.start + (in ? i : 0)) * a.q_stride + (size_t) (kvh * group + (in ? r - i * group : 0)) * a.hd;
@@ -315,6 +325,40 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
             }
         }
         const PaScale vs = pa_scale<CODE>(st.vs);
+        bool holes = false;
+        uint32_t hole[NT][DT > 8 ? 2 : 1];                        // a bit for each of this lane's sums, the last one lowest
+        if (CODE == EXL_PAGE_FP8 && border && row.fresh > 1) {
+            uint32_t nan = 0;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) nan |= pa_nan4(st.v[t].x) | pa_nan4(st.v[t].y) | pa_nan4(st.v[t].z) | pa_nan4(st.v[t].w);
+            holes = __any(nan);
+        }
+        if (holes) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) for (uint32_t& x : hole[nt]) x = 0;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {                        // a product of 1 (the code 0x38) at every NaN with 1 at every key that a query sees
+                uint4& v = st.v[t];
+                asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));       // (computed again, not kept from above)
+                const uint4 n = make_uint4(pa_nan4(v.x), pa_nan4(v.y), pa_nan4(v.z), pa_nan4(v.w));
+                v.x &= ~(n.x * 255); v.y &= ~(n.y * 255); v.z &= ~(n.z * 255); v.w &= ~(n.w * 255);
+                const f16x8 n0 = pa_numbers<CODE, false>(n.x * 0x38, n.y * 0x38, one), n1 = pa_numbers<CODE, false>(n.z * 0x38, n.w * 0x38, one);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    int n_seen = st.there ? limit[nt] + 1 - key0 : 0;
+                    asm volatile("" : "+v"(n_seen));
+                    f16x8 seen[2];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) seen[i >> 3][i & 7] = i < n_seen ? (f16) 1.f : (f16) 0.f;
+                    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+                    z = __builtin_amdgcn_mfma_f32_16x16x32_f16(n0, seen[0], z, 0, 0, 0);
+                    z = __builtin_amdgcn_mfma_f32_16x16x32_f16(n1, seen[1], z, 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) hole[nt][t >> 3] = hole[nt][t >> 3] << 1 | (z[j] > 0.f ? 1u : 0u);
+                }
+                __builtin_amdgcn_sched_barrier(0);                // (one after the other: all at once they take too many registers)
+            }
+        }
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
             const f16x8 v0 = pa_numbers<CODE, true>(st.v[t].x, st.v[t].y, vs), v1 = pa_numbers<CODE, true>(st.v[t].z, st.v[t].w, vs);
@@ -324,18 +368,25 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
                 o[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[nt][1], o[nt][t], 0, 0, 0);
             }
         }
+        if (holes) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) if (hole[nt][t >> 3] >> ((DT > 8 ? 31 : 4 * DT - 1) - (4 * t + j) % 32) & 1) o[nt][t][j] = NAN;
+        }
     };
 
     // a row's (or a stretch's) end: the sums of the four groups, and out.  `part`: where a partial result goes, or null
     auto end = [&](float* part) {
-        int cc = c, gg = g;
-        asm volatile("" : "+v"(cc), "+v"(gg));
+        const int here = lane_here(), cc = here & 15, gg = here >> 4;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float sum = l[nt];
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
-            const int r = nt * 16 + cc, i = r / group;
+            const int r = nt * 16 + cc, i = r * by_group >> 16;
             if (r >= row.fresh * group) continue;
             if (part) {
                 float* p = part + (size_t) r * (DP + 4);
@@ -376,13 +427,15 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
             work(tile, st);
             if (AHEAD) st = nx;
             else if (more) fetch(ntile, table, st);
-            if (tile == last) break;
+            if (tile >= last) break;
         }
         const bool whole = first == 0 && last == tiles - 1;
         float* part = parts + (((size_t) w * a.kv_heads + kvh) * 2 + (first == 0)) * pa_part_floats(DP, NT);
         end(whole ? nullptr : part);
+        int share = to.share;
+        asm volatile("" : "+s"(share));                           // (the division is not prepared before the loop)
         if (first == 0 && kvh == 0 && lane == 0)                  // for the joining kernel: where the row's parts begin, and how many there are
-            firsts[b] = make_int2(w, (at + PA_BEGIN + tiles - 1) / to.share - w + 1);
+            firsts[b] = make_int2(w, (at + PA_BEGIN + tiles - 1) / share - w + 1);
         if (nb == b) return;
         at += tiles + PA_BEGIN;
         b = nb;
@@ -392,7 +445,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
 
 // The parts of a row joined: `each` (1, 2, 4, ...) queries of one row and kv head for a workgroup, dp / 4 lanes for a query; the lanes that are
 // left take every so many-th part each, with a maximum of their own, and meet in LDS -- in an order that depends on the lengths alone.
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const float* __restrict__ parts, const int2* __restrict__ firsts, int dp, int nt, int each)
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const float* __restrict__ parts, const int2* __restrict__ firsts, int dp, int nt, int each, int target)
 {
     __shared__ f32x4 slice_o[256];
     __shared__ float slice_m[256], slice_l[256];
@@ -400,7 +453,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const
     const PaRow row = pa_row(a, b);
     if (row.keys == 0 || (int) blockIdx.y * each >= row.fresh * group) return;
     const int2 first = firsts[b];                                 // (the row had a first part: it was written)
-    if (first.y < 2) return;
+    if (first.y < 2 || first.x < 0 || first.y > target - first.x) return;      // (beyond the stretches: lengths that changed under the call)
     const int lanes = dp >> 2, slices = 256 / (lanes * each), d = (tid % lanes) * 4, q = tid / lanes % each, sl = tid / (lanes * each);
     const int r = blockIdx.y * each + q;
     const size_t size = pa_part_floats(dp, nt), step = 2 * a.kv_heads * size;
@@ -470,16 +523,17 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const
 
 // A tile of queries and a piece of its keys (all tiles of a row are cut in the same number of `pieces`)
 struct PmItem { int row, tile, piece, pieces; };
+struct PmFound { PmItem item; PaRow row; };                       // (the row as one thread read it: all waves walk the same tiles whatever happens to the lengths meanwhile)
 
 // Item `w` of the launch; row < 0: none.  The cost of a row is tiles of queries * tiles of keys; with `piece` = a `target`-th of all rows' cost
 // (or min_piece), rows of 1.5 times as many keys or more are cut into pieces of about that size -- 4 / 3 * target items at most, and these come first: an item's number is its place
 // among the partial results.  Tiles of a row come with the last (the longest) first; where every item of the launch is resident at once, the
 // second half comes shortest first: the two workgroups of a compute unit, half a launch apart, then have equal work together.
-// lds: 80 bytes, free again afterwards.
-__device__ __forceinline__ PmItem pm_find(const PagedAttn& a, const PaCut& cut, int w, void* lds)
+// lds: 96 bytes, free again afterwards.
+__device__ __forceinline__ PmFound pm_find(const PagedAttn& a, const PaCut& cut, int w, void* lds)
 {
     int64_t* sums = (int64_t*) lds;
-    PmItem& found = *(PmItem*) (sums + 2 * PA_WAVES);
+    PmFound& found = *(PmFound*) (sums + 2 * PA_WAVES);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, step = PA_WAVES * 64;
     struct Size { int q, keys; };
     auto size = [&](int b) -> Size {
@@ -497,7 +551,7 @@ __device__ __forceinline__ PmItem pm_find(const PagedAttn& a, const PaCut& cut, 
     const Size mine = tid < a.n ? size(tid) : Size{0, 0};           // (of the first 256 rows, kept)
     int64_t cost = 0;
     for (int b = tid; b < a.n; b += step) { const Size z = b == tid ? mine : size(b); cost += (int64_t) z.q * z.keys; }
-    if (tid == 0) found = {-1, 0, 0, 0};
+    if (tid == 0) found.item.row = -1;
     cost = total(cost, 0);
     const int64_t even = (cost + cut.target - 1) / cut.target;
     const int piece = (int) min(max(even, (int64_t) cut.min_piece), (int64_t) 1 << 30);
@@ -523,13 +577,14 @@ __device__ __forceinline__ PmItem pm_find(const PagedAttn& a, const PaCut& cut, 
         if (w >= base && w < base + here) {
             const int k = (int) (w - base), t = k / np, half = (z.q + 1) / 2;
             const bool fold = !first && cost <= (int64_t) cut.target * z.keys;        // (as many tiles as fit at once, or fewer)
-            found = {b, fold && t >= half ? t - half : z.q - 1 - t, k % np, np};
+            found.item = {b, fold && t >= half ? t - half : z.q - 1 - t, k % np, np};
+            found.row = pa_row(a, b);
         }
         before += sums[0] + sums[1] + sums[2] + sums[3];
         if (before > w) break;
     }
     __syncthreads();
-    const PmItem it = found;
+    const PmFound it = found;
     __syncthreads();                                              // `lds` is the caller's again
     return it;
 }
@@ -540,16 +595,21 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
                                                                                         PmItem* __restrict__ items, int part_items)
 {
     constexpr int KB = DP / 16, DT = DP / 32, PIECES = PA_KEYS * KB / 256;       // 16-byte pieces of codes per thread: keys, and as many of values
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // [2][keys: 2 * KB * 1024 bytes, values: 4 * DT * 1024 bytes]
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // [2][keys: 2 * KB * 1024 bytes, values: 4 * DT * 1024 bytes], [2][DP] maps, 2 ints
     constexpr int K_BYTES = 2 * KB * 1024, BUF = 2 * K_BYTES;
+    uint64_t* nan_map = (uint64_t*) (lds + 2 * BUF);              // by buffer, of a tile on the border: the tokens whose value is NaN, a word for each column
+    int* nan_tile = (int*) (nan_map + 2 * DP);                    // by buffer: the last tile on the border that held one
     // kv heads next to each other in launch order: consecutive workgroups go to different XCDs, so that those of one head (the same keys and
     // values) share an XCD's L2 where kv_heads is a multiple of 8, and every XCD gets tiles of all lengths
     const int kvh = blockIdx.x % a.kv_heads, w = blockIdx.x / a.kv_heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, g = lane >> 5;
-    const PmItem it = pm_find(a, cut, w, lds);
+    if (tid < 2) nan_tile[tid] = -1;                              // (pm_find has barriers)
+    const PmFound found = pm_find(a, cut, w, lds);
+    const PmItem it = found.item;
     if (kvh == 0 && tid == 0 && w < part_items) items[w] = it;                   // for the joining kernel
     if (it.row < 0) return;
-    const PaRow row = pa_row(a, __builtin_amdgcn_readfirstlane(it.row));
+    const PaRow row = {__builtin_amdgcn_readfirstlane(found.row.start), __builtin_amdgcn_readfirstlane(found.row.fresh), __builtin_amdgcn_readfirstlane(found.row.past),
+                       __builtin_amdgcn_readfirstlane(found.row.keys)};
     const int group = a.heads / a.kv_heads, lbs = 31 - __clz(a.block);
     const int64_t queries = (int64_t) row.fresh * group, q0 = (int64_t) it.tile * PM_ROWS;
     const int last_token = (int) ((min(q0 + PM_ROWS, queries) - 1) / group);
@@ -645,13 +705,28 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
         k_to[i] = (kt * KB + k_ch) * 1024 + ((m ^ (k_ch & 7)) << 4);
         v_to[i] = K_BYTES + ((v_kc >> 1) * 2 * DT + (d >> 5)) * 1024 + ((((v_kc & 1) * 32 + (d & 31)) ^ (v_kc << 1)) << 4);
     }
-    auto store = [&](Stage& st, unsigned char* buf) {
+    const int free_keys = (int) min((int64_t) row.past + (int) (q0 / group), (int64_t) row.keys - 1);       // the last key that all queries of the workgroup see
+    auto store = [&](int tile, Stage& st) {
+        unsigned char* buf = lds + ((tile - t_first) & 1) * BUF;
         if (__any(st.n < 16)) {                                   // bytes that hold no value may be anything, NaN too: a weight of 0 does not hide it
             uint32_t mask[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) mask[i] = st.n >= 4 * i + 4 ? 0xffffffffu : st.n <= 4 * i ? 0u : (1u << (8 * (st.n - 4 * i))) - 1;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) { st.v[i].x &= mask[0]; st.v[i].y &= mask[1]; st.v[i].z &= mask[2]; st.v[i].w &= mask[3]; }
+        }
+        if (CODE == EXL_PAGE_FP8 && tile * PA_KEYS + PA_KEYS - 1 > free_keys) {
+            uint32_t nan = 0;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                uint4& v = st.v[i];
+                const uint4 n = make_uint4(pa_nan4(v.x), pa_nan4(v.y), pa_nan4(v.z), pa_nan4(v.w));
+                v.x &= ~(n.x * 255); v.y &= ~(n.y * 255); v.z &= ~(n.z * 255); v.w &= ~(n.w * 255);
+                const uint32_t bits = pa_bits4(n.x) | pa_bits4(n.y) << 4 | pa_bits4(n.z) << 8 | pa_bits4(n.w) << 12;
+                ((uint16_t*) (nan_map + ((tile - t_first) & 1) * DP + v_d + 64 * i))[v_kc] = (uint16_t) bits;
+                nan |= bits;
+            }
+            if (nan) nan_tile[(tile - t_first) & 1] = tile;
         }
         const PaScale vscale = pa_scale<CODE>(st.vs);
         PaScale kscale[WIDE ? 1 : PIECES];
@@ -686,7 +761,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     if (t_first < t_last) {
         fetch(t_first, look(t_first), st);
         there = st.there;
-        store(st, lds);
+        store(t_first, st);
         if (t_first + 1 < t_last) fetch(t_first + 1, look(t_first + 1), st);
         if (t_first + 2 < t_last) id = look(t_first + 2);
     }
@@ -696,7 +771,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
         __syncthreads();                                          // this tile is in `buf`, and every wave is through with the other one
         if (tile + 1 < t_last) {
             there = st.there;
-            store(st, lds + ((tile + 1 - t_first) & 1) * BUF);
+            store(tile + 1, st);
             if (tile + 2 < t_last) {
                 fetch(tile + 2, id, st);
                 if (tile + 3 < t_last) id = look(tile + 3);
@@ -759,6 +834,19 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
                     const f16x8 v = *(const f16x8*) (buf + K_BYTES + ((kt * 2 + h) * DT + t) * 1024 + ((lane ^ (4 * kt + 2 * g)) << 4));
                     o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[kt][h], o[t], 0, 0, 0);
                 }
+        if (CODE == EXL_PAGE_FP8 && tile * PA_KEYS + PA_KEYS - 1 > free_keys && __builtin_amdgcn_readfirstlane(nan_tile[(tile - t_first) & 1]) == tile) {
+            uint64_t seen = 0;                                    // the keys of the tile that this lane's query sees
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int n = now >> u & 1 ? min(max(limit - (tile * PA_KEYS + 16 * u) + 1, 0), 16) : 0;
+                seen |= (uint64_t) ((1u << n) - 1) << (16 * u);
+            }
+            const uint64_t* map = nan_map + ((tile - t_first) & 1) * DP;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) if (map[32 * t + 8 * (j >> 2) + 4 * g + (j & 3)] & seen) o[t][j] = NAN;
+        }
     }
 
     // ---- out: row j of a product is column 32 t + 8 * (j >> 2) + 4 g + (j & 3)
@@ -880,14 +968,14 @@ template <int CODE> static int pa_launch(const PagedAttn& a, const PaPlan& p, vo
         int each = 1;                                             // queries of a joining workgroup: as many as leave work for the whole machine
         while (2 * each <= 1024 / p.dp && each < p.rows_y && (int64_t) a.n * a.kv_heads * ((p.rows_y + 2 * each - 1) / (2 * each)) >= 512) each *= 2;
         hipLaunchKernelGGL(paged_attn_join_kernel, dim3((unsigned) a.n, (unsigned) ((p.rows_y + each - 1) / each), (unsigned) a.kv_heads), dim3(256), 0, s, a, parts, firsts,
-                           p.dp, p.nt, each);
+                           p.dp, p.nt, each, p.cut.target);
         EXL_LAUNCH_CHECK();
         return 0;
     }
     PmItem* list = (PmItem*) workspace;
 #define PA_MANY(DP, WIDE) do { static bool done[EXL_MAX_DEVICES] = {};                                                                       \
     EXL_TRY(exl_lds_opt_in((const void*) paged_attn_many_kernel<CODE, DP, WIDE>, done));                                                      \
-    hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE>), grid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4, s, a, p.cut, parts, list, p.parts); } while (0)
+    hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE>), grid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4 + 2 * DP * 8 + 8, s, a, p.cut, parts, list, p.parts); } while (0)
     if (a.block >= PA_KEYS) { if (p.dp == 64) PA_MANY(64, true); else if (p.dp == 128) PA_MANY(128, true); else PA_MANY(256, true); }
     else                    { if (p.dp == 64) PA_MANY(64, false); else if (p.dp == 128) PA_MANY(128, false); else PA_MANY(256, false); }
 #undef PA_MANY
@@ -917,7 +1005,8 @@ extern "C" int exl_paged_attention(const void* q, long q_stride, const int32_t* 
                                    int num_kv_heads, int head_dim, float scale, const void* sin, const void* cos, int angle_rows, void* out,
                                    void* workspace, size_t workspace_bytes, void* stream)
 {
-    EXL_REQUIRE(q && starts && past_lens && new_lens && block_table && key_pages && value_pages && key_scales && value_scales && out, EXL_E_INVALID,
+    const bool none = rows == 0 || max_new == 0;                  // (nothing to do: empty tensors have no address)
+    EXL_REQUIRE(((q && out) || none) && starts && past_lens && new_lens && block_table && key_pages && value_pages && key_scales && value_scales, EXL_E_INVALID,
                 "paged_attention: null pointer");
     EXL_REQUIRE(n_rows > 0 && rows >= 0 && max_new >= 0 && table_width > 0 && num_blocks > 0 && num_heads > 0 && num_kv_heads > 0 &&
                 num_heads <= 65535, EXL_E_INVALID, "paged_attention: bad shape");
@@ -931,7 +1020,9 @@ extern "C" int exl_paged_attention(const void* q, long q_stride, const int32_t* 
     EXL_REQUIRE((int64_t) table_width * block_size <= 0x7fffffff, EXL_E_UNSUPPORTED, "paged_attention: the block table exceeds 2^31 tokens");
     EXL_REQUIRE((int64_t) n_rows * ((int64_t) table_width * block_size / PA_KEYS + PA_BEGIN + 1) < 1 << 30, EXL_E_UNSUPPORTED,
                 "paged_attention: %d rows of %d blocks are too many", n_rows, table_width);
-    if (rows == 0 || max_new == 0) return 0;
+    if (none) return 0;
+    EXL_REQUIRE((uintptr_t) out >= (uintptr_t) q + 2 * ((size_t) (rows - 1) * q_stride + (size_t) num_heads * head_dim) ||
+                (uintptr_t) q >= (uintptr_t) out + 2 * (size_t) rows * num_heads * head_dim, EXL_E_INVALID, "paged_attention: out overlaps q");
     PagedAttn a = {(const f16*) q, starts, past_lens, new_lens, block_table, (const uint8_t*) key_pages, (const uint8_t*) value_pages, key_scales,
                    value_scales, (const f16*) sin, (const f16*) cos, (f16*) out, n_rows, rows, max_new, table_width, num_blocks, block_size, num_heads,
                    num_kv_heads, head_dim, (head_dim + 15) / 16 * 16, angle_rows, q_stride, scale > 0.f ? scale : 1.f / sqrtf((float) head_dim)};

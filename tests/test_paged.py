@@ -119,3 +119,56 @@ def test_c_entries_refuse_before_they_launch(ext):
         msg = lib.exl_last_error().decode()
         assert msg.startswith("paged_" + fn.__name__), (fn.__name__, kw, msg)
     assert append(rows=0) == 0 and attention(rows=0) == 0 and attention(max_new=0) == 0
+
+
+def test_c_attention_refuses_a_small_workspace_and_an_out_that_overlaps(ext):
+    lib = ext._lib.load()
+    p, far = C.c_void_p(4096), C.c_void_p(1 << 20)            # never read: every call below is refused first
+
+    def attention(out, ws, ws_bytes, rows=40, n=2):
+        return lib.exl_paged_attention(p, 64, p, p, p, n, rows, rows, p, 400, p, p, p, p, 0, 8, 16, 1, 1, 64, 0.0, None, None, 0, out, ws, ws_bytes, None)
+
+    for rows in (1, 40):                                      # few queries, and many
+        need = lib.exl_paged_attention_workspace(2, rows, rows, 1, 1, 64, 400, 16)
+        assert need > 0
+        for out, ws, ws_bytes, what in ((far, None, need, "workspace"), (far, p, need - 1, "workspace"), (far, C.c_void_p(4104), need, "workspace"),
+                                        (p, p, need, "overlaps"), (C.c_void_p(4096 + 128 * rows - 2 * 4), p, need, "overlaps")):
+            assert attention(out, ws, ws_bytes, rows) < 0
+            assert what in lib.exl_last_error().decode(), (rows, what)
+    assert lib.exl_paged_attention_workspace(0, 1, 1, 1, 1, 64, 4, 16) == 0 and lib.exl_paged_attention_workspace(1, 1, 1, 3, 2, 64, 4, 16) == 0
+
+
+def test_c_entries_take_empty_tensors(ext):
+    """No rows: nothing is launched, and the addresses of empty tensors (null) are fine."""
+    lib = ext._lib.load()
+    p = C.c_void_p(4096)
+    assert lib.exl_paged_append(None, None, 64, 64, None, 0, p, p, p, p, 0, 8, 1, 16, 64, None, p, p, 4, None) == 0
+    assert lib.exl_paged_attention(None, 64, p, p, p, 1, 0, 1, p, 4, p, p, p, p, 0, 8, 16, 1, 1, 64, 0.0, None, None, 0, None, None, 0, None) == 0
+
+
+def test_kernels_fit_their_registers():
+    """No paged kernel spills, and each fits the waves per SIMD that it is declared for (512 registers of a SIMD: 256 for two waves)."""
+    import os
+    import sys
+    import tempfile
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    path = os.path.join(root, "exllama_amd", "libexl_amd.so")
+    if not os.path.exists(path):
+        pytest.skip("libexl_amd.so not built")
+    sys.path.insert(0, os.path.join(root, "scripts"))
+    import isa_lint
+
+    with tempfile.TemporaryDirectory() as d:
+        res = {n: r for n, r in isa_lint.kernel_resources(path, d).items() if "paged_" in n}
+    assert sum("paged_attn_few" in n for n in res) == 10 and sum("paged_attn_many" in n for n in res) == 12 and sum("paged_append" in n for n in res) == 20
+    for n, r in res.items():
+        assert r["scratch"] == 0, (n, r)
+        total = r["vgpr"]                                      # (of both kinds)
+        if "paged_attn_few" in n or "paged_attn_many" in n:
+            one = "ELi256E" in n or "ILi0ELi128ELi2E" in n or "ILi1ELi128ELi2E" in n
+            assert total <= (512 if one else 256), (n, r)
+        elif "paged_attn_join" in n:
+            assert total <= 128, (n, r)
+        elif "paged_slots" in n:
+            assert total <= 128, (n, r)                        # 1024 threads

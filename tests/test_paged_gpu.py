@@ -442,3 +442,232 @@ def test_calls_on_two_streams_do_not_meet(ext):
                 g.append(call(d))
     torch.cuda.synchronize()
     assert all(torch.equal(x, one) for x in got[0]) and all(torch.equal(x, two) for x in got[1])
+
+
+# ---- calls that are allowed and rarely made ----------------------------------------------------------------------------------------------
+
+def test_append_of_many_rows(ext):
+    """Enough token rows that a workgroup looks at 32 of them: long runs, runs of one token, skipped rows."""
+    rng = np.random.default_rng(20)
+    hd, kvh, block, blocks = 16, 32, 128, 80
+    pool = _pool(rng, blocks, kvh, block, hd, "fp8")
+    dev = _pool_dev(pool, "fp8")
+    slots, pos = _runs(rng, blocks, block, [(3, 1500), (0, 1), (-1, -33), (127, 1400), (64, 64), (5, 2), (0, 1200), (-1, -1)] + [(9, 1)] * 20)
+    t = len(slots)
+    assert t * kvh > 131072
+    x = rng.normal(0, 1, (2, t, kvh, hd)).astype(np.float16)
+    ext.ext_paged_append(*(torch.from_numpy(y).reshape(t, -1).to(DEV) for y in x), _dev(slots), *dev)
+    P.append(x[0], x[1], slots, *pool, "fp8")
+    for name, got, want in zip(("keys", "values", "key scales", "value scales"), dev, pool):
+        assert _same(_numbers(got), want), name
+
+
+@pytest.mark.parametrize("n,max_new", [(70, 1), (300, 1), (300, 3), (70, 60), (300, 40)])
+def test_attention_of_many_rows(ext, n, max_new):
+    """More rows than a wave, and than a workgroup, looks at once; most of them short, some without a token."""
+    rng = np.random.default_rng(n + max_new)
+    new = rng.integers(0, min(max_new, 4) + 1, n)
+    new[rng.integers(n)] = max_new
+    past = np.where(rng.random(n) < 0.05, 400, rng.integers(0, 40, n))
+    host, dev = _attention_case(rng, "int8", 64, 2, 1, 16, [(int(p), int(m)) for p, m in zip(past, new)])
+    _check_attention(ext, host, dev, 2, True)
+
+
+@pytest.mark.parametrize("code", ["fp8", "int8"])
+@pytest.mark.parametrize("hd,lens", [(128, [(90, 3), (700, 1)]), (256, [(5, 1)]), (64, [(90, 70), (700, 200)]), (100, [(1200, 90)])])
+def test_attention_under_the_largest_scales(ext, code, hd, lens):
+    """The upper end of the scales' range: codes * scale up to 65024 and 57344, keys and values alike, a scale for each page and head."""
+    rng = np.random.default_rng(hd)
+    host, dev = _attention_case(rng, code, hd, 4, 2, 16, lens)
+    for i in (2, 3):
+        host["pool"][i] = np.ldexp(1.0, rng.integers(3, P.EXP[code][1] + 1, host["pool"][i].shape))
+        dev["pool"][i] = _dev(host["pool"][i], torch.float32)
+    host["q"] = (host["q"].astype(np.float64) * 2.0 ** -13).astype(np.float16)
+    dev["q"] = torch.from_numpy(host["q"]).reshape(len(host["q"]), -1).to(DEV)
+    _check_attention(ext, host, dev, 4, True)
+    _check_attention(ext, host, dev, 4, False)
+
+
+# hd, heads, kv heads, (past, new): few queries, in one stretch and in several; many, in one piece and in several
+NAN_CASES = [(128, 4, 4, (70, 20)), (64, 8, 8, (1900, 30)), (256, 2, 2, (62, 14)), (100, 4, 2, (30, 16)), (128, 8, 1, (62, 4)), (128, 2, 2, (40, 200)),
+             (64, 4, 1, (900, 100)), (256, 2, 1, (1500, 130)), (80, 2, 2, (0, 300))]
+
+
+@pytest.mark.parametrize("what", ["value", "key", "query"])
+@pytest.mark.parametrize("hd,heads,kvh,row", NAN_CASES)
+def test_nan_stays_where_it_is_seen(ext, what, hd, heads, kvh, row):
+    """A token whose value, key or query is NaN: the queries that see it (and its columns; all of its row) are NaN, no other is."""
+    for block in (16, 64):
+        host, dev = _attention_case(np.random.default_rng(hd + block), "fp8", hd, heads, kvh, block, [row, (33, 2)])
+        past, new = row
+        group, at, j = heads // kvh, past + new // 3, new // 3
+        page, off = host["table"][0, at // block], at % block
+        want, bound = P.attention(host["q"], host["starts"], host["past"], host["new"], host["table"], *host["pool"], int(host["new"].max()))
+        nan = np.isnan(bound)
+        expect = np.zeros_like(nan)
+        if what == "value":
+            cols = [0, 7 % hd, hd - 1]
+            host["pool"][1][page, 0, cols, off] = np.nan
+            for c in cols:
+                expect[j:new, :group, c] = True
+        elif what == "key":
+            host["pool"][0][page, kvh - 1, off, 3] = np.nan
+            expect[j:new, heads - group:] = True
+        else:
+            host["q"][j, 1, hd - 2] = np.nan
+            dev["q"] = torch.from_numpy(host["q"]).reshape(len(host["q"]), -1).to(DEV)
+            expect[j, 1] = True
+        dev["pool"] = _pool_dev(host["pool"], "fp8")
+        got = ext.ext_paged_attention(dev["q"], dev["starts"], dev["past"], dev["new"], dev["table"], *dev["pool"], heads,
+                                      max_new=int(host["new"].max())).cpu().double().numpy().reshape(want.shape)
+        assert np.array_equal(np.isnan(got), expect)
+        ok = ~expect & ~nan
+        assert (np.abs(got - want)[ok] <= bound[ok]).all()
+
+
+def test_calls_without_rows(ext):
+    pool = _pool_dev(_pool(np.random.default_rng(21), 3, 2, 16, 64, "int8"), "int8")
+    before = [p.clone() for p in pool]
+    x = torch.zeros(0, 128, dtype=torch.float16, device=DEV)
+    none, one = torch.zeros(0, dtype=torch.int32, device=DEV), _dev([1])
+    ext.ext_paged_append(x, x, none, *pool)
+    ext.ext_paged_append(x, x, none, *pool, positions=none, sin=torch.zeros(4, 64, dtype=torch.float16, device=DEV),
+                         cos=torch.zeros(4, 64, dtype=torch.float16, device=DEV))
+    assert ext.ext_paged_attention(x, _dev([0, 0]), one, one, _dev([[0, 1]]), *pool, 2).shape == (0, 128)
+    y = torch.zeros(3, 128, dtype=torch.float16, device=DEV)
+    out = ext.ext_paged_attention(y, _dev([0, 0]), one, one, _dev([[0, 1]]), *pool, 2, max_new=0, out=torch.full_like(y, 3))
+    assert (out == 3).all()
+    held, table, ring, counters = _dev([0]), _dev([[-1, -1]]), _dev([0, 1, 2]), _dev([0, 3, 0, 0])
+    starts, slots, positions = ext.ext_paged_slots(_dev([5]), _dev([0]), held, table, ring, counters, 16, 0)
+    assert starts.tolist() == [0, 0] and slots.numel() == 0 and positions.numel() == 0
+    assert held.tolist() == [1] and table.tolist() == [[0, -1]] and counters.tolist() == [1, 2, 0, 0]
+    for a, b in zip(before, pool):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_all_rows_end_at_once(ext):
+    """Every block goes back, in the rows' order, and is handed out again by the next call."""
+    past, held, table = _dev([40, 0, 17]), _dev([3, 0, 2]), _dev([[4, 1, 0], [-1, -1, -1], [3, 2, -1]])
+    ring, counters = _dev([-7] * 5), _dev([2, 0, 0, 0])
+    _, slots, _ = ext.ext_paged_slots(past, _dev([-1, -1, -1]), held, table, ring, counters, 16, 4)
+    assert held.tolist() == [0, 0, 0] and (table == -1).all() and (slots == -1).all()
+    assert counters.tolist() == [2, 5, 0, 0] and ring.tolist() == [3, 2, 4, 1, 0]
+    past.zero_()
+    ext.ext_paged_slots(past, _dev([0, 33, 32]), held, table, ring, counters, 16, 65)
+    assert table.tolist() == [[-1, -1, -1], [4, 1, 0], [3, 2, -1]] and counters.tolist() == [2, 0, 0, 0]
+
+
+def test_padded_batch_through_all_three(ext):
+    """Rows a fixed distance apart, from the slots on: the padding is neither stored nor computed."""
+    rng, (n, stride, hd, heads, kvh, block, blocks) = np.random.default_rng(22), (4, 9, 64, 4, 2, 16, 30)
+    past, held = np.zeros(n, np.int32), np.zeros(n, np.int32)
+    table, ring, counters = np.full((n, 4), -1, np.int32), rng.permutation(blocks).astype(np.int32), np.array([7, blocks, 0, 0], np.int32)
+    pool = [np.zeros((blocks, kvh, block, hd)), np.zeros((blocks, kvh, hd, block)), np.ones((blocks, kvh)), np.ones((blocks, kvh))]
+    dpool = _pool_dev(pool, "fp8")
+    d = [_dev(x) for x in (past, held, table, ring, counters)]
+    for new in ([9, 3, 0, 20], [1, 1, 9, 1], [1, 9, 1, 1]):
+        new = np.array(new)
+        q, k, v = (rng.normal(0, 1, (n * stride, h, hd)).astype(np.float16) for h in (heads, kvh, kvh))
+        dq, dk, dv = (torch.from_numpy(x).reshape(n * stride, -1).to(DEV) for x in (q, k, v))
+        starts, slots, positions = P.slots(past, new, held, table, ring, counters, block, 64, stride, n * stride, stride)
+        gstarts, gslots, gpos = ext.ext_paged_slots(d[0], _dev(new), d[1], d[2], d[3], d[4], block, n * stride, max_new=stride, row_stride=stride)
+        assert gstarts.tolist() == starts.tolist() and gslots.tolist() == slots.tolist() and gpos.tolist() == positions.tolist()
+        ext.ext_paged_append(dk, dv, gslots, *dpool)
+        P.append(k, v, slots, *pool, "fp8")
+        new = np.minimum(new, stride)
+        out = torch.full((n * stride, heads * hd), 7.5, dtype=torch.float16, device=DEV)
+        ext.ext_paged_attention(dq, gstarts, d[0], _dev(new), d[2], *dpool, heads, max_new=stride, out=out)
+        want, bound = P.attention(q, starts, past, new, table, *pool, stride)
+        got, none = out.cpu().double().numpy().reshape(want.shape), np.isnan(bound)
+        assert (got[none] == 7.5).all() and (np.abs(got - want)[~none] <= bound[~none]).all()
+        past += new.astype(np.int32)
+        d[0].copy_(_dev(past))
+
+
+def test_captured_prompt_pieces_replay(ext):
+    """Attention of many queries captured once (rows cut into pieces, joined), replayed under other lengths, with eager work in between; a second
+    graph captured beside it has a workspace of its own."""
+    host, dev = _attention_case(np.random.default_rng(23), "fp8", 128, 8, 2, 64, [(1700, 120), (300, 60), (0, 90)])
+    call = lambda past, new, out: ext.ext_paged_attention(dev["q"], dev["starts"], past, new, dev["table"], *dev["pool"], 8, max_new=120,  # noqa: E731
+                                                          sin=dev["sin"], cos=dev["cos"], out=out)
+    sets = [(host["past"], host["new"]), (host["past"] // 2, host["new"]), (host["past"], np.array([120, 0, 3])), (host["past"] * 0, np.array([1, 60, 90]))]
+    graphs = []
+    side = torch.cuda.Stream()
+    for _ in range(2):
+        past, new, out = dev["past"].clone(), dev["new"].clone(), torch.zeros_like(dev["q"])
+        with torch.cuda.stream(side):
+            call(past, new, out)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(past, new, out)
+        graphs.append((g, past, new, out))
+    for step in range(8):
+        eager = []
+        for u, (g, past, new, out) in enumerate(graphs):
+            p, m = sets[(step + u) % 4]
+            past.copy_(_dev(p)); new.copy_(_dev(m)); out.fill_(7.5)
+            eager.append(call(_dev(p), _dev(m), torch.full_like(out, 7.5)))
+        for g, *_ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for (g, past, new, out), want in zip(graphs, eager):
+            assert torch.equal(out, want), step
+
+
+def test_prompts_on_two_streams_do_not_meet(ext):
+    host, dev = _attention_case(np.random.default_rng(24), "int8", 128, 4, 2, 32, [(1500, 100), (900, 150)])
+    other = dict(dev, past=_dev(host["past"] // 3))
+    call = lambda d: ext.ext_paged_attention(d["q"], d["starts"], d["past"], d["new"], d["table"], *d["pool"], 4, max_new=150)  # noqa: E731
+    one, two = call(dev), call(other)
+    torch.cuda.synchronize()
+    streams, got = (torch.cuda.Stream(), torch.cuda.Stream()), ([], [])
+    for _ in range(10):
+        for s, d, g in zip(streams, (dev, other), got):
+            with torch.cuda.stream(s):
+                g.append(call(d))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, one) for x in got[0]) and all(torch.equal(x, two) for x in got[1])
+
+
+def test_out_must_not_overlap_q(ext):
+    host, dev = _attention_case(np.random.default_rng(25), "fp8", 64, 2, 2, 16, [(20, 3)])
+    args = (dev["starts"], dev["past"], dev["new"], dev["table"], *dev["pool"], 2)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ext.ext_paged_attention(dev["q"], *args, out=dev["q"])
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ext.ext_paged_attention(dev["q"][:3], *args, out=dev["q"][2:5])
+    both = torch.cat((dev["q"], dev["q"]))                     # next to each other is fine
+    assert ext.ext_paged_attention(both[:5], *args, out=both[5:]).data_ptr() == both[5:].data_ptr()
+
+
+def test_compiled_binding_and_ctypes_path_agree(ext):
+    """The compiled binding against the ctypes methods that it replaces: the same results to the bit, the same refusals."""
+    fast, slow = ext.FAST_BINDING, type(ext.exllama_ext)
+    assert fast is not None and ext.paged_slots is fast.paged_slots and ext.paged_append is fast.paged_append and ext.paged_attention is fast.paged_attention
+    results = []
+    for pick in (lambda n: getattr(fast, n), lambda n: lambda *a, **k: getattr(slow, n)(ext.exllama_ext, *a, **k)):
+        rng = np.random.default_rng(26)
+        pool = _pool_dev(_pool(rng, 12, 2, 16, 64, "fp8"), "fp8")
+        past, new, held, table = _dev([5, 30]), _dev([4, 9]), _dev([0, 0]), torch.full((2, 4), -1, dtype=torch.int32, device=DEV)
+        ring, counters = _dev(rng.permutation(12)), _dev([3, 12, 0, 0])
+        sin, cos = (x.to(DEV) for x in _angles(64, 64))
+        x = [torch.from_numpy(rng.normal(0, 1, (14, h * 64)).astype(np.float16)).to(DEV) for h in (4, 2, 2)]
+        starts, slots, positions = pick("paged_slots")(past, new, held, table, ring, counters, 16, 14, max_len=60)
+        pick("paged_append")(x[1], x[2], slots, *pool, positions, sin, cos)
+        out = torch.full((14, 256), 7.5, dtype=torch.float16, device=DEV)
+        assert pick("paged_attention")(x[0], starts, past, new, table, *pool, 4, 9, sin, cos, 0.1, out) is out
+        fresh = pick("paged_attention")(x[0], starts, past, new, table, *pool, 4)
+        results.append([starts, slots, positions, held, table, ring, counters, *[p.view(torch.uint8) for p in pool], out, fresh])
+        for bad in (dict(out=out.float()), dict(out=out[:3]), dict(sin=sin), dict(sin=sin[:, :32], cos=cos[:, :32])):
+            with pytest.raises(RuntimeError):
+                pick("paged_attention")(x[0], starts, past, new, table, *pool, 4, **bad)
+        with pytest.raises(RuntimeError):
+            pick("paged_append")(x[1], x[2][:5], slots, *pool)
+        with pytest.raises(RuntimeError):
+            pick("paged_append")(x[1], x[2], slots[:5], *pool)
+        with pytest.raises(RuntimeError):
+            pick("paged_slots")(past, new[:1], held, table, ring, counters, 16, 14)
+        with pytest.raises(RuntimeError):
+            pick("paged_slots")(past, new, held, table[:1], ring, counters, 16, 14)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
