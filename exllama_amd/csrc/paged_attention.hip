@@ -708,23 +708,22 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     const int free_keys = (int) min((int64_t) row.past + (int) (q0 / group), (int64_t) row.keys - 1);       // the last key that all queries of the workgroup see
     auto store = [&](int tile, Stage& st) {
         unsigned char* buf = lds + ((tile - t_first) & 1) * BUF;
-        if (__any(st.n < 16)) {                                   // bytes that hold no value may be anything, NaN too: a weight of 0 does not hide it
-            uint32_t mask[4];
+        const bool border = tile * PA_KEYS + PA_KEYS - 1 > free_keys;
+        if (border || __any(st.n < 16)) {                         // bytes that hold no value may be anything, NaN too: a weight of 0 does not hide it
+            uint32_t mask[4], nan = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) mask[i] = st.n >= 4 * i + 4 ? 0xffffffffu : st.n <= 4 * i ? 0u : (1u << (8 * (st.n - 4 * i))) - 1;
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) { st.v[i].x &= mask[0]; st.v[i].y &= mask[1]; st.v[i].z &= mask[2]; st.v[i].w &= mask[3]; }
-        }
-        if (CODE == EXL_PAGE_FP8 && tile * PA_KEYS + PA_KEYS - 1 > free_keys) {
-            uint32_t nan = 0;
-#pragma unroll
             for (int i = 0; i < PIECES; ++i) {
                 uint4& v = st.v[i];
-                const uint4 n = make_uint4(pa_nan4(v.x), pa_nan4(v.y), pa_nan4(v.z), pa_nan4(v.w));
-                v.x &= ~(n.x * 255); v.y &= ~(n.y * 255); v.z &= ~(n.z * 255); v.w &= ~(n.w * 255);
-                const uint32_t bits = pa_bits4(n.x) | pa_bits4(n.y) << 4 | pa_bits4(n.z) << 8 | pa_bits4(n.w) << 12;
-                ((uint16_t*) (nan_map + ((tile - t_first) & 1) * DP + v_d + 64 * i))[v_kc] = (uint16_t) bits;
-                nan |= bits;
+                v.x &= mask[0]; v.y &= mask[1]; v.z &= mask[2]; v.w &= mask[3];
+                if (CODE == EXL_PAGE_FP8 && border) {
+                    const uint4 n = make_uint4(pa_nan4(v.x), pa_nan4(v.y), pa_nan4(v.z), pa_nan4(v.w));
+                    v.x &= ~(n.x * 255); v.y &= ~(n.y * 255); v.z &= ~(n.z * 255); v.w &= ~(n.w * 255);
+                    const uint32_t bits = pa_bits4(n.x) | pa_bits4(n.y) << 4 | pa_bits4(n.z) << 8 | pa_bits4(n.w) << 12;
+                    ((uint16_t*) (nan_map + ((tile - t_first) & 1) * DP + v_d + 64 * i))[v_kc] = (uint16_t) bits;
+                    nan |= bits;
+                }
             }
             if (nan) nan_tile[(tile - t_first) & 1] = tile;
         }
