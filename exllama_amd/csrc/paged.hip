@@ -472,8 +472,8 @@ __device__ __forceinline__ void append_run_wide(const AppendArgs& a, int h, int 
     }
 }
 
-// One workgroup = `chunk` (at most 32) token rows of one head: it does the runs that begin there.  The chunk's slots and the page that may follow
-// (at most 32 + 128 of them) are read in one round of loads, by one wave for all four (they have to agree on the runs whatever happens to the
+// One workgroup = `chunk` (at most 63) token rows of one head: it does the runs that begin there.  The chunk's slots and the page that may follow
+// (at most 63 + 127 of them, and the one before) are read in one round of loads, by one wave for all four (they have to agree on the runs whatever happens to the
 // slots meanwhile); a bit for each row says whether it continues the row before it.
 // P = 0: a wave for every run.
 template <int CODE, bool ROPE, int P> __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
@@ -549,8 +549,13 @@ extern "C" int exl_paged_append(const void* key_states, const void* value_states
                     head_dim % 16 ? 0u : by(head_dim / 16), by(head_dim / 4)};
     // passes of the wide form over a page: block tokens x head_dim / 16 threads (256 / (head_dim / 16) whole tokens at a time)
     const int step = head_dim % 16 ? 0 : 256 / (head_dim / 16), p = step ? (block_size + step - 1) / step : 0;
-    const int64_t work = (int64_t) rows * num_kv_heads;           // few rows: a run for every wave at once; many: fewer workgroups that find no run's beginning
-    a.chunk = work <= 16384 ? 4 : work <= 131072 ? 16 : 32;
+    // Token rows of a workgroup.  Few: the runs of single tokens go to many waves; many: fewer workgroups that find no run's beginning (they
+    // cost as much of the machine's registers as the others while they wait for their slots).  Measured, us, chunks of 4 / 16 / 32 / 63, head_dim 128:
+    //   256 single tokens x 8 heads 8.2 / 14.8 / 24 / 44      512 x 32: 35 / 33 / 40 / 54       256 runs of 8 x 32: 45 / 42 / 41 / 62
+    //   one prompt of 512 x 8 heads 10.1 / 7.7 / 8.1 / 7.8    2048 x 8: 17 / 12 / 9.6 / 9.4     2048 x 32: 37 / 21 / 19 / 16
+    //   8192 x 8 in pages of 128 (four passes: twice the registers) 84 / 56 / 48 / 29           30 k ragged tokens x 8: 156 / 63 / 42 / 39
+    const int64_t work = (int64_t) rows * num_kv_heads;
+    a.chunk = work <= 12000 ? 4 : work <= 24000 ? 16 : work <= 131072 && p < 4 ? 32 : 63;
     const int64_t groups = ((int64_t) rows + a.chunk - 1) / a.chunk * num_kv_heads;
     EXL_REQUIRE(groups <= 0x7fffffff, EXL_E_UNSUPPORTED, "paged_append: too many rows for %d kv heads", num_kv_heads);
     const dim3 grid((unsigned) groups);

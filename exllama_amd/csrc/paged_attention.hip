@@ -576,7 +576,7 @@ __device__ __forceinline__ PmFound pm_find(const PagedAttn& a, const PaCut& cut,
         for (int u = 0; u < wave; ++u) base += sums[u];
         if (w >= base && w < base + here) {
             const int k = (int) (w - base), t = k / np, half = (z.q + 1) / 2;
-            const bool fold = !first && cost <= (int64_t) cut.target * z.keys;        // (as many tiles as fit at once, or fewer)
+            const bool fold = !first && cost <= 2 * (int64_t) cut.target * z.keys;     // (as many tiles as fit at once, or fewer: a compute unit holds two)
             found.item = {b, fold && t >= half ? t - half : z.q - 1 - t, k % np, np};
             found.row = pa_row(a, b);
         }
@@ -875,46 +875,58 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     }
 }
 
-// The pieces of a query tile joined, in order: 16 lanes for a query, 32 queries of an item for a workgroup (most of which find nothing to do).
+// The pieces of a query tile joined, in order: 16 lanes for a query, 16 queries of an item for a workgroup (most of which find nothing to do).
 template <int DP> __global__ __launch_bounds__(256) void paged_attn_join_many_kernel(PagedAttn a, const float* __restrict__ parts, const PmItem* __restrict__ items)
 {
-    constexpr int V = DP / 64;                                    // groups of four columns of a lane
+    constexpr int V = DP / 64, U = DP <= 128 ? 4 : 2;             // groups of four columns of a lane; pieces in flight
     const int w = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x & 15;
     const PmItem it = items[w];
     if (it.row < 0 || it.piece != 0 || it.pieces < 2) return;
     const PaRow row = pa_row(a, it.row);
-    const int group = a.heads / a.kv_heads;
+    const int group = a.heads / a.kv_heads, q = blockIdx.z * 16 + (threadIdx.x >> 4);
     const size_t step = (size_t) a.kv_heads * PM_ROWS * (DP + 4);
+    const int64_t r = (int64_t) it.tile * PM_ROWS + q;
+    if (r >= (int64_t) row.fresh * group) return;
+    const float* p0 = parts + (((size_t) w * a.kv_heads + kvh) * PM_ROWS + q) * (DP + 4);
+    float m = -INFINITY, sum = 0.f;
+    f32x4 o[V] = {};
+    for (int k0 = 0; k0 < it.pieces; k0 += U) {
+        float pm[U], pl[U];
+        f32x4 po[U][V];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int q = blockIdx.z * 32 + u * 16 + (threadIdx.x >> 4);
-        const int64_t r = (int64_t) it.tile * PM_ROWS + q;
-        if (r >= (int64_t) row.fresh * group) return;
-        const float* p0 = parts + (((size_t) w * a.kv_heads + kvh) * PM_ROWS + q) * (DP + 4);
-        float top = -INFINITY;
-        for (int k = lane; k < it.pieces; k += 16) top = fmaxf(top, p0[k * step + DP]);
+        for (int u = 0; u < U; ++u) {
+            const float* p = p0 + min(k0 + u, it.pieces - 1) * step;
+            pm[u] = k0 + u < it.pieces ? p[DP] : -INFINITY;
+            pl[u] = p[DP + 1];
 #pragma unroll
-        for (int off = 8; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 16));
-        float sum = 0.f;
-        f32x4 o[V] = {};
-#pragma unroll 2
-        for (int k = 0; k < it.pieces; ++k) {
-            const float* p = p0 + k * step;
-            const float m = p[DP], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-            sum += f * p[DP + 1];
-#pragma unroll
-            for (int j = 0; j < V; ++j) o[j] += f * *(const f32x4*) (p + 64 * j + 4 * lane);
+            for (int j = 0; j < V; ++j) po[u][j] = *(const f32x4*) (p + 64 * j + 4 * lane);
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        f16* out = a.out + (size_t) (row.start + (int) (r / group)) * a.heads * a.hd + (size_t) (kvh * group + (int) (r % group)) * a.hd;
+        float top = m;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int d = 64 * j + 4 * lane;
-            f16x4 x;
+        for (int u = 0; u < U; ++u) top = fmaxf(top, pm[u]);
+        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        sum *= keep;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = (f16) (o[j][e] * inv);
-            if (d < a.hd) *(f16x4*) (out + d) = x;                  // (head_dim is a multiple of four)
+        for (int j = 0; j < V; ++j) o[j] *= keep;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 + u >= it.pieces) break;
+            const float f = pm[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm[u] - top);
+            sum += f * pl[u];
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] += f * po[u][j];
         }
+        m = top;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    f16* out = a.out + (size_t) (row.start + (int) (r / group)) * a.heads * a.hd + (size_t) (kvh * group + (int) (r % group)) * a.hd;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int d = 64 * j + 4 * lane;
+        f16x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (f16) (o[j][e] * inv);
+        if (d < a.hd) *(f16x4*) (out + d) = x;                    // (head_dim is a multiple of four)
     }
 }
 
@@ -933,14 +945,14 @@ static PaPlan pa_plan(int n, int rows, int max_new, int heads, int kv_heads, int
     p.rows_y = (int) queries;
     if (!p.many) {
         const int waves = 1024 * (p.dp * p.nt <= 128 ? 2 : 1);     // of the whole machine
-        p.cut = {kv_heads >= waves ? 1 : waves / kv_heads, 2};
+        p.cut = {kv_heads >= waves ? 1 : waves / kv_heads, 1};
         p.split = true;
         p.items = p.parts = p.cut.target;
         p.item_bytes = pa_round((size_t) n * sizeof(int2));
         p.part_bytes = pa_round((size_t) p.parts * kv_heads * 2 * pa_part_floats(p.dp, p.nt) * sizeof(float));
     } else {
         const int64_t fresh = (int64_t) n * max_new < rows ? (int64_t) n * max_new : rows, tiles = (fresh * p.group + PM_ROWS - 1) / PM_ROWS + n;
-        p.cut = {kv_heads >= 512 ? 1 : 512 / kv_heads, 8};
+        p.cut = {kv_heads >= 256 ? 1 : 256 / kv_heads, 8};
         p.split = longest > p.cut.min_piece * PA_KEYS;
         p.parts = p.split ? 2 * p.cut.target : 0;
         p.items = (int) (tiles + p.parts < 0x7fffffff ? tiles + p.parts : 0x7fffffff);
@@ -980,7 +992,7 @@ template <int CODE> static int pa_launch(const PagedAttn& a, const PaPlan& p, vo
 #undef PA_MANY
     EXL_LAUNCH_CHECK();
     if (p.split) {
-        const dim3 jgrid((unsigned) p.parts, (unsigned) a.kv_heads, PM_ROWS / 32);
+        const dim3 jgrid((unsigned) p.parts, (unsigned) a.kv_heads, PM_ROWS / 16);
         if (p.dp == 64)       hipLaunchKernelGGL((paged_attn_join_many_kernel<64>), jgrid, dim3(256), 0, s, a, parts, list);
         else if (p.dp == 128) hipLaunchKernelGGL((paged_attn_join_many_kernel<128>), jgrid, dim3(256), 0, s, a, parts, list);
         else                  hipLaunchKernelGGL((paged_attn_join_many_kernel<256>), jgrid, dim3(256), 0, s, a, parts, list);
