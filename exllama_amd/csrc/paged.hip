@@ -10,7 +10,9 @@
 //   new < 0: the row has ended; its blocks go to the ring's end in order, its table entries become -1
 // Then every token row's slot = table[pos / block] * block + pos % block.  Latency is all that matters (a step of 256 rows moves
 // 7 KB): one workgroup does both halves where the work is small, otherwise the scan runs in one workgroup and the filling in
-// many -- a second launch instead of a grid-wide wait.
+// many -- a second launch instead of a grid-wide wait.  Measured, us, one workgroup / scan + filling and
+// another launch: one row 3.0 / 2.8 + 1.6, 64 rows of 64 tokens 3.9 / 3.4 + 3.1, 256 rows 7.0 / 3.5 + 2.5, 512 rows (the limit) 9.2 / 5.2 + 3.5;
+// 2048 prompts of 300 k tokens 8.1 + 5.5 (2.4 MB of slots and positions).
 struct SlotRow { int start, take, past, kept, held, base, back, gone; };      // 32 bytes a row
 
 struct SlotArgs {
@@ -21,7 +23,7 @@ struct SlotArgs {
 
 #define SLOT_THREADS 1024
 #define SLOT_WAVES (SLOT_THREADS / 64)
-#define SLOT_SMALL_ROWS 1024                                      // rows and token rows up to which one workgroup does it all
+#define SLOT_SMALL_ROWS 512                                       // rows and token rows up to which one workgroup does it all
 #define SLOT_SMALL_TOKENS 4096
 
 // exclusive prefix sum over the workgroup, and the total; `lds`: SLOT_WAVES entries.  Up to 64 rows only the first wave has numbers: no barrier.
@@ -232,9 +234,13 @@ int paged_check_block(const char* what, int block_size, int num_blocks)
 // A RUN is the longest stretch of token rows whose slots are consecutive inside one page.  Per run and kv head, keys and values each:
 //   amax = max |x| (x clamped to +-top * 2^hi, NaN left out), e = the least exponent with amax <= top * 2^e; a run that does not start
 //   its page keeps the page's earlier tokens: e = max(e, the page's), their codes move by 2^(e_old - e);  code = round(x / 2^e)
-// Keys are rotated first when sin / cos are given; the code is one rounding of the exact rotation.  Short runs (single tokens, a few drafted ones) take a wave each; from APPEND_LONG tokens on, and
-// head_dim % 16 == 0, the whole workgroup takes the run: every number is read once and stays in registers between the maximum and the
-// rounding, and the values' codes are transposed in LDS.
+// Keys are rotated first when sin / cos are given; the code is one rounding of the exact rotation.  Short runs (single tokens, a few drafted
+// ones) take a wave each; from APPEND_LONG tokens on, and head_dim % 16 == 0, the whole workgroup takes the run: every number is read once and
+// stays in registers between the maximum and the rounding, and the values' codes are transposed in LDS.  (APPEND_LONG 4 / 8 / 32: 300 runs of 6
+// tokens x 8 heads 19 / 16 / 16 us, 128 of 16 13 / 15 / 22, 30 k ragged tokens 42 / 42 / 53.)
+// Bound by HBM for long runs (30 k ragged int8 tokens x 8 heads, 188 MB: 39 us = 4.8 TB/s; a prompt of 2048 x 32 heads with rotation, 51 MB: 18.8 us =
+// 2.7 TB/s, one round of workgroups), by latency for few (64 tokens x 8 heads: 5.6 us), by the values' columns for many single tokens (1024 x 32
+// heads 93 us: a token's value touches every line of its 8 KB page, which attention reads in whole lines for it).
 struct AppendArgs {
     const f16* k; const f16* v; const int32_t* slots; const int32_t* positions; const f16* sin; const f16* cos;
     uint8_t* kp; uint8_t* vp; float* ks; float* vs;

@@ -1,5 +1,11 @@
 // Attention over the paged 8-bit cache (paged.h).
 //   o[t, h] = sum_j p_j V[j] / sum_j p_j,   p_j = exp(s_j - max s),   s_j = scale * rope(q[t, h]) . K[j],   j <= past + i, j < past + new
+// Two forms, told apart by what the host knows, the most queries that a row has for one kv head (max_new * heads / kv_heads): up to 32 (head_dim over
+// 128: 16) the cache's bytes bound the work, above it the products do.  Measured (us, few / many; 32 queries a row, head_dim 128): 16 rows of 4000 keys
+// 51 / 68, one of 16000 30 / 40, 96 ragged ones 49 / 66, 8 of 300 19 / 17.
+// Rounding: codes * scale are fp16 numbers exactly (448 * 2^7, 127 * 2^9); weights are rounded to fp16 (2^-11 of each, relative to a reference that
+// lies at most 2^8 below the largest); sums, maxima and the softmax's denominator are 32 bits; a rotated query is an fp16 number and its
+// rest, also fp16 (2^-22) -- but for head_dim over 128 in the form for many queries; the result is rounded to fp16 once.
 #include "paged.h"
 #include <type_traits>
 
@@ -25,10 +31,14 @@ __device__ __forceinline__ PaRow pa_row(const PagedAttn& a, int b)
 
 // ---- rows of few queries: the cache's bytes are all that counts ------------------------------------------------------------------------
 // The tiles of 64 keys of all rows lie in one line, row behind row (each with PA_BEGIN places before it, for what beginning a row costs), and
-// every wave takes an equal stretch of it for one kv head: whatever the rows' lengths, all waves end together, none waits for another, and the next row's first tile is on its way while the last one's last is worked on.
+// every wave takes an equal stretch of it for one kv head: whatever the rows' lengths, all waves end together, none waits for another, and the
+// next row's first tile is on its way while the last one's last is worked on.
 // A wave does all queries of its row that read the kv head (up to 16 * NT: tokens * heads of the group, GQA reads the cache once).  A row
 // that lies in one stretch is written; the others leave one partial result for each stretch, joined in order by a second kernel -- the cut
 // depends on the lengths alone, so results do not depend on scheduling.
+// Bound by HBM: 8 rows of 65536 keys x 8 kv heads x 128 (1.07 GB) 201 us = 5.3 TB/s, 96 rows of 0 .. 16384 (434 MB) 93 us = 4.7 TB/s; one row of 2048 keys
+// x 32 heads (16.8 MB) is latency: 9 us, and 4 us for the joining kernel.
+// PA_BEGIN, measured 0 / 2 / 4: 96 ragged rows 134 / 104 / 105 us, five rows of four tokens 22 / 17 / 16, 96 equal rows 99 / 99 / 103.
 // Both products are MFMAs on fp16 numbers converted from the codes in registers; nothing goes through LDS:
 //   S^T = K Q^T   (16x16x32): A = keys.  MFMA row m of product t4 is key 16 * (m >> 2) + 4 * t4 + (m & 3) of the tile, so that a lane (query
 //                 column c = lane & 15, group g = lane >> 4) gets the 16 scores of keys 16 g .. 16 g + 15, in order, over the four products;
@@ -190,8 +200,8 @@ __device__ __forceinline__ PaStretch pa_stretch(const PagedAttn& a, const PaCut&
 // A partial result: [queries][DP + 4] floats (o, then m and l); a stretch has room for two: of the row that it continues, and of the one that goes on
 __host__ __device__ constexpr size_t pa_part_floats(int dp, int nt) { return (size_t) 16 * nt * (dp + 4); }
 
-// Registers (DP = 128, NT = 1): 64 for a tile's bytes, twice (the next tile is on its way while one is worked on), 32 of O, 32 of Q: two waves per
-// SIMD.  Twice the queries take one wave per SIMD, and so do wider heads, without the second set of bytes.
+// Registers (DP = 128, NT = 1): 64 for a tile's bytes, twice (the next tile is on its way while one is worked on), 32 of O, 32 of Q (241 in all):
+// two waves per SIMD.  Twice the queries take one wave per SIMD, and so do wider heads, without the second set of bytes.
 template <int CODE, int DP, int NT>
 __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_attn_few_kernel(PagedAttn a, PaCut cut, float* __restrict__ parts,
                                                                                             int2* __restrict__ firsts)
@@ -445,6 +455,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
 
 // The parts of a row joined: `each` (1, 2, 4, ...) queries of one row and kv head for a workgroup, dp / 4 lanes for a query; the lanes that are
 // left take every so many-th part each, with a maximum of their own, and meet in LDS -- in an order that depends on the lengths alone.
+// 4 us for a few rows (a launch and three rounds of loads), 9 us for 96 ragged rows x 64 heads (12 MB of parts).
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const float* __restrict__ parts, const int2* __restrict__ firsts, int dp, int nt, int each, int target)
 {
     __shared__ f32x4 slice_o[256];
@@ -519,6 +530,10 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const
 //   S^T = K Q^T (32x32x16): row m of the product is key 16 * ((m >> 2) & 1) + 4 * (m >> 3) + (m & 3) of a half tile, so that a lane (query
 //   column c = lane & 31, group g = lane >> 5) gets keys 16 g .. 16 g + 15 in order;   O^T = V^T P^T: the lane's own weights are the operand.
 // LDS pieces of 16 bytes are laid out by XOR so that neither the writes (one key, all columns) nor the reads (linear) meet in a bank.
+// Bound by the sum of MFMA and VALU time (conversion, exp2, masks), which two workgroups a compute unit do not hide behind each other.
+// LOW, head_dim up to 128: the rest of a rotated query is multiplied too -- half as many MFMAs again: a prompt of 2048 x 32 heads (34 GFLOP causal)
+// takes 77 us instead of 66, pieces of a 70B prompt (411 GFLOP) 622 instead of 503; without it the result is 3.9e-4 of its norm off, with it
+// 2.6e-4 (2.0e-4 are its own rounding).  Wider heads have no registers for it (spilled: 127 -> 213 us).
 #define PM_ROWS 128
 
 // A tile of queries and a piece of its keys (all tiles of a row are cut in the same number of `pieces`)
@@ -526,8 +541,8 @@ struct PmItem { int row, tile, piece, pieces; };
 struct PmFound { PmItem item; PaRow row; };                       // (the row as one thread read it: all waves walk the same tiles whatever happens to the lengths meanwhile)
 
 // Item `w` of the launch; row < 0: none.  The cost of a row is tiles of queries * tiles of keys; with `piece` = a `target`-th of all rows' cost
-// (or min_piece), rows of 1.5 times as many keys or more are cut into pieces of about that size -- 4 / 3 * target items at most, and these come first: an item's number is its place
-// among the partial results.  Tiles of a row come with the last (the longest) first; where every item of the launch is resident at once, the
+// (or min_piece), rows of 1.5 times as many keys or more are cut into pieces of about that size -- 4 / 3 * target items at most, and these come
+// first: an item's number is its place among the partial results.  Tiles of a row come with the last (the longest) first; where every item of the launch is resident at once, the
 // second half comes shortest first: the two workgroups of a compute unit, half a launch apart, then have equal work together.
 // lds: 96 bytes, free again afterwards.
 __device__ __forceinline__ PmFound pm_find(const PagedAttn& a, const PaCut& cut, int w, void* lds)
@@ -589,8 +604,8 @@ __device__ __forceinline__ PmFound pm_find(const PagedAttn& a, const PaCut& cut,
     return it;
 }
 
-// WIDE: pages of 64 or 128 tokens, a tile lies in one: its page is looked up once, in scalar registers.
-template <int CODE, int DP, bool WIDE>
+// WIDE: pages of 64 or 128 tokens, a tile lies in one: its page is looked up once, in scalar registers (pieces of a 70B prompt 651 -> 617 us).
+template <int CODE, int DP, bool WIDE, bool LOW>
 __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_many_kernel(PagedAttn a, PaCut cut, float* __restrict__ parts,
                                                                                         PmItem* __restrict__ items, int part_items)
 {
@@ -605,7 +620,8 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, g = lane >> 5;
     if (tid < 2) nan_tile[tid] = -1;                              // (pm_find has barriers)
     const PmFound found = pm_find(a, cut, w, lds);
-    const PmItem it = found.item;
+    const PmItem it = {__builtin_amdgcn_readfirstlane(found.item.row), __builtin_amdgcn_readfirstlane(found.item.tile), __builtin_amdgcn_readfirstlane(found.item.piece),
+                       __builtin_amdgcn_readfirstlane(found.item.pieces)};
     if (kvh == 0 && tid == 0 && w < part_items) items[w] = it;                   // for the joining kernel
     if (it.row < 0) return;
     const PaRow row = {__builtin_amdgcn_readfirstlane(found.row.start), __builtin_amdgcn_readfirstlane(found.row.fresh), __builtin_amdgcn_readfirstlane(found.row.past),
@@ -614,8 +630,8 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     const int64_t queries = (int64_t) row.fresh * group, q0 = (int64_t) it.tile * PM_ROWS;
     const int last_token = (int) ((min(q0 + PM_ROWS, queries) - 1) / group);
     const int all_tiles = (int) ((min((int64_t) row.past + last_token + 1, (int64_t) row.keys) + PA_KEYS - 1) / PA_KEYS);
-    const int t_first = __builtin_amdgcn_readfirstlane((int) ((int64_t) all_tiles * it.piece / it.pieces));
-    const int t_last = __builtin_amdgcn_readfirstlane((int) ((int64_t) all_tiles * (it.piece + 1) / it.pieces));
+    const int t_first = (int) ((int64_t) all_tiles * it.piece / it.pieces);
+    const int t_last = (int) ((int64_t) all_tiles * (it.piece + 1) / it.pieces);
 
     // this lane's query
     const int64_t r = q0 + wave * 32 + c;
@@ -626,9 +642,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     const int64_t wave_q0 = q0 + wave * 32;
     const int wave_free = wave_q0 < queries ? (int) min((int64_t) row.past + (int) (wave_q0 / group), (int64_t) row.keys - 1) : -1;
     const int wave_end = wave_q0 < queries ? (int) min((int64_t) row.past + (int) ((min(wave_q0 + 32, queries) - 1) / group), (int64_t) row.keys - 1) : -1;
-    // a rotated query is rounded to fp16 here, once.  Its rest costs as many products again as the scores themselves: with it, prompts take 20 %
-    // longer (67 -> 80 us, 538 -> 656 us) and the result's error falls from 3.6e-4 to 2.4e-4 of its norm (2.0e-4 are the output's own rounding)
-    f16x8 qf[KB];
+    f16x8 qf[KB], ql[KB];                                         // the query and what fp16 leaves of it after a rotation
     {
         const f16* q = a.q + (size_t) (row.start + token) * a.q_stride + (size_t) head * a.hd;
 #pragma unroll
@@ -636,10 +650,11 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
             PaQuery x = pa_query(a, q, (int64_t) row.past + token, 16 * kb + 8 * g);
             if (!in) x = {};
             qf[kb] = x.hi;
+            ql[kb] = x.lo;
         }
     }
 
-    const int32_t* table = a.table + (size_t) __builtin_amdgcn_readfirstlane(it.row) * a.width;
+    const int32_t* table = a.table + (size_t) it.row * a.width;
     const size_t page_bytes = (size_t) a.block * a.hd16;
     // staging roles: keys: piece i of this thread is column chunk k_ch of key k_key + (256 / KB) * i; values: 16 keys v_kc of column v_d + 64 * i
     const int k_ch = tid % KB, k_key = tid / KB, v_kc = tid & 3, v_d = tid >> 2;
@@ -787,7 +802,9 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
             for (int kb = 0; kb < KB; ++kb) {
                 const f16x8 k = *(const f16x8*) (buf + (kt * KB + kb) * 1024 + ((lane ^ (kb & 7)) << 4));
                 s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[kb], s[kt], 0, 0, 0);
+                if (LOW) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[kb], s[kt], 0, 0, 0);
             }
+            if (LOW) __builtin_amdgcn_sched_barrier(0);           // (fewer pieces of keys in flight: the query's second half takes their registers)
         }
         float mx = -INFINITY;
         if (__builtin_amdgcn_readfirstlane(border)) {
@@ -875,7 +892,8 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     }
 }
 
-// The pieces of a query tile joined, in order: 16 lanes for a query, 16 queries of an item for a workgroup (most of which find nothing to do).
+// The pieces of a query tile joined, in order: 16 lanes for a query, 16 queries of an item for a workgroup (most of which find nothing to do:
+// 4.5 us where no row is cut).  Four parts in flight: one at a time 100 queries x 32 heads took 21 us for six parts each.
 template <int DP> __global__ __launch_bounds__(256) void paged_attn_join_many_kernel(PagedAttn a, const float* __restrict__ parts, const PmItem* __restrict__ items)
 {
     constexpr int V = DP / 64, U = DP <= 128 ? 4 : 2;             // groups of four columns of a lane; pieces in flight
@@ -944,7 +962,9 @@ static PaPlan pa_plan(int n, int rows, int max_new, int heads, int kv_heads, int
     p.nt = queries <= 16 ? 1 : 2;
     p.rows_y = (int) queries;
     if (!p.many) {
-        const int waves = 1024 * (p.dp * p.nt <= 128 ? 2 : 1);     // of the whole machine
+        // All waves that the machine holds at once.  Half / all / twice as many: 96 ragged rows 108 / 104 / 110 us, 32 queries a row 69 / 53 / 65.
+        // Stretches of at least one tile: 1 / 2 / 4: one row of 2048 keys 12.8 / 14.8 / 18.9 us
+        const int waves = 1024 * (p.dp * p.nt <= 128 ? 2 : 1);
         p.cut = {kv_heads >= waves ? 1 : waves / kv_heads, 1};
         p.split = true;
         p.items = p.parts = p.cut.target;
@@ -952,6 +972,8 @@ static PaPlan pa_plan(int n, int rows, int max_new, int heads, int kv_heads, int
         p.part_bytes = pa_round((size_t) p.parts * kv_heads * 2 * pa_part_floats(p.dp, p.nt) * sizeof(float));
     } else {
         const int64_t fresh = (int64_t) n * max_new < rows ? (int64_t) n * max_new : rows, tiles = (fresh * p.group + PM_ROWS - 1) / PM_ROWS + n;
+        // A workgroup for every compute unit, pieces of 8 tiles or more.  128 / 256 / 512 workgroups: 100 tokens x 32 heads after 3000 43 / 41 / 49 us,
+        // x 64 heads with 8 kv heads 58 / 45 / 48.  Pieces of at least 4 / 8 / 16 tiles: 40 / 41 / 48 and 45 / 45 / 48
         p.cut = {kv_heads >= 256 ? 1 : 256 / kv_heads, 8};
         p.split = longest > p.cut.min_piece * PA_KEYS;
         p.parts = p.split ? 2 * p.cut.target : 0;
@@ -984,12 +1006,14 @@ template <int CODE> static int pa_launch(const PagedAttn& a, const PaPlan& p, vo
         return 0;
     }
     PmItem* list = (PmItem*) workspace;
-#define PA_MANY(DP, WIDE) do { static bool done[EXL_MAX_DEVICES] = {};                                                                       \
-    EXL_TRY(exl_lds_opt_in((const void*) paged_attn_many_kernel<CODE, DP, WIDE>, done));                                                      \
-    hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE>), grid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4 + 2 * DP * 8 + 8, s, a, p.cut, parts, list, p.parts); } while (0)
+#define PA_MANY_R(DP, WIDE, ROPE) do { static bool done[EXL_MAX_DEVICES] = {};                                                               \
+    EXL_TRY(exl_lds_opt_in((const void*) paged_attn_many_kernel<CODE, DP, WIDE, ROPE>, done));                                                \
+    hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE, ROPE>), grid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4 + 2 * DP * 8 + 8, s, a, p.cut, parts, list, p.parts); } while (0)
+#define PA_MANY(DP, WIDE) do { if (DP <= 128 && a.sin) PA_MANY_R(DP, WIDE, (DP <= 128)); else PA_MANY_R(DP, WIDE, false); } while (0)
     if (a.block >= PA_KEYS) { if (p.dp == 64) PA_MANY(64, true); else if (p.dp == 128) PA_MANY(128, true); else PA_MANY(256, true); }
     else                    { if (p.dp == 64) PA_MANY(64, false); else if (p.dp == 128) PA_MANY(128, false); else PA_MANY(256, false); }
 #undef PA_MANY
+#undef PA_MANY_R
     EXL_LAUNCH_CHECK();
     if (p.split) {
         const dim3 jgrid((unsigned) p.parts, (unsigned) a.kv_heads, PM_ROWS / 16);

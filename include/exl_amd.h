@@ -225,17 +225,18 @@ int exl_paged_slots(const int32_t* past_lens, const int32_t* new_lens, int32_t* 
                     int32_t* starts, int32_t* slots, int32_t* positions, int32_t* scratch, void* stream);
 /* New keys and values, fp16 rows key_states + t * key_stride (elements) of kv_heads * head_dim, into the pages at slots[t] (-1, or outside
  * the pool: skipped).  The tokens of one page stand next to each other in ascending order, as exl_paged_slots lays them; a page is
- * written through one row of the batch at a time.  A run of tokens that starts a page sets the page's scale from its largest
- * magnitude; one that continues a page keeps the earlier tokens, whose codes move to the larger of the two scales.  Each code is ONE
- * rounding (nearest even) of x / scale; NaN stays NaN (int8: 0).  sin / cos (fp16 [angle_rows, head_dim], both or neither): keys are rotated
+ * written through one row of the batch at a time, and no slot stands there twice (its code would be either token's).  A run of tokens that
+ * starts a page sets the page's scale from its largest magnitude; one that continues a page keeps the earlier tokens, whose codes move to the
+ * larger of the two scales.  Each code is ONE rounding (nearest even) of x / scale; NaN stays NaN (int8: 0).  sin / cos (fp16 [angle_rows, head_dim], both or neither): keys are rotated
  * by halves at positions[t] first (exactly; the code is one rounding of the rotated key). */
 int exl_paged_append(const void* key_states, const void* value_states, long key_stride, long value_stride, const int32_t* slots, int rows,
                      void* key_pages, void* value_pages, float* key_scales, float* value_scales, int code, int num_blocks, int num_kv_heads,
                      int block_size, int head_dim, const int32_t* positions, const void* sin, const void* cos, int angle_rows, void* stream);
 /* Attention over the pages: query row starts[b] + i (q + t * q_stride, heads * head_dim fp16; i < new_lens[b], at most max_new) sees the keys
  * j <= past_lens[b] + i of row b, j < past + new and inside the table; softmax(scale * q . k), fp32 sums, one rounding to fp16.  scale <= 0:
- * 1 / sqrt(head_dim).  sin / cos: q is rotated at its position first (fp32, rounded to fp16).  Pages outside the pool are not seen; a
- * query that sees nothing gives zeros; rows of `out` [rows, heads * head_dim] that belong to no row of the batch are left as they were.
+ * 1 / sqrt(head_dim).  sin / cos: q is rotated at its position first (to twice fp16's digits; head_dim over 128 and more than 16 queries a row
+ * and kv head: rounded to fp16).  Pages outside the pool are not seen; a query that sees nothing gives zeros, one that sees a NaN NaN, no
+ * other; rows of `out` [rows, heads * head_dim] that belong to no row of the batch are left as they were.  out must not overlap q.
  * workspace: at least exl_paged_attention_workspace(...) bytes, for this call alone until it has run. */
 size_t exl_paged_attention_workspace(int n_rows, int rows, int max_new, int num_heads, int num_kv_heads, int head_dim, int table_width, int block_size);
 int exl_paged_attention(const void* q, long q_stride, const int32_t* starts, const int32_t* past_lens, const int32_t* new_lens, int n_rows, int rows,

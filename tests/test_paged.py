@@ -161,7 +161,7 @@ def test_kernels_fit_their_registers():
 
     with tempfile.TemporaryDirectory() as d:
         res = {n: r for n, r in isa_lint.kernel_resources(path, d).items() if "paged_" in n}
-    assert sum("paged_attn_few" in n for n in res) == 10 and sum("paged_attn_many" in n for n in res) == 12 and sum("paged_append" in n for n in res) == 20
+    assert sum("paged_attn_few" in n for n in res) == 10 and sum("paged_attn_many" in n for n in res) == 20 and sum("paged_append" in n for n in res) == 20
     for n, r in res.items():
         assert r["scratch"] == 0, (n, r)
         total = r["vgpr"]                                      # (of both kinds)
