@@ -89,9 +89,28 @@ template <int CODE, bool BIG> __device__ __forceinline__ f16x8 pa_numbers(uint32
 }
 
 // A value that is NaN and that only some of a tile's queries see (a token of this call, in e4m3 pages): a weight of 0 does not hide it from the
-// others.  In tiles on the border such codes become 0 in the product with the weights, and the sums that they belong to become NaN behind it.
+// others.  In tiles on the border such codes become 0 in the product with the weights, and the sums that they belong to become NaN: few queries: by
+// two more products, of bf16's largest number at every NaN with the same number at every key that a query sees, which is infinity, and
+// with its negative (sums set by a comparison each would be copied out of the matrix cores' registers and back); many queries: behind the last tile.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ uint32_t pa_nan4(uint32_t codes) { return (((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7; }       // 1 in each byte that is NaN
 __device__ __forceinline__ uint32_t pa_bits4(uint32_t ones) { return ones * 0x10204080u >> 28; }                                        // four bytes of 0 or 1 as four bits
+__device__ __forceinline__ bf16x8 pa_holes(uint32_t lo, uint32_t hi)                                      // of eight bytes of 0 or 1
+{
+    union { uint32_t u[4]; bf16x8 v; } x;
+    lo *= 0x7f; hi *= 0x7f;
+    x.u[0] = __builtin_amdgcn_perm(0, lo, 0x01010000u); x.u[1] = __builtin_amdgcn_perm(0, lo, 0x03030202u);
+    x.u[2] = __builtin_amdgcn_perm(0, hi, 0x01010000u); x.u[3] = __builtin_amdgcn_perm(0, hi, 0x03030202u);
+    return x.v;
+}
+__device__ __forceinline__ bf16x8 pa_seen(int n, bool negative)                                           // the first n of eight
+{
+    union { uint32_t u[4]; bf16x8 v; } x;
+    const uint32_t most = negative ? 0xff7fff7fu : 0x7f7f7f7fu;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.u[i] = n >= 2 * i + 2 ? most : n == 2 * i + 1 ? most & 0xffff : 0u;
+    return x.v;
+}
 
 // Query elements d .. d + 7 of one token and head (zeros behind head_dim), rotated at `pos` when there are tables.  A rotated query is no fp16
 // number: hi is the nearest one, lo what it leaves (0 without a rotation).
@@ -316,7 +335,8 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             // the reference moves only when a score passes it by 2^8: the weights are relative to it, fp16 holds them up to 2^16
-            if (__any(mx > m[nt] + 8.f)) {
+            // (one pass at most; a loop for wide heads, whose sums lie in the matrix cores' own registers: what it copies out and back stays in it)
+            for (bool moves = __any(mx > m[nt] + 8.f); moves; moves = DP > 128 && __any(mx > m[nt] + 8.f)) {
                 const float mn = fmaxf(m[nt], mx);
                 const float keep = m[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[nt] - mn);
                 l[nt] *= keep;
@@ -335,38 +355,29 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
             }
         }
         const PaScale vs = pa_scale<CODE>(st.vs);
-        bool holes = false;
-        uint32_t hole[NT][DT > 8 ? 2 : 1];                        // a bit for each of this lane's sums, the last one lowest
         if (CODE == EXL_PAGE_FP8 && border && row.fresh > 1) {
             uint32_t nan = 0;
 #pragma unroll
             for (int t = 0; t < DT; ++t) nan |= pa_nan4(st.v[t].x) | pa_nan4(st.v[t].y) | pa_nan4(st.v[t].z) | pa_nan4(st.v[t].w);
-            holes = __any(nan);
-        }
-        if (holes) {
+            if (__any(nan)) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) for (uint32_t& x : hole[nt]) x = 0;
+                for (int t = 0; t < DT; ++t) {
+                    uint4& v = st.v[t];
+                    asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));       // (computed again, not kept from above)
+                    const uint4 n = make_uint4(pa_nan4(v.x), pa_nan4(v.y), pa_nan4(v.z), pa_nan4(v.w));
+                    v.x &= ~(n.x * 255); v.y &= ~(n.y * 255); v.z &= ~(n.z * 255); v.w &= ~(n.w * 255);
+                    const bf16x8 n0 = pa_holes(n.x, n.y), n1 = pa_holes(n.z, n.w);
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {                        // a product of 1 (the code 0x38) at every NaN with 1 at every key that a query sees
-                uint4& v = st.v[t];
-                asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));       // (computed again, not kept from above)
-                const uint4 n = make_uint4(pa_nan4(v.x), pa_nan4(v.y), pa_nan4(v.z), pa_nan4(v.w));
-                v.x &= ~(n.x * 255); v.y &= ~(n.y * 255); v.z &= ~(n.z * 255); v.w &= ~(n.w * 255);
-                const f16x8 n0 = pa_numbers<CODE, false>(n.x * 0x38, n.y * 0x38, one), n1 = pa_numbers<CODE, false>(n.z * 0x38, n.w * 0x38, one);
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    int n_seen = st.there ? limit[nt] + 1 - key0 : 0;
-                    asm volatile("" : "+v"(n_seen));
-                    f16x8 seen[2];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) seen[i >> 3][i & 7] = i < n_seen ? (f16) 1.f : (f16) 0.f;
-                    f32x4 z = {0.f, 0.f, 0.f, 0.f};
-                    z = __builtin_amdgcn_mfma_f32_16x16x32_f16(n0, seen[0], z, 0, 0, 0);
-                    z = __builtin_amdgcn_mfma_f32_16x16x32_f16(n1, seen[1], z, 0, 0, 0);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) hole[nt][t >> 3] = hole[nt][t >> 3] << 1 | (z[j] > 0.f ? 1u : 0u);
+                        for (int sign = 0; sign < 2; ++sign) {
+                            int seen = st.there ? limit[nt] + 1 - key0 : 0;
+                            asm volatile("" : "+v"(seen));
+                            o[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(n0, pa_seen(seen, sign), o[nt][t], 0, 0, 0);
+                            o[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(n1, pa_seen(seen - 8, sign), o[nt][t], 0, 0, 0);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);        // (one after the other: all at once they take too many registers)
                 }
-                __builtin_amdgcn_sched_barrier(0);                // (one after the other: all at once they take too many registers)
             }
         }
 #pragma unroll
@@ -377,14 +388,6 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
                 o[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[nt][0], o[nt][t], 0, 0, 0);
                 o[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[nt][1], o[nt][t], 0, 0, 0);
             }
-        }
-        if (holes) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int t = 0; t < DT; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) if (hole[nt][t >> 3] >> ((DT > 8 ? 31 : 4 * DT - 1) - (4 * t + j) % 32) & 1) o[nt][t][j] = NAN;
         }
     };
 
@@ -610,7 +613,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
                                                                                         PmItem* __restrict__ items, int part_items)
 {
     constexpr int KB = DP / 16, DT = DP / 32, PIECES = PA_KEYS * KB / 256;       // 16-byte pieces of codes per thread: keys, and as many of values
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // [2][keys: 2 * KB * 1024 bytes, values: 4 * DT * 1024 bytes], [2][DP] maps, 2 ints
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // [2][keys: 2 * KB * 1024 bytes, values: 4 * DT * 1024 bytes], [2][DP] maps, 2 ints, [DT][256] bits
     constexpr int K_BYTES = 2 * KB * 1024, BUF = 2 * K_BYTES;
     uint64_t* nan_map = (uint64_t*) (lds + 2 * BUF);              // by buffer, of a tile on the border: the tokens whose value is NaN, a word for each column
     int* nan_tile = (int*) (nan_map + 2 * DP);                    // by buffer: the last tile on the border that held one
@@ -618,7 +621,9 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     // values) share an XCD's L2 where kv_heads is a multiple of 8, and every XCD gets tiles of all lengths
     const int kvh = blockIdx.x % a.kv_heads, w = blockIdx.x / a.kv_heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, g = lane >> 5;
+    uint16_t* hole = (uint16_t*) (nan_tile + 2) + tid;            // [DT][256]: a bit for each of this lane's sums that is NaN
     if (tid < 2) nan_tile[tid] = -1;                              // (pm_find has barriers)
+    if (CODE == EXL_PAGE_FP8) for (int t = 0; t < DT; ++t) hole[t * 256] = 0;
     const PmFound found = pm_find(a, cut, w, lds);
     const PmItem it = {__builtin_amdgcn_readfirstlane(found.item.row), __builtin_amdgcn_readfirstlane(found.item.tile), __builtin_amdgcn_readfirstlane(found.item.piece),
                        __builtin_amdgcn_readfirstlane(found.item.pieces)};
@@ -638,10 +643,10 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     const bool in = r < queries;
     const int token = in ? (int) (r / group) : 0, head = kvh * group + (in ? (int) (r % group) : 0);
     const int limit = in ? (int) min((int64_t) row.past + token, (int64_t) row.keys - 1) : -1;
-    // the first and the last key that bound what this wave has to mask and to walk
+    // the last key that all queries of this wave see.  (A tile behind what any of them sees is worked on like the others, all masked: a short cut around
+    // it made the compiler keep the accumulators in two places and copy them in every tile.)
     const int64_t wave_q0 = q0 + wave * 32;
     const int wave_free = wave_q0 < queries ? (int) min((int64_t) row.past + (int) (wave_q0 / group), (int64_t) row.keys - 1) : -1;
-    const int wave_end = wave_q0 < queries ? (int) min((int64_t) row.past + (int) ((min(wave_q0 + 32, queries) - 1) / group), (int64_t) row.keys - 1) : -1;
     f16x8 qf[KB], ql[KB];                                         // the query and what fp16 leaves of it after a rotation
     {
         const f16* q = a.q + (size_t) (row.start + token) * a.q_stride + (size_t) head * a.hd;
@@ -772,14 +777,14 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
     Stage st;
     Ids id;
     uint32_t there = 15;
-    if (t_first < t_last) {
+    if (__builtin_expect(t_first < t_last, 1)) {
         fetch(t_first, look(t_first), st);
         there = st.there;
         store(t_first, st);
         if (t_first + 1 < t_last) fetch(t_first + 1, look(t_first + 1), st);
         if (t_first + 2 < t_last) id = look(t_first + 2);
     }
-    for (int tile = t_first; tile < t_last; ++tile) {
+    if (__builtin_expect(t_first < t_last, 1)) for (int tile = t_first; ; ) {
         unsigned char* buf = lds + ((tile - t_first) & 1) * BUF;
         const uint32_t now = there;
         __syncthreads();                                          // this tile is in `buf`, and every wave is through with the other one
@@ -791,7 +796,6 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
                 if (tile + 3 < t_last) id = look(tile + 3);
             }
         }
-        if (tile * PA_KEYS > wave_end) continue;
         const bool border = tile * PA_KEYS + PA_KEYS - 1 > wave_free || now != 15;
         f32x16 s[2];
 #pragma unroll
@@ -821,7 +825,8 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
             for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[kt][j]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c1;
         // the reference moves only when a score passes it by 2^8: the weights are relative to it, fp16 holds them up to 2^16
-        if (__any(mx > m + 8.f)) {
+        // (one pass at most; a loop for wide heads, whose sums lie in the matrix cores' own registers: what it copies out and back stays in it)
+        for (bool moves = __any(mx > m + 8.f); moves; moves = DP > 128 && __any(mx > m + 8.f)) {
             const float mn = fmaxf(m, mx);
             const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             l *= keep;
@@ -857,17 +862,31 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
                 const int n = now >> u & 1 ? min(max(limit - (tile * PA_KEYS + 16 * u) + 1, 0), 16) : 0;
                 seen |= (uint64_t) ((1u << n) - 1) << (16 * u);
             }
-            const uint64_t* map = nan_map + ((tile - t_first) & 1) * DP;
+            const uint64_t* map = nan_map + ((tile - t_first) & 1) * DP + 4 * g;
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
+            for (int t = 0; t < DT; ++t) {
+                uint32_t bits = 0;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) if (map[32 * t + 8 * (j >> 2) + 4 * g + (j & 3)] & seen) o[t][j] = NAN;
+                for (int j = 0; j < 16; ++j) bits = bits << 1 | ((map[32 * t + 8 * (j >> 2) + (j & 3)] & seen) ? 1u : 0u);
+                hole[t * 256] |= (uint16_t) bits;
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
+        if (++tile >= t_last) break;
     }
 
     // ---- out: row j of a product is column 32 t + 8 * (j >> 2) + 4 g + (j & 3)
     l += __shfl_xor(l, 32, 64);
     if (!in) return;
+    if (CODE == EXL_PAGE_FP8) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            const uint32_t bits = hole[t * 256];
+            if (bits)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) if (bits >> (15 - j) & 1) o[t][j] = NAN;
+        }
+    }
     if (it.pieces == 1) {
         f16* out = a.out + (size_t) (row.start + token) * a.heads * a.hd + (size_t) head * a.hd;
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -1008,7 +1027,7 @@ template <int CODE> static int pa_launch(const PagedAttn& a, const PaPlan& p, vo
     PmItem* list = (PmItem*) workspace;
 #define PA_MANY_R(DP, WIDE, ROPE) do { static bool done[EXL_MAX_DEVICES] = {};                                                               \
     EXL_TRY(exl_lds_opt_in((const void*) paged_attn_many_kernel<CODE, DP, WIDE, ROPE>, done));                                                \
-    hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE, ROPE>), grid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4 + 2 * DP * 8 + 8, s, a, p.cut, parts, list, p.parts); } while (0)
+    hipLaunchKernelGGL((paged_attn_many_kernel<CODE, DP, WIDE, ROPE>), grid, dim3(PA_WAVES * 64), 2 * PA_KEYS * DP * 4 + 2 * DP * 8 + 8 + DP / 32 * 512, s, a, p.cut, parts, list, p.parts); } while (0)
 #define PA_MANY(DP, WIDE) do { if (DP <= 128 && a.sin) PA_MANY_R(DP, WIDE, (DP <= 128)); else PA_MANY_R(DP, WIDE, false); } while (0)
     if (a.block >= PA_KEYS) { if (p.dp == 64) PA_MANY(64, true); else if (p.dp == 128) PA_MANY(128, true); else PA_MANY(256, true); }
     else                    { if (p.dp == 64) PA_MANY(64, false); else if (p.dp == 128) PA_MANY(128, false); else PA_MANY(256, false); }

@@ -598,9 +598,8 @@ class ExLlamaPagedCache:
         for d in self._dev.values():
             d["past"].copy_(torch.tensor(self.seq_lens, dtype=torch.int32))
 
-    def begin(self, new_lens, q_len):
-        """Blocks, slots and positions of a pass that brings new_lens[b] tokens to row b, token rows b * q_len ..; used by ExLlama.forward."""
-        new_lens = [int(n) for n in new_lens]
+    def blocks_for(self, new_lens, q_len):
+        """The blocks that each row will hold with new_lens[b] tokens more, or a refusal; nothing changes."""
         if len(new_lens) != self.batch_size or any(not 0 <= n <= q_len for n in new_lens):
             raise RuntimeError(f"row_lens must give each of the {self.batch_size} rows 0 .. {q_len} tokens")
         need = []
@@ -610,6 +609,12 @@ class ExLlamaPagedCache:
             need.append(max(held, -(-(past + n) // self.block_size)))
         if sum(need) - sum(self._held) > self._free:
             raise RuntimeError(f"ExLlamaPagedCache: {sum(need) - sum(self._held)} more blocks are needed, {self._free} of {self.num_blocks} are free: release rows")
+        return need
+
+    def begin(self, new_lens, q_len):
+        """Blocks, slots and positions of a pass that brings new_lens[b] tokens to row b, token rows b * q_len ..; used by ExLlama.forward."""
+        new_lens = [int(n) for n in new_lens]
+        need = self.blocks_for(new_lens, q_len)
         self._free -= sum(need) - sum(self._held)
         self._held = need
         for dev, d in self._dev.items():
@@ -912,8 +917,7 @@ class ExLlama:
         if bsz != cache.batch_size:
             raise RuntimeError(f"input_ids has {bsz} rows, the cache {cache.batch_size}")
         row_lens = [q_len] * bsz if row_lens is None else [int(n) for n in row_lens]
-        if len(row_lens) != bsz or any(not 0 <= n <= q_len for n in row_lens):
-            raise RuntimeError(f"row_lens must give each of the {bsz} rows 0 .. {q_len} tokens")
+        cache.blocks_for(row_lens, q_len)                         # (refused before the first of several chunks, not between them)
         if output_device is None:
             output_device = input_ids.device
         chunk_cap = max(1, cfg.max_input_len // bsz)

@@ -166,3 +166,21 @@ def test_refusals():
         cache.release(2)
     assert cache.seq_lens == [0, 0]
     model.free_unmanaged()
+
+
+def test_a_pass_in_chunks_is_refused_before_its_first_chunk():
+    """max_input_len cuts the pass; what the pool or the rows cannot hold as a whole changes nothing."""
+    from exllama_amd.model import ExLlamaPagedCache
+    dims = synth.LLAMA_TINY_HD128
+    model = _model(dims, max_input_len=32)
+    cache = ExLlamaPagedCache(model, batch_size=2, block_size=16, num_blocks=6, max_seq_len=100)
+    ids = _ids(dims, 2, 120, seed=6)
+    model.forward(ids[:, :10], cache, preprocess_only=True)
+    state = {k: v.clone() for k, v in cache._dev["cuda:0"].items()}
+    for n, match in ((80, "release rows"), (120, "exceeds the cache length")):
+        with pytest.raises(RuntimeError, match=match):
+            model.forward(ids[:, :n], cache)
+        assert cache.seq_lens == [10, 10] and cache._held == [1, 1] and cache._free == 4
+        assert all(torch.equal(v, state[k]) for k, v in cache._dev["cuda:0"].items())
+    assert model.forward(ids[:, :38], cache).shape == (2, 1, dims.vocab_size) and cache.seq_lens == [48, 48] and cache._free == 0
+    model.free_unmanaged()
