@@ -113,7 +113,8 @@ __device__ __forceinline__ bf16x8 pa_seen(int n, bool negative)                 
 }
 
 // Query elements d .. d + 7 of one token and head (zeros behind head_dim), rotated at `pos` when there are tables.  A rotated query is no fp16
-// number: hi is the nearest one, lo what it leaves (0 without a rotation).
+// number, and up to sqrt(2) times as large as the largest: it is taken by halves (exact, the scores are doubled: pa_c1); hi is the nearest fp16
+// number, lo what it leaves (0 without a rotation).
 struct PaQuery { f16x8 hi, lo; };
 __device__ __forceinline__ PaQuery pa_query(const PagedAttn& a, const f16* q, int64_t pos, int d)
 {
@@ -125,7 +126,7 @@ __device__ __forceinline__ PaQuery pa_query(const PagedAttn& a, const f16* q, in
         const size_t at = (size_t) (pos < a.angle_rows ? pos : a.angle_rows - 1) * a.hd;
         sin = a.sin + at; cos = a.cos + at;
     }
-    auto put = [&](int i, float x) { r.hi[i] = (f16) x; r.lo[i] = (f16) (x - (float) r.hi[i]); };
+    auto put = [&](int i, float x) { x *= 0.5f; r.hi[i] = (f16) x; r.lo[i] = (f16) (x - (float) r.hi[i]); };
     if (a.hd % 16 == 0) {
         r.hi = *(const f16x8_a8*) (q + d);
         if (sin) {
@@ -149,10 +150,16 @@ __device__ __forceinline__ PaQuery pa_query(const PagedAttn& a, const f16* q, in
             else for (int i = 0; i < 4; ++i) o[i] = q[e + i < half ? e + i + half : e + i - half];
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) put(u + i, sin ? fmaf((float) x[i], (float) co[i], (e + i < half ? -(float) o[i] : (float) o[i]) * (float) si[i]) : (float) x[i]);
+        for (int i = 0; i < 4; ++i) {
+            if (sin) put(u + i, fmaf((float) x[i], (float) co[i], (e + i < half ? -(float) o[i] : (float) o[i]) * (float) si[i]));
+            else r.hi[u + i] = x[i];
+        }
     }
     return r;
 }
+
+// What a product of query and key is multiplied by: scores in powers of two
+__device__ __forceinline__ float pa_c1(const PagedAttn& a) { return a.scale * (a.sin ? 2 * 1.44269504f : 1.44269504f); }
 
 // How the work is cut: few queries: `target` waves for a kv head, no stretch of less than `min_piece` tiles; many queries: pm_find below
 struct PaCut { int target, min_piece; };
@@ -255,7 +262,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
         st.there = vok;
     };
 
-    const float c1 = a.scale * 1.44269504f;                       // scores in powers of two
+    const float c1 = pa_c1(a);
     const PaScale one = pa_scale<CODE>(1.f);
     f16x8 qf[NT][KS][2], ql[NT][KS][2];                          // the query and what fp16 leaves of it: the matrix cores have time for both
     int limit[NT];                                               // the last key this lane's query sees
@@ -772,7 +779,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[t][j] = 0.f;
     float m = -INFINITY, l = 0.f;
-    const float c1 = a.scale * 1.44269504f;
+    const float c1 = pa_c1(a);
 
     Stage st;
     Ids id;

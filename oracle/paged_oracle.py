@@ -96,14 +96,22 @@ def append(k, v, slot, key_codes, value_codes, key_scales, value_scales, code, p
         t += n
 
 
-def attention(q, starts, past, new, table, key_codes, value_codes, key_scales, value_scales, max_new, scale=None, sin=None, cos=None):
+def attention(q, starts, past, new, table, key_codes, value_codes, key_scales, value_scales, max_new, scale=None, sin=None, cos=None, sharp=None):
     """q [rows, heads, hd]; returns (out, bound): the rows that belong to no row of the batch are NaN in both.
 
     bound: how far a kernel may be off that rounds q after the rotation (2^-11 of each element, if there is one), the weights p (2^-11 of each,
     2^-25 where they are subnormal) and the result (2^-11) to fp16 and sums n terms in fp32: with a = sum p |v| / sum p and d = scale * sum |q k|
     (what the scores' terms add up to)
         |delta s| <= u = d * 2^-11 (rotated) + d * hd * 2^-24 + 2^-21 * (1 + |s|)   (products, sums and exp2's argument in fp32)
-        |delta o| <= a * (2 u + 2 * 2^-11 + keys * 2^-23) + keys * 2^-25 * max |v| / sum p + (2^-11 |o| + 2^-25)"""
+        |delta o| <= a * (2 u + 2 * 2^-11 + keys * 2^-23) + keys * 2^-25 * max |v| / sum p + (2^-11 |o| + 2^-25)
+
+    sharp = b: the bound of a kernel that rotates q in fp32 (2^-24 of both products), holds it to b bits (2^-b of each element, 2^-24 at least: the last
+    place of an fp16 rest, of a halved query; not rotated: exact) and the weights in fp16 relative to 2^7 or more at the largest (so that a
+    subnormal one is off by 2^-32 of it), each key with its own error
+        u_j = scale * sum |k_j| * (2^-b |q'| + 2^-24 (|q cos| + |q sin|) + 2^-24) + d_j * 2 hd * 2^-24 + 2^-21 * (1 + |s_j| + max |s|)
+        |delta o| <= (sum p_j u_j |v_j - o| + sum (2^-11 p_j + 2^-32) |v_j|) / sum p + a * keys * 2^-24 + 2^-11 |o| + 2^-25
+    (a weight's rounding counts in the numerator alone; keys * 2^-25 each for the numerator's sum and the denominator's, of which a lane adds a
+    quarter at most; first order: u_j is well below 1)"""
     rows, heads, hd = q.shape
     blocks, kvh, block, _ = key_codes.shape
     out = np.full((rows, heads, hd), np.nan)
@@ -120,7 +128,11 @@ def attention(q, starts, past, new, table, key_codes, value_codes, key_scales, v
             t = starts[b] + i
             x = np.asarray(q[t], np.float64)
             if sin is not None:
-                x = rotate(x[None], sin, cos, np.array([min(int(past[b]) + i, len(sin) - 1)]))[0]
+                at = np.array([min(int(past[b]) + i, len(sin) - 1)])
+                size = rotate(np.abs(x)[None], np.abs(sin), np.abs(cos), at)[0]
+                half = hd // 2
+                size[:, :half] += 2 * np.abs(x[:, half:]) * np.abs(np.asarray(sin, np.float64)[at[0], :half])      # |q cos| + |q sin|
+                x = rotate(x[None], sin, cos, at)[0]
             seen = there & (j <= past[b] + i)
             for h in range(heads):
                 g = h * kvh // heads
@@ -131,6 +143,16 @@ def attention(q, starts, past, new, table, key_codes, value_codes, key_scales, v
                     continue
                 s = scale * (k @ x[h])
                 d = scale * (np.abs(k) @ np.abs(x[h]))
+                if sharp:
+                    p, top = np.exp(s - s.max()), np.abs(s).max()
+                    o, n, av = p @ v / p.sum(), len(k), np.abs(v)
+                    u = d * hd * 2.0 ** -23 + 2.0 ** -21 * (1 + np.abs(s) + top)
+                    if sin is not None:
+                        u += scale * (np.abs(k) @ (2.0 ** -sharp * np.abs(x[h]) + 2.0 ** -24 * size[h] + 2.0 ** -24))
+                    out[t, h] = o
+                    bound[t, h] = (((p * u) @ np.abs(v - o) + (2.0 ** -11 * p + 2.0 ** -32) @ av) / p.sum() + (p @ av / p.sum()) * n * 2.0 ** -24
+                                   + 2.0 ** -11 * np.abs(o) + 2.0 ** -25)
+                    continue
                 u = d.max() * (2.0 ** -11 * (sin is not None) + hd * 2.0 ** -24) + 2.0 ** -21 * (1 + np.abs(s).max())
                 p = np.exp(s - s.max())
                 out[t, h] = p @ v / p.sum()

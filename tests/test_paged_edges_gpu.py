@@ -1,0 +1,67 @@
+"""The paged 8-bit cache where it can go wrong without a loose bound noticing: rotated queries beyond fp16's range, small weights in long rows, every key
+counted once over all the cuts of a row, and what a rotated query keeps behind fp16's digits."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_oracle as P
+from test_paged_gpu import DEV, _angles, _attention_case, _dev, _numbers, _pool, _pool_dev, _runs, _same
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ext():
+    from exllama_amd import cuda_ext
+    return cuda_ext
+
+
+def _attention(ext, host, dev, heads, rope=False, scale=0.0):
+    """The call's result as numbers [rows, heads, hd]; NaN in rows that belong to no row of the batch."""
+    out = torch.full((host["q"].shape[0], heads * host["q"].shape[2]), float("nan"), dtype=torch.float16, device=DEV)
+    ext.ext_paged_attention(dev["q"], dev["starts"], dev["past"], dev["new"], dev["table"], *dev["pool"], heads, max_new=int(host["new"].max()), out=out,
+                            scale=scale, **(dict(sin=dev["sin"], cos=dev["cos"]) if rope else {}))
+    return out.cpu().double().numpy().reshape(host["q"].shape)
+
+
+def _sharp(host, bits, rope=True, scale=None, **other):
+    args = dict(host, **other)
+    return P.attention(args["q"], args["starts"], args["past"], args["new"], args["table"], *args["pool"], int(args["new"].max()), scale=scale, sharp=bits,
+                       **(dict(sin=args["sin"], cos=args["cos"]) if rope else {}))
+
+
+def _rest(hd, heads, kvh, new):
+    """The bits that a rotated query keeps: two fp16 numbers, but one where head_dim is over 128 and a row has more than 16 queries for a kv head."""
+    return 11 if hd > 128 and new * heads // kvh > 16 else 22
+
+
+def _set_q(host, dev, q):
+    host["q"] = q.astype(np.float16)
+    dev["q"] = torch.from_numpy(host["q"]).reshape(len(q), -1).to(DEV)
+
+
+# ---- numbers at the ends of their ranges --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("code", ["fp8", "int8"])
+@pytest.mark.parametrize("hd,heads,kvh,lens", [(128, 4, 2, [(70, 3), (5, 1)]), (128, 4, 1, [(200, 4)]), (256, 2, 2, [(40, 5)]), (256, 4, 2, [(0, 60)]),
+                                               (100, 4, 2, [(30, 6)]), (64, 4, 2, [(90, 70)]), (128, 8, 2, [(600, 40), (3, 9)])])
+def test_rotated_queries_beyond_fp16(ext, code, hd, heads, kvh, lens):
+    """A rotated element is up to sqrt(2) times as large as fp16's largest number; its keys are small, so that the scores are ordinary ones."""
+    rng = np.random.default_rng(hd + heads)
+    host, dev = _attention_case(rng, code, hd, heads, kvh, 16, lens)
+    q, half = host["q"].astype(np.float64), hd // 2
+    for c in (0, 1, half - 1):
+        some = rng.random(q.shape[:2]) < 0.5
+        q[some, c], q[some, c + half] = 60000.0 * rng.choice([-1, 1], int(some.sum())), 61000.0 * rng.choice([-1, 1], int(some.sum()))
+        small = rng.integers(-3, 4, host["pool"][0][..., 0].shape)
+        for k in (c, c + half):
+            host["pool"][0][..., k] = np.where(np.isnan(host["pool"][0][..., k]), np.nan, small * (2.0 ** -9 if code == "fp8" else 1.0))
+    host["pool"][2] = np.ldexp(1.0, rng.integers(-9, -6, host["pool"][2].shape) - (5 if code == "int8" else 0))
+    dev["pool"] = _pool_dev(host["pool"], code)
+    _set_q(host, dev, q)
+    turned = P.rotate(host["q"][:lens[0][1]].astype(np.float64), host["sin"], host["cos"], lens[0][0] + np.arange(lens[0][1]))
+    want, bound = _sharp(host, _rest(hd, heads, kvh, int(host["new"].max())))
+    got, some = _attention(ext, host, dev, heads, rope=True), ~np.isnan(bound)
+    assert np.abs(turned).max() > 65520
+    assert np.isfinite(got[some]).all()
+    assert (np.abs(got - want)[some] <= bound[some]).all()
