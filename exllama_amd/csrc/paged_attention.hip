@@ -3,8 +3,9 @@
 // Two forms, told apart by what the host knows, the most queries that a row has for one kv head (max_new * heads / kv_heads): up to 32 (head_dim over
 // 128: 16) the cache's bytes bound the work, above it the products do.  Measured (us, few / many; 32 queries a row, head_dim 128): 16 rows of 4000 keys
 // 51 / 68, one of 16000 30 / 40, 96 ragged ones 49 / 66, 8 of 300 19 / 17.
-// Rounding: codes * scale are fp16 numbers exactly (448 * 2^7, 127 * 2^9); weights are rounded to fp16 (2^-11 of each, relative to a reference that
-// lies at most 2^8 below the largest); sums, maxima and the softmax's denominator are 32 bits; a rotated query is an fp16 number and its
+// Rounding: codes * scale are fp16 numbers exactly (448 * 2^7, 127 * 2^9); weights are rounded to fp16 for the product with the values, the
+// denominator adds them as they are: 2^-11 of a weight, for one below 2^-21 of the largest (there fp16 is subnormal) 2^-32 of the largest;
+// sums, maxima and the softmax's denominator are 32 bits; a rotated query is an fp16 number and its
 // rest, also fp16 (2^-22) -- but for head_dim over 128 in the form for many queries; the result is rounded to fp16 once.
 #include "paged.h"
 #include <type_traits>
@@ -46,6 +47,8 @@ __device__ __forceinline__ PaRow pa_row(const PagedAttn& a, int b)
 #define PA_WAVES 4
 #define PA_KEYS 64
 #define PA_BEGIN 2
+#define PA_MOST 15.f                                              // the largest weight: 2^15
+#define PA_BIAS 7.f                                               // the largest weight of a tile that moves the reference: 2^7
 
 // A page's scale as the conversions take it.  int8: 2^e is the exponent field of the fp16 numbers that a code's byte becomes the mantissa of:
 // (1024 + u) * 2^e with u = code + 128, minus 1152 * 2^e -- up to e = 5; beyond (`big`, for every lane as soon as one has it) a product follows.
@@ -341,10 +344,12 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
             }
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            // the reference moves only when a score passes it by 2^8: the weights are relative to it, fp16 holds them up to 2^16
-            // (one pass at most; a loop for wide heads, whose sums lie in the matrix cores' own registers: what it copies out and back stays in it)
-            for (bool moves = __any(mx > m[nt] + 8.f); moves; moves = DP > 128 && __any(mx > m[nt] + 8.f)) {
-                const float mn = fmaxf(m[nt], mx);
+            // the weights are relative to a reference, which moves only when one would pass 2^15, so that the tile's largest becomes 2^7: fp16 holds them up
+            // to 2^16, and with all of its digits down to 2^-14, that is 2^-21 of the largest or less
+            // (one pass at most: mx - m is then 8 or less, whatever mx - 7 was rounded to; a loop for wide heads, whose sums lie in the matrix cores' own
+            // registers: what it copies out and back stays in it)
+            for (bool moves = __any(mx - m[nt] > PA_MOST); moves; moves = DP > 128 && __any(mx - m[nt] > PA_MOST)) {
+                const float mn = fmaxf(m[nt], mx - PA_BIAS);
                 const float keep = m[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[nt] - mn);
                 l[nt] *= keep;
 #pragma unroll
@@ -354,12 +359,14 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
                 m[nt] = mn;
             }
             const float ref = m[nt] == -INFINITY ? 0.f : m[nt];
+            float sum = 0.f;                                     // (of the tile: small weights one by one beside a large sum would lose their ends, all to one side)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float e = __builtin_amdgcn_exp2f(x[i] - ref);
-                l[nt] += e;
+                sum += e;
                 p[nt][i >> 3][i & 7] = (f16) e;
             }
+            l[nt] += sum;
         }
         const PaScale vs = pa_scale<CODE>(st.vs);
         if (CODE == EXL_PAGE_FP8 && border && row.fresh > 1) {
@@ -831,10 +838,12 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
 #pragma unroll
             for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[kt][j]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c1;
-        // the reference moves only when a score passes it by 2^8: the weights are relative to it, fp16 holds them up to 2^16
-        // (one pass at most; a loop for wide heads, whose sums lie in the matrix cores' own registers: what it copies out and back stays in it)
-        for (bool moves = __any(mx > m + 8.f); moves; moves = DP > 128 && __any(mx > m + 8.f)) {
-            const float mn = fmaxf(m, mx);
+        asm("" : "+v"(mx));                                       // (rounded here: contracted into the difference below, a pass might not be the last)
+        // the reference moves as in the other form
+        // (one pass at most: mx - m is then 8 or less, whatever mx - 7 was rounded to; a loop for wide heads, whose sums lie in the matrix cores' own
+        // registers: what it copies out and back stays in it)
+        for (bool moves = __any(mx - m > PA_MOST); moves; moves = DP > 128 && __any(mx - m > PA_MOST)) {
+            const float mn = fmaxf(m, mx - PA_BIAS);
             const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             l *= keep;
 #pragma unroll
@@ -845,14 +854,16 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
         }
         const float ref = m == -INFINITY ? 0.f : m;
         f16x8 p[2][2];
+        float sum = 0.f;                                          // (of the tile, as in the other form)
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const float e = __builtin_amdgcn_exp2f(fmaf(s[kt][j], c1, -ref));
-                l += e;
+                sum += e;
                 p[kt][j >> 3][j & 7] = (f16) e;
             }
+        l += sum;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll

@@ -65,3 +65,33 @@ def test_rotated_queries_beyond_fp16(ext, code, hd, heads, kvh, lens):
     assert np.abs(turned).max() > 65520
     assert np.isfinite(got[some]).all()
     assert (np.abs(got - want)[some] <= bound[some]).all()
+
+
+@pytest.mark.parametrize("code", ["fp8", "int8"])
+@pytest.mark.parametrize("below", [17.5, 19.5, 22.5])
+@pytest.mark.parametrize("new", [1, 40])
+def test_many_small_weights_beside_a_large_one(ext, code, below, new):
+    """One key, the row's first, with a score of 0, 65535 others `below` powers of two under it and with values of 1: together they are a tenth of the result, or
+    a quarter, or a hundredth.  64 rows of 32 heads, all on the same pages, so that no wave and no workgroup begins in the middle of one."""
+    hd, heads, keys, block, n = 64, 32, 65536, 128, 64
+    blocks, kind = keys // block, {"fp8": torch.float8_e4m3fn, "int8": torch.int8}[code]
+    kp = torch.zeros(blocks, heads, block, hd, dtype=torch.float32, device=DEV)
+    kp[..., 0] = -16
+    kp[0, :, 0, 0] = 0
+    kp = kp.to(kind)
+    vp = torch.ones(blocks, heads, hd, block, dtype=torch.float32, device=DEV)
+    vp[0, :, :, 0] = 0
+    vp = vp.to(kind)
+    scales = torch.ones(blocks, heads, device=DEV)
+    q = torch.zeros(n * new, heads, hd, dtype=torch.float16, device=DEV)
+    q[..., 0] = below / 16                                    # (exact)
+    past = np.full(n, keys - new)
+    out = ext.ext_paged_attention(q.view(n * new, -1), _dev(np.arange(n + 1) * new), _dev(past), _dev(np.full(n, new)),
+                                  _dev(np.tile(np.arange(blocks), (n, 1))), kp, vp, scales, scales, heads, max_new=new, scale=float(np.log(2)))
+    others = (keys - new + np.arange(new)) * 2.0 ** -below
+    want = np.tile(others / (1 + others), n)[:, None, None]
+    # a weight's rounding, the same for all of them (2^-11), the result's (2^-11), the scores' (2^-20 each with log 2 in 32 bits), and the sums', at most 2^-24
+    # each and all to one side: the denominator's of 1024 tiles (2^-14), the product's of 4096 steps of 16 keys (2^-12)
+    tol = 2.0 ** -11 + 2.0 ** -11 + 2.0 ** -18 + 2.0 ** -14 + 2.0 ** -12
+    got = out.view(n * new, heads, hd).cpu().double().numpy()
+    assert np.abs(got / want - 1).max() <= tol
