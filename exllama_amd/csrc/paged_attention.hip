@@ -339,6 +339,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 x[i] = s[nt][i >> 2][i & 3] * sc;
+                asm("" : "+v"(x[i]));                             // (rounded here, for the maximum and for the weight alike)
                 if (border && (!st.there || key0 + i > limit[nt])) x[i] = -INFINITY;
                 mx = fmaxf(mx, x[i]);
             }
@@ -552,6 +553,14 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const
 // takes 77 us instead of 66, pieces of a 70B prompt (411 GFLOP) 622 instead of 503; without it the result is 3.9e-4 of its norm off, with it
 // 2.6e-4 (2.0e-4 are its own rounding).  Wider heads have no registers for it (spilled: 127 -> 213 us).
 #define PM_ROWS 128
+
+// s * c1, rounded, and how far it lies above ref
+__device__ __forceinline__ float pa_above(float s, float c1, float ref)
+{
+    float x = s * c1;
+    asm("" : "+v"(x));                                            // (not contracted)
+    return x - ref;
+}
 
 // A tile of queries and a piece of its keys (all tiles of a row are cut in the same number of `pieces`)
 struct PmItem { int row, tile, piece, pieces; };
@@ -852,7 +861,15 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
                 for (int j = 0; j < 16; ++j) o[t][j] *= keep;
             m = mn;
         }
-        const float ref = m == -INFINITY ? 0.f : m;
+        float ref = m == -INFINITY ? 0.f : m;
+        if (__any(fabsf(ref) > 0x1p22f)) {                        // scores so large that one fma and a product with a difference disagree by more than 2^-2: as mx was
+            const float back = 1.f / c1;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[kt][j] = pa_above(s[kt][j], c1, ref) * back;
+            ref = 0.f;
+        }
         f16x8 p[2][2];
         float sum = 0.f;                                          // (of the tile, as in the other form)
 #pragma unroll

@@ -95,3 +95,31 @@ def test_many_small_weights_beside_a_large_one(ext, code, below, new):
     tol = 2.0 ** -11 + 2.0 ** -11 + 2.0 ** -18 + 2.0 ** -14 + 2.0 ** -12
     got = out.view(n * new, heads, hd).cpu().double().numpy()
     assert np.abs(got / want - 1).max() <= tol
+
+
+@pytest.mark.parametrize("code", ["fp8", "int8"])
+@pytest.mark.parametrize("hd,heads,kvh,lens", [(128, 4, 2, [(130, 3), (5, 1)]), (64, 4, 2, [(90, 70)]), (256, 4, 2, [(700, 40)]), (128, 2, 2, [(2000, 1)])])
+def test_scores_beyond_every_ordinary_size(ext, code, hd, heads, kvh, lens):
+    """Scores of 2^29 and more, where neighbours in 32 bits lie 32 apart: the largest takes all the weight, and nothing overflows."""
+    rng = np.random.default_rng(hd + heads)
+    host, dev = _attention_case(rng, code, hd, heads, kvh, 16, lens)
+    _set_q(host, dev, rng.choice([-1.0, 1.0], host["q"].shape) * rng.integers(20000, 60000, host["q"].shape))
+    host["pool"][2][:] = 2.0 ** P.EXP[code][1]
+    dev["pool"] = _pool_dev(host["pool"], code)
+    want, _ = _sharp(host, 22, rope=False)
+    got, some = _attention(ext, host, dev, heads), ~np.isnan(want)
+    assert np.isfinite(got[some]).all()
+    # one key takes all: its value to fp16 (2^-11) and by a quotient (2^-23) -- where the first two scores lie far apart for 32 bits
+    top = np.full(want.shape[:2], np.inf)
+    for b, (past, new) in enumerate(lens):
+        for i in range(new):
+            j = np.arange(past + i + 1)
+            page = host["table"][b][j // 16]
+            for h in range(heads):
+                g = h * kvh // heads
+                s = np.sort((host["pool"][0][page, g, j % 16, :hd] * host["pool"][2][page, g][:, None]) @ host["q"][host["starts"][b] + i, h].astype(np.float64))
+                s *= hd ** -0.5
+                # (a score's terms are summed in 32 bits: 2 hd roundings of 2^-24 of what they add up to, at most hd * 2^16 * 2^16 / sqrt(hd))
+                top[host["starts"][b] + i, h] = (s[-1] - s[-2] if len(s) > 1 else np.inf) / (2 * hd * 2.0 ** -24 * hd ** 0.5 * 2.0 ** 32)
+    sure = some & (top > 2)[..., None]
+    assert sure.any() and (np.abs(got - want)[sure] <= 2.0 ** -10 * np.abs(want[sure]) + 2.0 ** -25).all()
