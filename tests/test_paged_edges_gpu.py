@@ -123,3 +123,77 @@ def test_scores_beyond_every_ordinary_size(ext, code, hd, heads, kvh, lens):
                 top[host["starts"][b] + i, h] = (s[-1] - s[-2] if len(s) > 1 else np.inf) / (2 * hd * 2.0 ** -24 * hd ** 0.5 * 2.0 ** 32)
     sure = some & (top > 2)[..., None]
     assert sure.any() and (np.abs(got - want)[sure] <= 2.0 ** -10 * np.abs(want[sure]) + 2.0 ** -25).all()
+
+
+# ---- every key, once ----------------------------------------------------------------------------------------------------------------------
+
+# few queries: in one stretch, in several, several rows in one; single tokens and drafts; many: in one piece and in several, beside short rows
+EVERY = [(128, 32, 32, 64, [(2047, 1)]), (128, 16, 2, 32, [(5000, 1), (100, 1), (2000, 1), (0, 1)]), (64, 4, 2, 16, [(777, 5), (63, 3), (64, 2), (0, 5)]),
+         (256, 4, 2, 128, [(3000, 2), (1, 2)]), (128, 8, 1, 64, [(6000, 4)]), (100, 8, 8, 16, [(1300, 1), (62, 1), (63, 1), (64, 1)]),
+         (128, 8, 8, 16, [(191 + 37 * i, 1) for i in range(60)]), (128, 4, 4, 64, [(9000, 1)]), (64, 64, 64, 32, [(3000, 1), (40, 0), (2999, 1)]),
+         (128, 8, 1, 64, [(6000, 20)]), (128, 4, 4, 64, [(0, 700), (1500, 90)]), (256, 4, 2, 128, [(1000, 129), (50, 1)]), (64, 4, 4, 16, [(2300, 40), (7, 1)]),
+         (128, 16, 2, 16, [(200, 300), (3, 260)]), (100, 4, 2, 32, [(4100, 33), (60, 257)])]
+
+
+@pytest.mark.parametrize("code", ["fp8", "int8"])
+@pytest.mark.parametrize("equal", [True, False])
+@pytest.mark.parametrize("hd,heads,kvh,block,lens", EVERY)
+def test_every_key_counts_once(ext, code, equal, hd, heads, kvh, block, lens):
+    """A key's value is 1 in two columns, of its place in its tile of 64 and of its tile, and 0 elsewhere; its score is a whole power of two (0, or -12 .. 12 drawn
+    for the key, so that the softmax's reference moves).  Every weight is then an fp16 number, a column is the sum of one class of keys over the
+    sum of all, and a tile that is lost or taken twice anywhere changes its column by far more than the roundings."""
+    rng = np.random.default_rng(hd + len(lens))
+    host, dev = _attention_case(rng, code, hd, heads, kvh, block, lens)
+    kc, vc, ks, vs = host["pool"]
+    half = hd // 2
+    power = {}
+    for b, (past, new) in enumerate(lens):
+        j = np.arange(past + new)
+        page, off = host["table"][b][j // block], j % block
+        power[b] = np.zeros(len(j)) if equal else np.clip(rng.integers(-6, 7, len(j) // 64 + 1)[j // 64] + rng.integers(-6, 7, len(j)), -12, 12)
+        kc[page, :, off] = 0.0
+        vc[page, :, :, off] = 0.0
+        kc[page, :, off, 0] = power[b][:, None]
+        vc[page, :, (j % 64) % half, off] = 64.0
+        vc[page, :, half + (j // 64) % half, off] = 64.0
+    ks[:] = 1.0
+    vs[:] = 2.0 ** 7
+    dev["pool"] = _pool_dev(host["pool"], code)
+    q = np.zeros(host["q"].shape)
+    q[..., 0] = 1.0
+    _set_q(host, dev, q)
+    got = _attention(ext, host, dev, heads, scale=float(np.log(2)))
+    for b, (past, new) in enumerate(lens):
+        if not new:
+            continue
+        j = np.arange(past + new)
+        w = np.zeros((len(j), hd))
+        w[j, (j % 64) % half] += 2.0 ** power[b]
+        w[j, half + (j // 64) % half] += 2.0 ** power[b]
+        want = 2.0 ** 13 * (np.cumsum(w, 0) / np.cumsum(2.0 ** power[b])[:, None])[past:]
+        x = got[host["starts"][b]:host["starts"][b] + new]
+        # the result's rounding (2^-11; 2^-25 below fp16's normal range), sums of positive numbers in 32 bits (a lane adds a quarter of the keys: at most
+        # 2^-26 of the sum for each key, numerator and denominator) and exp2 (2^-21 for scores that log 2 in 32 bits makes 2^-20 off at most)
+        tol = 2.0 ** -11 + len(j) * 2.0 ** -25 + 2.0 ** -18
+        assert (np.abs(x - want[:, None]) <= tol * want[:, None] + 2.0 ** -25).all(), (b, past, new)
+
+
+@pytest.mark.parametrize("hd,heads,kvh,block,lens,spread,bites", [
+    (128, 4, 2, 16, [(60, 8), (5, 3)], 8, True), (128, 4, 2, 64, [(10, 40)], 8, True), (128, 4, 2, 64, [(100, 40)], 32, True), (64, 4, 2, 32, [(10, 40)], 8, True),
+    (100, 4, 2, 16, [(10, 40)], 16, True), (100, 4, 4, 16, [(20, 6), (9, 1)], 16, True), (256, 2, 2, 64, [(10, 7)], 4, False), (256, 4, 2, 64, [(200, 40)], 2, False),
+    (128, 8, 1, 64, [(6000, 20)], 2, False), (128, 4, 4, 64, [(9000, 1)], 2, False), (128, 16, 2, 32, [(5000, 1), (100, 1), (2000, 1)], 2, False)])
+def test_a_rotated_query_keeps_what_fp16_leaves(ext, hd, heads, kvh, block, lens, spread, bites):
+    """Against the bound of a kernel that holds a rotated query to 22 bits.  `bites`: the formula with the rotated query rounded to fp16 breaks that bound, so
+    that a kernel which drops the rest fails."""
+    host, dev = _attention_case(np.random.default_rng(1), "fp8", hd, heads, kvh, block, lens, spread=spread)
+    want, bound = _sharp(host, _rest(hd, heads, kvh, int(host["new"].max())))
+    some = ~np.isnan(bound)
+    if bites:
+        rounded = host["q"].astype(np.float64)
+        for b, (past, new) in enumerate(lens):
+            rows = slice(host["starts"][b], host["starts"][b] + new)
+            rounded[rows] = P.rotate(rounded[rows], host["sin"], host["cos"], past + np.arange(new)).astype(np.float16)
+        off, _ = _sharp(host, 22, rope=False, q=rounded)
+        assert (np.abs(off - want)[some] > bound[some]).mean() > 0.005
+    got = _attention(ext, host, dev, heads, rope=True)
+    assert (np.abs(got - want)[some] <= bound[some]).all()
