@@ -197,3 +197,26 @@ def test_a_rotated_query_keeps_what_fp16_leaves(ext, hd, heads, kvh, block, lens
         assert (np.abs(off - want)[some] > bound[some]).mean() > 0.005
     got = _attention(ext, host, dev, heads, rope=True)
     assert (np.abs(got - want)[some] <= bound[some]).all()
+
+
+# ---- append: every number of rows that a workgroup can take ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("code", ["fp8", "int8"])
+@pytest.mark.parametrize("hd,kvh,block,spec", [
+    (64, 8, 16, [(0, 900), (-1, -5), (3, 700), (15, 2)] + [(9, 1)] * 70 + [(0, 300)]),                   # 16000 token rows * heads: 16 rows a workgroup
+    (64, 8, 32, [(0, 2000), (-1, -3), (31, 1500)] + [(9, 1)] * 50 + [(5, 9), (1, 2)]),                   # 28600: 32 rows
+    (100, 8, 16, [(0, 900), (-1, -5), (3, 700), (15, 2)] + [(9, 1)] * 70), (100, 4, 128, [(7, 5000), (-1, -70), (0, 1), (120, 60)]),
+    (16, 32, 64, [(0, 700), (63, 1), (0, 64), (1, 63)] + [(60, 9)] * 9)])
+def test_append_of_every_chunk(ext, code, hd, kvh, block, spec):
+    rng = np.random.default_rng(hd + kvh)
+    blocks = sum(-(-(o % block + n) // block) for o, n in spec if n > 0) + 2
+    pool = _pool(rng, blocks, kvh, block, hd, code)
+    dev = _pool_dev(pool, code)
+    slots, pos = _runs(rng, blocks, block, spec)
+    t = len(slots)
+    x = (rng.normal(0, 1, (2, t, kvh, hd)) * np.exp(rng.normal(0, 1.5, (2, 1, kvh, hd)))).astype(np.float16)
+    sin, cos = _angles(6000, hd)
+    ext.ext_paged_append(*(torch.from_numpy(y).reshape(t, -1).to(DEV) for y in x), _dev(slots), *dev, positions=_dev(pos), sin=sin.to(DEV), cos=cos.to(DEV))
+    P.append(x[0], x[1], slots, *pool, code, pos, sin.numpy(), cos.numpy())
+    for name, got, want in zip(("keys", "values", "key scales", "value scales"), dev, pool):
+        assert _same(_numbers(got), want), name
