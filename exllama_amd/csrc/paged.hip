@@ -8,6 +8,8 @@
 //   want  = max(0, ceil(min(past + take, max_len) / block) - held), got = clamp(avail - sum(want), 0, want)
 //   table[held + i] = ring[(head + sum(want) + i) mod blocks], i < got
 //   new < 0: the row has ended; its blocks go to the ring's end in order, its table entries become -1
+//   past > held * block, and new or held > 0: earlier tokens found no block.  want = 0, what the row lacks counts as missing: a block handed out now would
+//   begin with what another row left in it, in place of those tokens
 // Then every token row's slot = table[pos / block] * block + pos % block.  Latency is all that matters (a step of 256 rows moves
 // 7 KB): one workgroup does both halves where the work is small, otherwise the scan runs in one workgroup and the filling in
 // many -- a second launch instead of a grid-wide wait.  Measured, us, one workgroup / scan + filling and
@@ -56,14 +58,16 @@ __device__ __forceinline__ int64_t slot_scan(int64_t v, int64_t* lds, bool one_w
 template <int R> __device__ __forceinline__ void slot_scan_rows(const SlotArgs& a, SlotRow* desc)
 {
     __shared__ int64_t lds[SLOT_WAVES];
+    __shared__ unsigned long long lacking;                        // blocks that rows without their earlier tokens' lack
     const bool one_wave = a.n <= 64 * R;
     if (one_wave && threadIdx.x >= 64) return;
+    if (threadIdx.x == 0) lacking = 0;                            // (a scan's barrier, or the wave's order, stands between this and the first sum)
     const int head = (int) ((uint32_t) a.counters[0] % (uint32_t) a.blocks);
     const int avail = min(max(a.counters[1], 0), a.blocks);
     int64_t rows_before = 0, want_before = 0, back_before = 0;
     for (int b0 = 0; b0 < a.n; b0 += SLOT_THREADS * R) {
         const int first = b0 + threadIdx.x * R;
-        int fresh[R], held[R], past[R], take[R], start[R], want[R], back[R];
+        int fresh[R], held[R], past[R], take[R], start[R], want[R], back[R], lost[R];
         int64_t mine = 0, total;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -97,6 +101,8 @@ template <int R> __device__ __forceinline__ void slot_scan_rows(const SlotArgs& 
             const int end = (int) min((int64_t) past[i] + take[i], (int64_t) a.max_len);
             const int need = (int) (((int64_t) end + (1 << a.lbs) - 1) >> a.lbs);
             want[i] = first + i < a.n && fresh[i] >= 0 ? max(0, need - held[i]) : 0;
+            lost[i] = (fresh[i] > 0 || held[i] > 0) && (int64_t) past[i] > (int64_t) held[i] << a.lbs ? want[i] : 0;
+            want[i] -= lost[i];
             back[i] = fresh[i] < 0 ? held[i] : 0;
             mine += (int64_t) want[i] << 32 | back[i];
         }
@@ -107,6 +113,7 @@ template <int R> __device__ __forceinline__ void slot_scan_rows(const SlotArgs& 
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             if (first + i >= a.n) break;
+            if (lost[i]) atomicAdd(&lacking, (unsigned long long) lost[i]);
             const int got = (int) min(max((int64_t) avail - base, (int64_t) 0), (int64_t) want[i]);
             SlotRow r;
             r.start = start[i]; r.take = take[i]; r.past = past[i]; r.held = held[i];
@@ -126,7 +133,7 @@ template <int R> __device__ __forceinline__ void slot_scan_rows(const SlotArgs& 
         const int got = (int) min(want_before, (int64_t) avail);
         a.counters[0] = (head + got) % a.blocks;
         a.counters[1] = (int) min((int64_t) avail - got + back_before, (int64_t) a.blocks);
-        a.counters[2] = (int) min(want_before - got, (int64_t) 0x7fffffff);
+        a.counters[2] = (int) min(want_before - got + (int64_t) lacking, (int64_t) 0x7fffffff);
         a.counters[3] = 0;
         a.starts[a.n] = (int) min(a.row_stride > 0 ? (int64_t) a.n * a.row_stride : rows_before, (int64_t) a.rows);
     }

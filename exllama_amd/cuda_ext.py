@@ -757,7 +757,11 @@ def ext_paged_slots(past_lens, new_lens, held, block_table, ring, counters, bloc
     token rows from starts[b] on (one row of the batch behind the other; row_stride > 0: starts[b] = b * row_stride), and block_table
     [n, width], held [n], ring [blocks], counters [4] (head of the ring, free blocks, missing blocks, 0) are updated in place so that the
     row owns the blocks of past + new tokens (at most max_len).  slots: block * block_size + offset, -1 without a token or a block.
-    The same call again changes nothing more; past_lens stays as it is.  All lengths are read on the device."""
+    The same call again changes nothing more (but where blocks were missing: it hands out what ended rows gave back in the first); past_lens
+    stays as it is.  All lengths are read on the device.  Where blocks can run out or max_len can be reached, past_lens must become
+    min(past_lens + new_lens, held * block_size, max_len), not past_lens + new_lens: tokens without a slot are not in the cache.  A row for
+    which past_lens says more than its blocks hold gets no block and no slot until past_lens is set back or the row ends (one that brings and holds
+    nothing gets the blocks of its past, for the caller to fill)."""
     return paged_slots(past_lens, new_lens, held, block_table, ring, counters, block_size, rows, max_new, max_len, row_stride)
 
 

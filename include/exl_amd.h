@@ -219,7 +219,13 @@ int exl_attention(const void* q, const void* key_cache, const void* value_cache,
  * blocks, ring [num_blocks].  new_lens[b] < 0: the row has ended, its blocks go to the ring's end (free from the NEXT call on), its table
  * entries become -1, held 0.  slots [rows] = block * block_size + offset of each token row, -1 without a token or a block; positions [rows];
  * starts [n_rows + 1].  counters[2] = blocks that were wanted and not there.  block_table, held, ring and counters are updated in place;
- * the same call again changes nothing more.  past_lens is not touched.  scratch: 8 * n_rows ints. */
+ * the same call again changes nothing more (but where blocks were missing: it hands out what ended rows gave back in the first).  past_lens
+ * is not touched.  scratch: 8 * n_rows ints.  block_table entries behind the held ones have to be -1.
+ * Tokens that got no slot are not in the cache, and the caller must not count them: a row holds min(past + taken, held * block_size, max_len) tokens
+ * after the append (held as this call leaves it), which is what past_lens may become; where max_len cuts a block, exl_paged_attention's new_lens
+ * must not reach beyond it either.  A row for which past_lens says more than its held blocks hold gets no block and no slot (what other
+ * rows left in a block would stand for the missing tokens) until past_lens is set back or the row ends -- unless it brings and holds nothing: then it
+ * gets the blocks of its past, for the caller to fill. */
 int exl_paged_slots(const int32_t* past_lens, const int32_t* new_lens, int32_t* held, int32_t* block_table, int32_t* ring, int32_t* counters,
                     int n_rows, int table_width, int block_size, int num_blocks, int max_len, int max_new, int rows, int row_stride,
                     int32_t* starts, int32_t* slots, int32_t* positions, int32_t* scratch, void* stream);

@@ -22,6 +22,9 @@ def slots(past, new, held, table, ring, counters, block, max_len, max_new, rows,
             held[b] = 0
             continue
         want = max(0, -(-min(int(past[b]) + take, max_len) // block) - int(held[b]))
+        if (new[b] > 0 or held[b] > 0) and past[b] > int(held[b]) * block:         # earlier tokens found no block: the row gets none behind them
+            missing += want
+            want = 0
         for _ in range(want):
             if taken < len(free):
                 table[b, held[b]] = free[taken]

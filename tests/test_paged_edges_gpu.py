@@ -220,3 +220,88 @@ def test_append_of_every_chunk(ext, code, hd, kvh, block, spec):
     P.append(x[0], x[1], slots, *pool, code, pos, sin.numpy(), cos.numpy())
     for name, got, want in zip(("keys", "values", "key scales", "value scales"), dev, pool):
         assert _same(_numbers(got), want), name
+
+
+# ---- pools that run dry ---------------------------------------------------------------------------------------------------------------------
+
+class _Dry:
+    """Three rows on a pool of six pages of 16 that hold another sequence's leavings, NaN among them."""
+
+    def __init__(self, rng, new_rows=3):
+        self.rng, self.hd, self.kvh, self.heads, self.block = rng, 64, 2, 4, 16
+        codes = P.nearest(rng.normal(0, 100, (6, 2, 16, 64)), "fp8"), P.nearest(rng.normal(0, 100, (6, 2, 64, 16)), "fp8")
+        for c in codes:
+            c[rng.random(c.shape) < 0.3] = np.nan
+        self.pool = [codes[0], codes[1], np.full((6, 2), 2.0 ** 7), np.full((6, 2), 2.0 ** 7)]
+        self.dpool = _pool_dev(self.pool, "fp8")
+        self.past, self.held, self.counters = np.zeros(3, np.int32), np.zeros(3, np.int32), np.array([0, 6, 0, 0], np.int32)
+        self.table, self.ring = np.full((3, 5), -1, np.int32), rng.permutation(6).astype(np.int32)
+        self.d = {k: _dev(getattr(self, k)) for k in ("past", "held", "table", "ring", "counters")}
+
+    def step(self, ext, new, max_len=80, check=True):
+        """One pass; returns (slots, the result) and, with `check`, holds both against the oracle."""
+        rows = int(np.maximum(new, 0).sum())
+        q, k, v = (self.rng.normal(0, 1, (rows, h, self.hd)).astype(np.float16) for h in (self.heads, self.kvh, self.kvh))
+        dq, dk, dv = (torch.from_numpy(x).reshape(rows, x.shape[1] * self.hd).to(DEV) for x in (q, k, v))
+        dnew, top = _dev(new), max(int(np.max(new)), 1)
+        starts, slots, _ = ext.ext_paged_slots(self.d["past"], dnew, self.d["held"], self.d["table"], self.d["ring"], self.d["counters"], 16, rows, max_new=top,
+                                               max_len=max_len)
+        ext.ext_paged_append(dk, dv, slots, *self.dpool)
+        fits = torch.minimum(dnew.clamp(min=0), (max_len - self.d["past"]).clamp(min=0))
+        out = ext.ext_paged_attention(dq, starts, self.d["past"], fits, self.d["table"], *self.dpool, self.heads, max_new=top)
+        got = out.cpu().double().numpy().reshape(rows, self.heads, self.hd)
+        if check:
+            s, want_slots, _ = P.slots(self.past, new, self.held, self.table, self.ring, self.counters, 16, max_len, top, rows)
+            P.append(k, v, want_slots, *self.pool, "fp8")
+            want, bound = P.attention(q, s, self.past, fits.cpu().numpy(), self.table, *self.pool, top)
+            for name in ("held", "table", "ring", "counters"):
+                assert np.array_equal(self.d[name].cpu().numpy(), getattr(self, name)), name
+            assert np.array_equal(slots.cpu().numpy(), want_slots)
+            some = ~np.isnan(bound)
+            assert (np.abs(got - want)[some] <= bound[some]).all()
+        assert np.isfinite(got).all()
+        return slots.cpu().numpy(), got
+
+
+def test_a_row_that_lost_tokens_reads_no_other_rows_pages(ext):
+    """past_lens advanced by all of new_lens although the pool ran dry: when pages come free again, the row gets none of them, and every result is
+    that of the keys it holds; set back to what it holds, it goes on."""
+    dry = _Dry(np.random.default_rng(0))
+
+    def blindly(new):
+        dry.past += np.maximum(new, 0).astype(np.int32)
+        dry.past[new < 0] = 0
+        dry.d["past"].copy_(_dev(dry.past))
+
+    for new in ([40, 30, 10], [1, 1, 1], [0, 5, 6], [1, 1, 1]):       # 3 + 2 + 1 pages: all; then row 1 and row 2 lose tokens
+        dry.step(ext, np.array(new))
+        blindly(np.array(new))
+    assert dry.held.tolist() == [3, 2, 1] and dry.past.tolist() == [42, 37, 18]
+    dry.step(ext, np.array([-1, 0, 0]))                               # three pages come free
+    blindly(np.array([-1, 0, 0]))
+    held = dry.held.copy()
+    for new in ([0, 1, 1], [0, 0, 2], [20, 1, 3]):
+        slots, _ = dry.step(ext, np.array(new))
+        blindly(np.array(new))
+        assert (slots[new[0]:] == -1).all() and dry.counters[2] > 0
+    assert (dry.held[1:] == held[1:]).all()
+    dry.past[:] = np.minimum(dry.past, dry.held * 16)                 # set back
+    dry.d["past"].copy_(_dev(dry.past))
+    dry.step(ext, np.array([0, 1, 0]))
+    assert dry.held[1] == held[1] + 1
+
+
+def test_lengths_that_advance_by_what_was_placed(ext):
+    """The rule for a step on the device: past = min(past + new, held * block, max_len).  A row that is short of pages or at max_len (which cuts a page) stays
+    where it is, and goes on when it can."""
+    dry = _Dry(np.random.default_rng(1))
+    for new in ([40, 30, 10], [9, 5, 1], [1, 5, 6], [1, 1, 1], [-1, 1, 1], [0, 9, 9], [0, 1, 9], [30, 9, 9], [1, 1, 1]):
+        new = np.array(new)
+        slots, _ = dry.step(ext, new, max_len=44)
+        d = dry.d
+        taken = _dev(new).clamp(min=0)
+        d["past"].copy_(torch.minimum(torch.minimum(d["past"] + taken, d["held"] * 16), torch.full_like(taken, 44)))
+        placed = np.array([(slots[s:s + n] >= 0).sum() for s, n in zip(np.cumsum(np.maximum(new, 0)) - np.maximum(new, 0), np.maximum(new, 0))])
+        dry.past = np.where(new < 0, 0, dry.past + placed).astype(np.int32)
+        assert d["past"].tolist() == dry.past.tolist()
+    assert dry.past.max() == 44
