@@ -1106,7 +1106,8 @@ extern "C" int exl_paged_attention(const void* q, long q_stride, const int32_t* 
     EXL_REQUIRE(q_stride >= (long) num_heads * head_dim && q_stride % 4 == 0 && ((uintptr_t) q | (uintptr_t) out) % 8 == 0, EXL_E_INVALID,
                 "paged_attention: q rows must be 8-byte aligned and at least heads * head_dim apart");
     EXL_REQUIRE(((uintptr_t) key_pages | (uintptr_t) value_pages) % 16 == 0, EXL_E_INVALID, "paged_attention: pages must be 16-byte aligned");
-    EXL_REQUIRE((int64_t) table_width * block_size <= 0x7fffffff, EXL_E_UNSUPPORTED, "paged_attention: the block table exceeds 2^31 tokens");
+    EXL_REQUIRE((int64_t) table_width * block_size <= 0x7fffffff - PA_KEYS, EXL_E_UNSUPPORTED,      // (lengths are rounded up to tiles in 32 bits)
+                "paged_attention: the block table exceeds 2^31 - %d tokens", PA_KEYS + 1);
     EXL_REQUIRE((int64_t) n_rows * ((int64_t) table_width * block_size / PA_KEYS + PA_BEGIN + 1) < 1 << 30, EXL_E_UNSUPPORTED,
                 "paged_attention: %d rows of %d blocks are too many", n_rows, table_width);
     if (none) return 0;

@@ -243,6 +243,7 @@ int exl_paged_append(const void* key_states, const void* value_states, long key_
  * 1 / sqrt(head_dim).  sin / cos: q is rotated at its position first (to twice fp16's digits; head_dim over 128 and more than 16 queries a row
  * and kv head: rounded to fp16).  Pages outside the pool are not seen; a query that sees nothing gives zeros, one that sees a NaN NaN, no
  * other; rows of `out` [rows, heads * head_dim] that belong to no row of the batch are left as they were.  out must not overlap q.
+ * table_width * block_size: at most 2^31 - 65.  No two rows of the batch share a row of q.
  * workspace: at least exl_paged_attention_workspace(...) bytes, for this call alone until it has run. */
 size_t exl_paged_attention_workspace(int n_rows, int rows, int max_new, int num_heads, int num_kv_heads, int head_dim, int table_width, int block_size);
 int exl_paged_attention(const void* q, long q_stride, const int32_t* starts, const int32_t* past_lens, const int32_t* new_lens, int n_rows, int rows,

@@ -22,3 +22,26 @@ def test_a_row_that_lost_tokens_gets_no_block():
     assert call(1, 1, 0) == ([0, 1], [-1, 32, 33, 34, -1, -1, -1, -1], 1)
     assert call(32, 2, 2) == ([3, 1], [32, 33, 48, 49, 50, -1, -1, -1], 0)
     assert call(33, 0, 0) == ([3, 1], [80, 81, 82, -1, -1, -1, -1, -1], 0)
+
+
+@pytest.fixture(scope="module")
+def ext():
+    from exllama_amd import cuda_ext
+    return cuda_ext
+
+
+def test_attention_refuses_tables_at_the_end_of_32_bits(ext):
+    """A length is rounded up to a tile of 64 keys in 32 bits: tables of more than 2^31 - 65 tokens are refused, the largest below is not (it is refused for its
+    workspace, the last check before a launch)."""
+    lib = ext._lib.load()
+    p, far = C.c_void_p(4096), C.c_void_p(1 << 20)            # never read: every call below is refused first
+
+    def attention(width, block, rows):
+        assert lib.exl_paged_attention(p, 64, p, p, p, 1, rows, rows, p, width, p, p, p, p, 0, 8, block, 1, 1, 64, 0.0, None, None, 0, far, None, 0, None) < 0
+        return lib.exl_last_error().decode()
+
+    for rows in (1, 40):
+        for block in (16, 32, 64, 128):
+            most = (2 ** 31 - 65) // block
+            assert "workspace" in attention(most, block, rows)
+            assert "block table" in attention(most + 1, block, rows), block
