@@ -445,7 +445,8 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP * NT <= 128 ? 2 : 1) void paged_a
         const int tiles = (row.keys + PA_KEYS - 1) / PA_KEYS, first = max(from - PA_BEGIN, 0), last = min(from + left - PA_BEGIN, tiles) - 1;
         left -= tiles + PA_BEGIN - from;
         int nb = b;                                               // the next row that has any keys, if it has a tile in this stretch
-        if (left > PA_BEGIN) do ++nb; while (nb < a.n - 1 && pa_row_of_wave(a, nb).keys == 0);
+        // (b + 1 < n always holds where places are left -- but for lengths that changed under the call)
+        if (left > PA_BEGIN && b + 1 < a.n) do ++nb; while (nb < a.n - 1 && pa_row_of_wave(a, nb).keys == 0);
         for (int tile = first; ; ++tile) {
             const bool more = tile < last || nb != b;
             const int32_t* table = a.table + (size_t) (tile < last ? b : nb) * a.width;
