@@ -19,6 +19,8 @@ template <> struct PagedRange<EXL_PAGE_INT8> { static constexpr int lo = -24, hi
 #ifdef __HIPCC__
 typedef f16x4 f16x4_a4 __attribute__((aligned(4)));       // head_dim % 8 != 0: rows of a head are only 4- or 8-byte aligned
 typedef f16x8 f16x8_a8 __attribute__((aligned(8)));
+typedef f16x4 f16x4_a2 __attribute__((aligned(2)));       // sin and cos may begin anywhere
+typedef f16x8 f16x8_a2 __attribute__((aligned(2)));
 
 __device__ __forceinline__ float paged_pow2(int e) { return __uint_as_float((uint32_t) (e + 127) << 23); }
 

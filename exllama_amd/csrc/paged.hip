@@ -415,8 +415,8 @@ __device__ __forceinline__ void append_run_wide(const AppendArgs& a, int h, int 
     for (int p = 0; p < P; ++p) {
         if (ROPE) {
             const size_t to = (size_t) min(max(pos[p], 0), a.angle_rows - 1) * a.hd + 8 * j;
-            const f16x8 sl = *(const f16x8_a8*) (a.sin + to), sh = *(const f16x8_a8*) (a.sin + to + half);
-            const f16x8 cl = *(const f16x8_a8*) (a.cos + to), ch = *(const f16x8_a8*) (a.cos + to + half);
+            const f16x8 sl = *(const f16x8_a2*) (a.sin + to), sh = *(const f16x8_a2*) (a.sin + to + half);
+            const f16x8 cl = *(const f16x8_a2*) (a.cos + to), ch = *(const f16x8_a2*) (a.cos + to + half);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 k[p][e] = rot_code(lo[p][e], cl[e], hi[p][e], sl[e], -1.f);

@@ -133,7 +133,7 @@ __device__ __forceinline__ PaQuery pa_query(const PagedAttn& a, const f16* q, in
     if (a.hd % 16 == 0) {
         r.hi = *(const f16x8_a8*) (q + d);
         if (sin) {
-            const f16x8 x = r.hi, o = *(const f16x8_a8*) (q + (d < half ? d + half : d - half)), s = *(const f16x8_a8*) (sin + d), c = *(const f16x8_a8*) (cos + d);
+            const f16x8 x = r.hi, o = *(const f16x8_a8*) (q + (d < half ? d + half : d - half)), s = *(const f16x8_a2*) (sin + d), c = *(const f16x8_a2*) (cos + d);
             const float sign = d < half ? -1.f : 1.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) put(i, fmaf((float) x[i], (float) c[i], sign * (float) o[i] * (float) s[i]));
@@ -147,8 +147,8 @@ __device__ __forceinline__ PaQuery pa_query(const PagedAttn& a, const f16* q, in
         const f16x4 x = *(const f16x4_a4*) (q + e);
         f16x4 o = {}, si = {}, co = {};
         if (sin) {
-            si = *(const f16x4_a4*) (sin + e);
-            co = *(const f16x4_a4*) (cos + e);
+            si = *(const f16x4_a2*) (sin + e);
+            co = *(const f16x4_a2*) (cos + e);
             if (e + 4 <= half || e >= half) o = *(const f16x4_a4*) (q + (e < half ? e + half : e - half));
             else for (int i = 0; i < 4; ++i) o[i] = q[e + i < half ? e + i + half : e + i - half];
         }

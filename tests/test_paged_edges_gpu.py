@@ -305,3 +305,25 @@ def test_lengths_that_advance_by_what_was_placed(ext):
         dry.past = np.where(new < 0, 0, dry.past + placed).astype(np.int32)
         assert d["past"].tolist() == dry.past.tolist()
     assert dry.past.max() == 44
+
+
+# ---- tensors at other addresses -------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("hd", [128, 100])
+def test_angles_that_begin_anywhere(ext, hd):
+    """sin and cos tables at an odd element of a buffer: the same results to the bit."""
+    rng = np.random.default_rng(hd)
+    host, dev = _attention_case(rng, "fp8", hd, 4, 2, 16, [(70, 3), (5, 20)])
+    x = [torch.from_numpy(rng.normal(0, 1, (23, 2 * hd)).astype(np.float16)).to(DEV) for _ in range(2)]
+    slots = _dev(np.r_[np.arange(3) + 5, np.arange(20) + 32])
+    results = []
+    for at in (0, 1, 3):
+        sin, cos = (torch.cat((t.new_zeros(at), t.flatten()))[at:].view(t.shape) for t in (dev["sin"], dev["cos"]))
+        assert sin.data_ptr() % 16 == 2 * at
+        pool = [p.clone() for p in dev["pool"]]
+        ext.ext_paged_append(*x, slots, *pool, positions=_dev(np.r_[np.arange(3) + 70, np.arange(20) + 5]), sin=sin, cos=cos)
+        out = ext.ext_paged_attention(dev["q"], dev["starts"], dev["past"], dev["new"], dev["table"], *dev["pool"], 4, max_new=20, sin=sin, cos=cos)
+        one = ext.ext_paged_attention(dev["q"], dev["starts"], dev["past"], _dev([3, 1]), dev["table"], *dev["pool"], 4, max_new=3, sin=sin, cos=cos)
+        results.append([out, one] + [p.view(torch.uint8) for p in pool])
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
