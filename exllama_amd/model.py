@@ -928,7 +928,8 @@ class ExLlama:
             cache.begin(new, end - begin)
             hidden = self.forward_layers(self.embed(input_ids[:, begin:end]), cache, None, lora)
             cache.end(new)
-            self._count_path("ops_general")
+            if q_len == 1:
+                self._count_path("ops_general")
             if preprocess_only:
                 continue
             if not last_id_only:
@@ -1010,7 +1011,7 @@ class ExLlama:
         "layer_call": "batch 2 .. 256, one token each: ONE native call per layer (exl_q4_layer_prompt: the short-prompt launches on "
                       "fragment-order activations, csrc/q4_gemm_frag.hip) -- no adapter, bias, mask or tensor-parallel shard",
         "ops_general": "op by op, general path: norm, q/k/v projections, RoPE, cache update, attention, o_proj, norm, gate/up, SiLU, down "
-                       "(batched generation, fused_attn off, or a tensor-parallel shard outside the executor; <= fused_mlp_thd rows still "
+                       "(batched generation, fused_attn off, an ExLlamaPagedCache, or a tensor-parallel shard outside the executor; <= fused_mlp_thd rows still "
                        "take q4_mlp for the MLP half, as in the reference)",
     }
 
@@ -1068,9 +1069,12 @@ class ExLlama:
         bsz = batch_size if batch_size is not None else (cache.batch_size if cache is not None else 1)
         on_executor = (st is not None and (cache is None or cache is st["cache"]) and bsz == 1 and lora is st.get("lora")
                        and st["has_embed"] and st["has_head"])
-        tier = self._executor_tier(st) if on_executor else self._op_tier(bsz, lora)
+        paged = isinstance(cache, ExLlamaPagedCache)
+        tier = self._executor_tier(st) if on_executor else "ops_general" if paged else self._op_tier(bsz, lora)
         why = []
-        if not on_executor:
+        if paged:
+            why = ["an ExLlamaPagedCache runs op by op: the executor, the fused attention ops and the per-layer call keep an fp16 ExLlamaCache"]
+        elif not on_executor:
             obstacles = self.executor_obstacles(bsz, lora)
             if obstacles:
                 why = obstacles

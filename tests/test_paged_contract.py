@@ -45,3 +45,27 @@ def test_attention_refuses_tables_at_the_end_of_32_bits(ext):
             most = (2 ** 31 - 65) // block
             assert "workspace" in attention(most, block, rows)
             assert "block table" in attention(most + 1, block, rows), block
+
+
+# ---- the model's side ---------------------------------------------------------------------------------------------------------------------
+
+def _bare_cache(batch_size=1):
+    from exllama_amd.model import ExLlamaPagedCache
+    cache = object.__new__(ExLlamaPagedCache)                 # (no device here: what is asked of it below needs none of its tensors)
+    cache.batch_size, cache.step = batch_size, {}
+    return cache
+
+
+@pytest.mark.parametrize("batch_size", [1, 8])
+def test_the_decode_report_names_the_path_of_a_paged_cache(batch_size):
+    import types
+
+    from exllama_amd.model import ExLlama
+    model = object.__new__(ExLlama)
+    model._decoder, model.layers = None, []
+    model.config = types.SimpleNamespace(tp=None, fused_attn=True, head_dim=128, hidden_size=4096, intermediate_size=11008,
+                                         device_map=types.SimpleNamespace(layers=["cuda:0"]))
+    report = model.decode_path_report(_bare_cache(batch_size))
+    assert report["tier"] == "ops_general" and len(report["why_not_faster"]) == 1 and "ExLlamaPagedCache" in report["why_not_faster"][0]
+    other = types.SimpleNamespace(batch_size=batch_size)      # any other cache is answered as before
+    assert model.decode_path_report(other)["tier"] == ("ops_fused" if batch_size == 1 else "layer_call")
