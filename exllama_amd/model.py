@@ -398,8 +398,11 @@ class ExLlamaAttention:
         """The general path over an ExLlamaPagedCache: hidden += o_proj(attention over the pages), keys rotated and quantised by the append, queries
         rotated by the attention kernel (each row of the batch at its own position)."""
         cfg = self.config
+        step = cache.step.get(str(hidden.device))
+        if step is None:
+            raise RuntimeError("an ExLlamaPagedCache is used through ExLlama.forward, which prepares its pages for the pass")
+        pages = cache.pages[self.index]
         q, k, v = (p.forward(normed, lora).view(-1, p.out_features) for p in (self.q_proj, self.k_proj, self.v_proj))
-        step, pages = cache.step[str(hidden.device)], cache.pages[self.index]
         cuda_ext.ext_paged_append(k, v, step.slots, *pages, positions=step.positions, sin=self.sin, cos=self.cos)
         attn = torch.zeros_like(q) if step.padded else torch.empty_like(q)            # (rows of padding are not written)
         cuda_ext.ext_paged_attention(q, step.starts, step.past, step.new, step.table, *pages, cfg.num_attention_heads, max_new=step.max_new, sin=self.sin,
@@ -544,7 +547,9 @@ class ExLlamaPagedCache:
     Pages of `block_size` tokens (16, 32, 64 or 128) come from one pool of `num_blocks` (default: enough for every row to reach max_seq_len; fewer
     serve rows that are not all long at once) and hold e4m3 or int8 codes with one power-of-two scale for each page and head: half the
     memory of ExLlamaCache for the same tokens.  `ExLlama.forward(ids, cache, row_lens=[...])` takes right-padded rows; `release(row)`
-    gives a row's pages back.  `seq_lens` are the rows' lengths; `current_seq_len` is the longest of them, and setting it sets all rows."""
+    gives a row's pages back.  `seq_lens` are the rows' lengths; `current_seq_len` is the longest of them, and setting it sets all rows.
+    What ExLlamaCache does to single columns of its tensors (roll_left, copy_states) pages under one scale cannot do exactly: both refuse, and so does
+    clone."""
 
     class _Step:
         """What one forward pass needs on one device: token rows' starts, slots and positions (ext_paged_slots), lengths and table."""
@@ -556,6 +561,10 @@ class ExLlamaPagedCache:
             raise RuntimeError("ExLlamaPagedCache: tensor-parallel shards are not supported")
         if dtype not in cuda_ext.PAGE_CODES:
             raise RuntimeError("ExLlamaPagedCache: dtype must be torch.float8_e4m3fn or torch.int8")
+        if block_size not in (16, 32, 64, 128):
+            raise RuntimeError("ExLlamaPagedCache: block_size must be 16, 32, 64 or 128")
+        if batch_size < 1 or (num_blocks is not None and num_blocks < 1):
+            raise RuntimeError("ExLlamaPagedCache: at least one row and one block")
         self.model, self.config, self.batch_size, self.block_size, self.dtype = model, cfg, batch_size, block_size, dtype
         self.max_seq_len = max_seq_len if max_seq_len != -1 else cfg.max_seq_len
         if self.max_seq_len > cfg.max_seq_len:
@@ -647,6 +656,16 @@ class ExLlamaPagedCache:
     def zero(self):
         """Every row empty, every page back in the pool."""
         self.release(*range(self.batch_size))
+
+    def roll_left(self):
+        raise RuntimeError("ExLlamaPagedCache.roll_left: a page's tokens share a scale and cannot move by one; drop tokens from the end (set_seq_lens) or "
+                           "start the row anew (release)")
+
+    def copy_states(self, target, from_column, from_columns, to_column, to_columns, from_row, from_rows, to_row, to_rows):
+        raise RuntimeError("ExLlamaPagedCache.copy_states: a page's tokens share a scale and cannot be copied by columns; use an ExLlamaCache")
+
+    def clone(self):
+        raise RuntimeError("ExLlamaPagedCache.clone: not supported; use an ExLlamaCache")
 
 
 class ExLlamaBuffer:

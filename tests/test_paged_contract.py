@@ -69,3 +69,22 @@ def test_the_decode_report_names_the_path_of_a_paged_cache(batch_size):
     assert report["tier"] == "ops_general" and len(report["why_not_faster"]) == 1 and "ExLlamaPagedCache" in report["why_not_faster"][0]
     other = types.SimpleNamespace(batch_size=batch_size)      # any other cache is answered as before
     assert model.decode_path_report(other)["tier"] == ("ops_fused" if batch_size == 1 else "layer_call")
+
+
+def test_what_a_paged_cache_cannot_do_it_refuses_with_a_message():
+    cache = _bare_cache()
+    for call in (cache.roll_left, cache.clone, lambda: cache.copy_states(cache, 0, 1, 0, 1, 0, 1, 0, 1)):
+        with pytest.raises(RuntimeError, match="ExLlamaPagedCache"):
+            call()
+
+
+@pytest.mark.parametrize("kw,match", [({"block_size": 24}, "block_size"), ({"block_size": 256}, "block_size"), ({"num_blocks": 0}, "one block"),
+                                      ({"num_blocks": -3}, "one block"), ({"batch_size": 0}, "one row"), ({"dtype": torch.float16}, "dtype")])
+def test_a_paged_cache_that_cannot_work_is_refused_before_it_takes_memory(kw, match):
+    import types
+
+    from exllama_amd.model import ExLlamaPagedCache
+    config = types.SimpleNamespace(tp=None, max_seq_len=64, head_dim=64, num_hidden_layers=1, num_key_value_heads=1,
+                                   device_map=types.SimpleNamespace(layers=["meta"]))
+    with pytest.raises(RuntimeError, match=match):
+        ExLlamaPagedCache(types.SimpleNamespace(config=config), **kw)
