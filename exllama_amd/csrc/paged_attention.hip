@@ -558,8 +558,8 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const
 // s * c1, rounded, and how far it lies above ref
 __device__ __forceinline__ float pa_above(float s, float c1, float ref)
 {
-    float x = s * c1;
-    asm("" : "+v"(x));                                            // (not contracted)
+#pragma clang fp contract(off)
+    const float x = s * c1;
     return x - ref;
 }
 
@@ -863,7 +863,9 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
             m = mn;
         }
         float ref = m == -INFINITY ? 0.f : m;
-        if (__any(fabsf(ref) > 0x1p22f)) {                        // scores so large that one fma and a product with a difference disagree by more than 2^-2: as mx was
+        // Scores so large that one fma and a product with a difference disagree by more than 2^-2: rounded as mx was.  (Wide heads always: a branch here
+        // made the compiler copy sums in every tile.)
+        if (DP <= 128 && __any(fabsf(ref) > 0x1p22f)) {
             const float back = 1.f / c1;
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
@@ -877,7 +879,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_m
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[kt][j], c1, -ref));
+                const float e = __builtin_amdgcn_exp2f(DP > 128 ? pa_above(s[kt][j], c1, ref) : fmaf(s[kt][j], c1, -ref));
                 sum += e;
                 p[kt][j >> 3][j & 7] = (f16) e;
             }
