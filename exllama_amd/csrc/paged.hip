@@ -101,7 +101,7 @@ template <int R> __device__ __forceinline__ void slot_scan_rows(const SlotArgs& 
             const int end = (int) min((int64_t) past[i] + take[i], (int64_t) a.max_len);
             const int need = (int) (((int64_t) end + (1 << a.lbs) - 1) >> a.lbs);
             want[i] = first + i < a.n && fresh[i] >= 0 ? max(0, need - held[i]) : 0;
-            lost[i] = (fresh[i] > 0 || held[i] > 0) && (int64_t) past[i] > (int64_t) held[i] << a.lbs ? want[i] : 0;
+            lost[i] = (fresh[i] > 0 || held[i] > 0) && (past[i] - 1) >> a.lbs >= held[i] ? want[i] : 0;
             want[i] -= lost[i];
             back[i] = fresh[i] < 0 ? held[i] : 0;
             mine += (int64_t) want[i] << 32 | back[i];
