@@ -13,7 +13,7 @@
 // Then every token row's slot = table[pos / block] * block + pos % block.  Latency is all that matters (a step of 256 rows moves
 // 7 KB): one workgroup does both halves where the work is small, otherwise the scan runs in one workgroup and the filling in
 // many -- a second launch instead of a grid-wide wait.  Measured, us, one workgroup / scan + filling and
-// another launch: one row 3.0 / 2.8 + 1.6, 64 rows of 64 tokens 3.9 / 3.4 + 3.1, 256 rows 7.0 / 3.5 + 2.5, 512 rows (the limit) 9.2 / 5.2 + 3.5;
+// another launch: one row 3.0 / 2.8 + 1.6, 64 rows of 64 tokens 3.9 / 3.4 + 3.1, 256 rows 7.2 / 3.5 + 2.5, 512 rows (the limit) 9.2 / 5.2 + 3.5;
 // 2048 prompts of 300 k tokens 8.1 + 5.5 (2.4 MB of slots and positions).
 struct SlotRow { int start, take, past, kept, held, base, back, gone; };      // 32 bytes a row
 
@@ -488,7 +488,8 @@ __device__ __forceinline__ void append_run_wide(const AppendArgs& a, int h, int 
 // One workgroup = `chunk` (at most 63) token rows of one head: it does the runs that begin there.  The chunk's slots and the page that may follow
 // (at most 63 + 127 of them, and the one before) are read in one round of loads, by one wave for all four (they have to agree on the runs whatever happens to the
 // slots meanwhile); a bit for each row says whether it continues the row before it.
-// P = 0: a wave for every run.
+// P = 0, head_dim no multiple of 16: a wave for every run, its codes stored byte by byte, however long: a prompt of 2048 x 32 heads of 100 takes
+// 127 us, of 112 19.5 (single tokens, 64 x 32 heads: 7.6 and 8.2).
 template <int CODE, bool ROPE, int P> __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];

@@ -37,7 +37,7 @@ __device__ __forceinline__ PaRow pa_row(const PagedAttn& a, int b)
 // A wave does all queries of its row that read the kv head (up to 16 * NT: tokens * heads of the group, GQA reads the cache once).  A row
 // that lies in one stretch is written; the others leave one partial result for each stretch, joined in order by a second kernel -- the cut
 // depends on the lengths alone, so results do not depend on scheduling.
-// Bound by HBM: 8 rows of 65536 keys x 8 kv heads x 128 (1.07 GB) 201 us = 5.3 TB/s, 96 rows of 0 .. 16384 (434 MB) 93 us = 4.7 TB/s; one row of 2048 keys
+// Bound by HBM: 8 rows of 65536 keys x 8 kv heads x 128 (1.07 GB) 199 us = 5.4 TB/s, 96 rows of 0 .. 16384 (434 MB) 93 us = 4.7 TB/s; one row of 2048 keys
 // x 32 heads (16.8 MB) is latency: 9 us, and 4 us for the joining kernel.
 // PA_BEGIN, measured 0 / 2 / 4: 96 ragged rows 134 / 104 / 105 us, five rows of four tokens 22 / 17 / 16, 96 equal rows 99 / 99 / 103.
 // Both products are MFMAs on fp16 numbers converted from the codes in registers; nothing goes through LDS:
@@ -549,10 +549,11 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, const
 //   S^T = K Q^T (32x32x16): row m of the product is key 16 * ((m >> 2) & 1) + 4 * (m >> 3) + (m & 3) of a half tile, so that a lane (query
 //   column c = lane & 31, group g = lane >> 5) gets keys 16 g .. 16 g + 15 in order;   O^T = V^T P^T: the lane's own weights are the operand.
 // LDS pieces of 16 bytes are laid out by XOR so that neither the writes (one key, all columns) nor the reads (linear) meet in a bank.
-// Bound by the sum of MFMA and VALU time (conversion, exp2, masks), which two workgroups a compute unit do not hide behind each other.
+// Bound by the sum of MFMA and VALU time (conversion, exp2, masks), which two workgroups a compute unit do not hide behind each other (pieces of a 70B
+// prompt: 48 % and 54 % of the cycles).
 // LOW, head_dim up to 128: the rest of a rotated query is multiplied too -- half as many MFMAs again: a prompt of 2048 x 32 heads (34 GFLOP causal)
-// takes 77 us instead of 66, pieces of a 70B prompt (411 GFLOP) 622 instead of 503; without it the result is 3.9e-4 of its norm off, with it
-// 2.6e-4 (2.0e-4 are its own rounding).  Wider heads have no registers for it (spilled: 127 -> 213 us).
+// takes 86 us instead of 76, pieces of a 70B prompt (410 GFLOP) 634 instead of 523 (in turn on one GPU); without it the result is 3.8e-4 of its norm
+// off, with it 2.65e-4 (2.05e-4 are its own rounding).  Wider heads have no registers for it (spilled: 127 -> 213 us).
 #define PM_ROWS 128
 
 // s * c1, rounded, and how far it lies above ref

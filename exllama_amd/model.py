@@ -859,7 +859,8 @@ class ExLlama:
         """Same contract as the reference (model.py:924-986): chunks long inputs by max_input_len, returns
         fp32 logits [bsz, 1 or q_len, vocab] on `output_device` (default: input_ids' device), or None.
         `row_lens` (an ExLlamaPagedCache only; default: q_len for every row): the tokens of each right-padded row that count, 0 for a row that
-        sits this pass out.  With last_id_only the logits are those of each row's last token (a row of none: its first padding's)."""
+        sits this pass out.  With last_id_only the logits are those of each row's last token (a row of none: its first padding's).  Padding is
+        neither stored nor attended to, but it runs through the projections: rows of very different lengths cost as much as the longest of them each."""
         if isinstance(cache, ExLlamaPagedCache):
             return self._forward_paged(input_ids, cache, last_id_only, preprocess_only, lora, output_device, input_mask, row_lens)
         if row_lens is not None:
