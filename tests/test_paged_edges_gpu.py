@@ -227,7 +227,7 @@ def test_append_of_every_chunk(ext, code, hd, kvh, block, spec):
 class _Dry:
     """Three rows on a pool of six pages of 16 that hold another sequence's leavings, NaN among them."""
 
-    def __init__(self, rng, new_rows=3):
+    def __init__(self, rng):
         self.rng, self.hd, self.kvh, self.heads, self.block = rng, 64, 2, 4, 16
         codes = P.nearest(rng.normal(0, 100, (6, 2, 16, 64)), "fp8"), P.nearest(rng.normal(0, 100, (6, 2, 64, 16)), "fp8")
         for c in codes:
