@@ -178,14 +178,16 @@ def test_every_key_counts_once(ext, code, equal, hd, heads, kvh, block, lens):
         assert (np.abs(x - want[:, None]) <= tol * want[:, None] + 2.0 ** -25).all(), (b, past, new)
 
 
+@pytest.mark.parametrize("code", ["fp8", "int8"])
 @pytest.mark.parametrize("hd,heads,kvh,block,lens,spread,bites", [
     (128, 4, 2, 16, [(60, 8), (5, 3)], 8, True), (128, 4, 2, 64, [(10, 40)], 8, True), (128, 4, 2, 64, [(100, 40)], 32, True), (64, 4, 2, 32, [(10, 40)], 8, True),
     (100, 4, 2, 16, [(10, 40)], 16, True), (100, 4, 4, 16, [(20, 6), (9, 1)], 16, True), (256, 2, 2, 64, [(10, 7)], 4, False), (256, 4, 2, 64, [(200, 40)], 2, False),
     (128, 8, 1, 64, [(6000, 20)], 2, False), (128, 4, 4, 64, [(9000, 1)], 2, False), (128, 16, 2, 32, [(5000, 1), (100, 1), (2000, 1)], 2, False)])
-def test_a_rotated_query_keeps_what_fp16_leaves(ext, hd, heads, kvh, block, lens, spread, bites):
+def test_a_rotated_query_keeps_what_fp16_leaves(ext, code, hd, heads, kvh, block, lens, spread, bites):
     """Against the bound of a kernel that holds a rotated query to 22 bits.  `bites`: the formula with the rotated query rounded to fp16 breaks that bound, so
     that a kernel which drops the rest fails."""
-    host, dev = _attention_case(np.random.default_rng(1), "fp8", hd, heads, kvh, block, lens, spread=spread)
+    spread *= 1 if code == "fp8" else 3                       # (int8 codes are a third as large)
+    host, dev = _attention_case(np.random.default_rng(1), code, hd, heads, kvh, block, lens, spread=spread)
     want, bound = _sharp(host, _rest(hd, heads, kvh, int(host["new"].max())))
     some = ~np.isnan(bound)
     if bites:
@@ -305,6 +307,38 @@ def test_lengths_that_advance_by_what_was_placed(ext):
         dry.past = np.where(new < 0, 0, dry.past + placed).astype(np.int32)
         assert d["past"].tolist() == dry.past.tolist()
     assert dry.past.max() == 44
+
+
+@pytest.mark.parametrize("n,rows,stride", [(3, 40, 0), (64, 300, 0), (65, 300, 0), (300, 1000, 0), (512, 4096, 0), (513, 2000, 0), (300, 5000, 0), (2100, 9000, 0),
+                                           (5000, 20000, 0), (300, 300 * 4, 4), (700, 700 * 4, 4)])
+def test_slots_of_rows_that_lost_tokens(ext, n, rows, stride):
+    """Lengths beyond the held blocks in a third of the rows, among ended, idle and ordinary ones: in one workgroup's wave, in all of its waves, and in the scan
+    of its own launch, once around and twice."""
+    for seed in range(3):
+        rng = np.random.default_rng(seed)
+        width, block, spare = 9, 16, 2 * n
+        held = rng.integers(0, 7, n).astype(np.int32)
+        past = np.maximum(held * block - rng.integers(0, block, n), 0)
+        past = np.where(rng.random(n) < 0.3, held * block + rng.integers(1, 40, n), past)
+        new = rng.integers(0, 5, n)
+        new[rng.random(n) < 0.2] = 0
+        new[rng.random(n) < 0.1] = -1
+        blocks = int(held.sum()) + spare
+        order = rng.permutation(blocks)
+        table, at = np.full((n, width), -1, np.int32), 0
+        for b in range(n):
+            table[b, :held[b]] = order[at:at + held[b]]
+            at += held[b]
+        head = int(rng.integers(blocks))
+        ring = np.full(blocks, -7, np.int32)
+        ring[(head + np.arange(spare)) % blocks] = order[at:]
+        counters = np.array([head, spare, 0, 0], np.int32)
+        d = [_dev(x) for x in (past, new, held, table, ring, counters)]
+        got = ext.ext_paged_slots(*d, block, rows, max_new=4, row_stride=stride)
+        want = P.slots(past, new, held, table, ring, counters, block, width * block, 4, rows, stride)
+        for name, x, y in zip(("starts", "slots", "positions", "held", "table", "ring", "counters"), (*got, *d[2:]), (*want, held, table, ring, counters)):
+            assert np.array_equal(x.cpu().numpy(), y), (name, seed)
+        assert n < 60 or counters[2] > 0
 
 
 # ---- tensors at other addresses -------------------------------------------------------------------------------------------------------------
