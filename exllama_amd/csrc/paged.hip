@@ -61,7 +61,8 @@ template <int R> __device__ __forceinline__ void slot_scan_rows(const SlotArgs& 
     __shared__ unsigned long long lacking;                        // blocks that rows without their earlier tokens' lack
     const bool one_wave = a.n <= 64 * R;
     if (one_wave && threadIdx.x >= 64) return;
-    if (threadIdx.x == 0) lacking = 0;                            // (a scan's barrier, or the wave's order, stands between this and the first sum)
+    if (threadIdx.x == 0) lacking = 0;                            // (a scan's barrier, or in one wave this fence, stands between this and the first sum)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const int head = (int) ((uint32_t) a.counters[0] % (uint32_t) a.blocks);
     const int avail = min(max(a.counters[1], 0), a.blocks);
     int64_t rows_before = 0, want_before = 0, back_before = 0;
@@ -128,7 +129,8 @@ template <int R> __device__ __forceinline__ void slot_scan_rows(const SlotArgs& 
             back_base += back[i];
         }
     }
-    if (!one_wave) __syncthreads();                               // every thread has read the counters
+    if (!one_wave) __syncthreads();                               // every thread has read the counters, and added what its rows lack
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (threadIdx.x == 0) {
         const int got = (int) min(want_before, (int64_t) avail);
         a.counters[0] = (head + got) % a.blocks;
